@@ -148,6 +148,128 @@ def _sym(kind, action):
     return "tqt_%s_%s_%s" % (action, name, VARIANT)
 
 
+class RopeMap(ctypes.Structure):
+    """struct tqt_rope_map (include/tqt_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("table", c_vp),
+        ("max_pos", c_size),
+        ("rotary_dim", c_size),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+    ]
+
+
+class RopeParams(ctypes.Structure):
+    """struct tqt_rope_params (include/tqt_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("tokens", c_size),
+        ("heads", c_size),
+        ("head_dim", c_size),
+        ("X", c_vp),
+        ("x_token_stride", c_size),
+        ("x_head_stride", c_size),
+        ("Y", c_vp),
+        ("y_token_stride", c_size),
+        ("y_head_stride", c_size),
+        ("positions", c_vp),
+        ("map", RopeMap),
+    ]
+
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP, ROPE_TURNS = range(5)
+
+
+class RopeTableParams(ctypes.Structure):
+    """struct tqt_rope_table_params (include/tqt_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("table", c_vp),
+        ("max_pos", c_size),
+        ("rotary_dim", c_size),
+        ("scaling", ctypes.c_int32),
+        ("base", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("original_max_pos", ctypes.c_double),
+        ("low_turns", ctypes.c_double),
+        ("high_turns", ctypes.c_double),
+        ("amplitude", ctypes.c_double),
+    ]
+
+
+class PagedKV(ctypes.Structure):
+    """struct tqt_paged_kv (include/tqt_kv_append_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("k", c_vp),
+        ("v", c_vp),
+        ("scale_k", c_vp),
+        ("scale_v", c_vp),
+        ("num_pages", c_size),
+        ("page_size", c_size),
+        ("kv_heads", c_size),
+        ("head_dim", c_size),
+        ("page_stride", c_size),
+        ("token_stride", c_size),
+        ("head_stride", c_size),
+    ]
+
+
+class KVAppendRopeParams(ctypes.Structure):
+    """struct tqt_kv_append_rope_params (include/tqt_kv_append_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("tokens", c_size),
+        ("K", c_vp),
+        ("k_token_stride", c_size),
+        ("k_head_stride", c_size),
+        ("V", c_vp),
+        ("v_token_stride", c_size),
+        ("v_head_stride", c_size),
+        ("q_heads", c_size),
+        ("Q", c_vp),
+        ("q_token_stride", c_size),
+        ("q_head_stride", c_size),
+        ("Q_out", c_vp),
+        ("qo_token_stride", c_size),
+        ("qo_head_stride", c_size),
+        ("positions", c_vp),
+        ("slots", c_vp),
+        ("map", RopeMap),
+        ("kv", PagedKV),
+    ]
+
+
+class AttnPagedParams(ctypes.Structure):
+    """struct tqt_attn_paged_params (include/tqt_attn_paged_gfx950.h)."""
+
+    _fields_ = [
+        ("batch", c_size),
+        ("q_tokens", c_size),
+        ("q_heads", c_size),
+        ("max_q_len", c_size),
+        ("max_kv_len", c_size),
+        ("Q", c_vp),
+        ("q_token_stride", c_size),
+        ("q_head_stride", c_size),
+        ("D", c_vp),
+        ("d_token_stride", c_size),
+        ("d_head_stride", c_size),
+        ("lse", c_vp),
+        ("q_start", c_vp),
+        ("kv_len", c_vp),
+        ("block_table", c_vp),
+        ("ld_table", c_size),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("window", c_size),
+        ("kv", PagedKV),
+        ("workspace", c_vp),
+        ("workspace_size", c_size),
+    ]
+
+
 # C type (as written in include/*.h, parameter name dropped) -> ctypes type.
 _CTYPES = {
     "size_t": c_size,
@@ -167,6 +289,10 @@ _CTYPES = {
     "const struct tqt_qai8dx_qsi4cx_params *": ctypes.POINTER(QAI8DXQSI4CXParams),
     "const struct tqt_qai8dxp_qsi8cxp_params *": ctypes.POINTER(QAI8DXPQSI8CXPParams),
     "const struct tqt_qai8_qsi8dx_qai8_params *": ctypes.POINTER(QAI8QSI8DXQAI8Params),
+    "const struct tqt_rope_params *": ctypes.POINTER(RopeParams),
+    "const struct tqt_rope_table_params *": ctypes.POINTER(RopeTableParams),
+    "const struct tqt_kv_append_rope_params *": ctypes.POINTER(KVAppendRopeParams),
+    "const struct tqt_attn_paged_params *": ctypes.POINTER(AttnPagedParams),
 }
 # f16 / bf16 values are passed in SSE registers on x86-64, which ctypes cannot fill: functions
 # taking them are checked for export but not bound (the test shim in tests/abi_shim calls them).
@@ -225,6 +351,13 @@ class Lib:
 
     def fn(self, kind, action):
         return self._fns[_sym(kind, action)]
+
+    def op(self, name, action):
+        """An operator that is no GEMM or convolution type: ``op("rope_f16", "run_async")``,
+        ``op("attn_paged", "get_workspace_size")``, ``op("attn_paged_f16_f16", "get_error")``."""
+        tail = "_async" if action.endswith("_async") else ""
+        action = action[:len(action) - len(tail)]
+        return self._fns["tqt_%s_%s_gfx950%s" % (action, name, tail)]
 
     def symbol_names(self):
         return sorted(self._decls)
