@@ -1,11 +1,20 @@
-// What the attention kernels over a paged cache share: a call's arguments and how a sequence is found.
+// What the attention kernels over a paged cache share: a call's arguments, how a sequence and a key are
+// found, the matrix instructions and conversions of the two 16-bit types.
 #pragma once
 
+#include <type_traits>
+
+#include "attn_route.hpp"
 #include "fast_div.hpp"
 #include "paged_kv.hpp"
 #include "tqt_hip_common.hpp"
 
 namespace tqt {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct AttnArgs
 {
@@ -21,8 +30,14 @@ struct AttnArgs
     int num_pages;
     FastDiv page, group;  // group: query heads per key head
     int batch, q_tokens, q_heads, kv_heads, head_dim, max_q_len, max_kv_len;
-    float scale;
+    // Scores are q . k times `scale` > 0, which holds log2(e) too; `sign` (-1, 0 or 1, times Q) is the
+    // sign of the caller's scale.
+    float scale, sign;
     int causal, window;  // window 0: none
+    // the split of the keys over workgroups: spans of so many keys, joined from the workspace's f32 sums
+    int few_chunk;
+    float *part_o;   // [splits][q_tokens * q_heads][head_dim], not divided by the sum
+    float *part_ml;  // [splits][q_tokens * q_heads][2]: maximum (log2) and sum
 };
 
 // A sequence of the batch, with every length brought inside what the host checked.
@@ -30,6 +45,7 @@ struct AttnSeq
 {
     int first;   // its first row of Q
     int q_len, kv_len;
+    int nq;      // queries that are computed
     int pos0;    // position of query 0 (negative: the first queries see nothing)
 };
 
@@ -40,6 +56,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b)
     const int end = min(max(a.q_start[b + 1], s.first), a.q_tokens);
     s.q_len = end - s.first;
     s.kv_len = min(max(a.kv_len[b], 0), a.max_kv_len);
+    s.nq = min(s.q_len, a.max_q_len);
     s.pos0 = s.kv_len - s.q_len;
     return s;
 }
@@ -47,8 +64,200 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b)
 // The keys [lo, hi) that the query at `pos` may see.
 __device__ __forceinline__ void attn_bounds(const AttnArgs &a, const AttnSeq &s, int pos, int &lo, int &hi)
 {
-    hi = a.causal ? min(pos + 1, s.kv_len) : s.kv_len;
+    hi = a.causal ? min(max(pos + 1, 0), s.kv_len) : s.kv_len;
     lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+}
+
+// Workgroups that share the keys [first, last) of some rows.
+__device__ __forceinline__ int attn_splits(int first, int last, int chunk)
+{
+    return max(1, (last - first + chunk - 1) / chunk);
+}
+
+// N elements of a row's sums from d0 on (d0 + N <= head_dim or d0 >= head_dim): the result where one
+// workgroup has all of its keys, else this split's part. sum == 0: no key, or scores of -infinity alone.
+template <typename T, int N>
+__device__ __forceinline__ void attn_put(const AttnArgs &a, int split, int splits, int token, int head, int d0,
+                                         const float (&acc)[N], float m, float sum)
+{
+    const long long row = static_cast<long long>(token) * a.q_heads + head;
+    if (splits > 1) {
+        const long long at = static_cast<long long>(split) * a.q_tokens * a.q_heads + row;
+        if (d0 < a.head_dim) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                *reinterpret_cast<f32x4 *>(a.part_o + at * a.head_dim + d0 + e) =
+                    f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            }
+        }
+        if (d0 == 0) {
+            a.part_ml[2 * at] = m;
+            a.part_ml[2 * at + 1] = sum;
+        }
+        return;
+    }
+    if (d0 < a.head_dim) {
+        typedef T out_vec __attribute__((ext_vector_type(N)));
+        out_vec y;
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            y[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[e] * inv);
+        }
+        *reinterpret_cast<out_vec *>(static_cast<T *>(a.d) + token * a.d_ts + head * a.d_hs + d0) = y;
+    }
+    if (a.lse != nullptr && d0 == 0) {
+        a.lse[row] = (m + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+    }
+}
+
+// Element offset of a key's row of one key head, or -1: past `hi`, or on no page of the cache.
+struct KeyRow
+{
+    long long at;
+    int page, offset;
+    bool kept;
+};
+
+__device__ __forceinline__ KeyRow attn_key(const AttnArgs &a, const int32_t *table, int head, int j, int hi)
+{
+    KeyRow r;
+    uint32_t offset;
+    const uint32_t pi = fast_div(static_cast<uint32_t>(j), a.page, offset);
+    r.page = j < hi ? table[pi] : -1;
+    r.offset = static_cast<int>(offset);
+    r.kept = r.page >= 0 && r.page < a.num_pages;
+    r.at = r.kept ? r.page * a.page_stride + r.offset * a.token_stride + head * a.head_stride : 0;
+    return r;
+}
+
+// 8 values of a 16-bit type as a matrix operand, and the two shapes of product used.
+template <typename T>
+struct Half8;
+template <>
+struct Half8<_Float16>
+{
+    typedef f16x8 type;
+};
+template <>
+struct Half8<__bf16>
+{
+    typedef bf16x8 type;
+};
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Four rows of a 16-bit matrix in LDS, read down a column: the 16 lanes of a group give the addresses of
+// 4 rows x 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and lane i receives column i.
+__device__ __forceinline__ u32x2 lds_read_column4(const void *p)
+{
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)p));
+}
+
+// Orders a wave's own LDS writes before other lanes' reads of them (a wave's LDS operations complete in
+// order; this holds the compiler to it).
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 16 int8 as 16-bit floats, exactly: [0] the first 8, [1] the others.
+__device__ __forceinline__ void int8_to_half(u32x4 x, f16x8 (&y)[2])
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // value + 128 in the low bits of 1024.0's significand, then less 1152
+        const uint32_t u = x[i] ^ 0x80808080u;
+        const f16x2 base = {1152.0f16, 1152.0f16};
+        w[2 * i] = __builtin_bit_cast(
+            uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - base);
+        w[2 * i + 1] = __builtin_bit_cast(
+            uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - base);
+    }
+    __builtin_memcpy(&y[0], w, 16);
+    __builtin_memcpy(&y[1], w + 4, 16);
+}
+
+__device__ __forceinline__ void int8_to_half(u32x4 x, bf16x8 (&y)[2])
+{
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f[j] = static_cast<float>(static_cast<int8_t>(x[i] >> (8 * j)));
+        }
+        // whole numbers of 8 bits: the upper halves of the f32 hold them
+        w[2 * i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[1]),
+                                         __builtin_bit_cast(uint32_t, f[0]), 0x07060302u);
+        w[2 * i + 1] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[3]),
+                                             __builtin_bit_cast(uint32_t, f[2]), 0x07060302u);
+    }
+    __builtin_memcpy(&y[0], w, 16);
+    __builtin_memcpy(&y[1], w + 4, 16);
+}
+
+// Whether any of 2 packed 16-bit values is an infinity or NaN (exponent bits all set).
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(uint32_t x)
+{
+    constexpr uint32_t mask = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
+    return (x & mask) == mask || ((x >> 16) & mask) == mask;
+}
+
+// Values that are no numbers, in a tile where some rows do not see some keys: 0 x infinity would reach
+// them through the matrix product. The product takes 0 in their place (`clean`), and a second one, of
+// `code` with 1 for every key a row sees, tells which of them each row meets: counts of +infinity,
+// -infinity and NaN in steps of 1, 64 and 4096, which 32 keys do not overflow.
+template <typename T>
+__device__ __forceinline__ void split_not_finite(u32x4 x, u32x4 &clean, u32x4 &code)
+{
+    constexpr bool f16 = std::is_same<T, _Float16>::value;
+    constexpr uint32_t mask = f16 ? 0x7c00u : 0x7f80u, mant = f16 ? 0x3ffu : 0x7fu;
+    constexpr uint32_t one = f16 ? 0x3c00u : 0x3f80u, c64 = f16 ? 0x5400u : 0x4280u,
+                       c4096 = f16 ? 0x6c00u : 0x4580u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        clean[i] = 0;
+        code[i] = 0;
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+            const uint32_t v = (x[i] >> h) & 0xffffu;
+            const bool bad = (v & mask) == mask;
+            clean[i] |= (bad ? 0u : v) << h;
+            code[i] |= (!bad ? 0u : (v & mant) ? c4096 : (v & 0x8000u) ? c64 : one) << h;
+        }
+    }
+}
+
+// What a row's sum becomes by the values that are no numbers it meets.
+__device__ __forceinline__ float not_finite_term(float count)
+{
+    const int n = static_cast<int>(count);
+    float t = 0.0f;
+    if (n >= 4096) {
+        t = __builtin_nanf("");
+    }
+    if ((n & 4095) >= 64) {
+        t -= INFINITY;
+    }
+    if ((n & 63) > 0) {
+        t += INFINITY;
+    }
+    return t;
 }
 
 }  // namespace tqt

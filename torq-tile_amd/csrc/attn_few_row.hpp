@@ -1,0 +1,336 @@
+// Attention of few rows: sequences with at most 16 rows to a key head (one decoded token of up to 16 query
+// heads, or a few tokens of fewer), over a span of the keys.
+//
+// Bound by the cache's bytes: per key 2 d elements are read once for 4 d 16 flops on the matrix cores. A
+// workgroup is four independent waves; wave w takes the 32-key tiles w, w + 4, ... of the span, with sums of
+// its own, and the four meet once at the end. No barrier in the loop. A tile's keys and values are in
+// registers one tile ahead of their use (16 KB a wave in flight at d 128).
+//
+// With the keys as the rows of the first product, S^T = K Q^T, each lane holds 4 + 4 keys of one query: the
+// softmax is 8 values in a lane and two exchanges, its statistics are one value a lane, and P^T is the second
+// operand of O^T = V^T P^T as it stands. K comes from memory in the operand's layout; V goes through a
+// wave's own LDS, which is read down its columns.
+#pragma once
+
+#include "attn_common.hpp"
+
+namespace tqt {
+namespace {
+
+// DP: head_dim rounded up to 64, 128 or 256.
+template <typename T, typename C, int DP>
+struct FewRowTile
+{
+    static constexpr bool kQuant = std::is_same<C, int8_t>::value;
+    static constexpr int kPieces = DP * static_cast<int>(sizeof(C)) / 64;  // 16-byte pieces of a row per lane
+    static constexpr int kStride = DP * 2 + 16;                           // bytes of a value row in LDS
+    static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 256 : 0);
+};
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(AttnArgs a)
+{
+    typedef FewRowTile<T, C, DP> Tile;
+    typedef typename Half8<T>::type half8;
+    constexpr bool kQuant = Tile::kQuant;
+    constexpr int kPieces = Tile::kPieces, kSteps = DP / 32, kStride = Tile::kStride;
+    constexpr int kElems = 16 / static_cast<int>(sizeof(C));  // elements of a piece
+    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::kWaveBytes];
+    __shared__ float s_m[4][16], s_l[4][16];
+
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int col = lane & 15, g = lane >> 4;
+    const AttnSeq s = attn_seq(a, b);
+    const int group = static_cast<int>(a.group.d);
+    const int rows = s.nq * group;
+    if (rows == 0 || rows > kAttnFewRows) {
+        return;
+    }
+    // the keys that any row sees
+    int first, last, unused;
+    attn_bounds(a, s, s.pos0, first, unused);
+    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
+    const int splits = attn_splits(first, last, a.few_chunk);
+    if (split >= splits) {
+        return;
+    }
+    const int lo = first + split * a.few_chunk, hi = min(last, lo + a.few_chunk);
+    const int32_t *table = a.table + b * a.ld_table;
+    const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
+    char *mine = lds + wave * Tile::kWaveBytes;
+
+    // this lane's row, and the keys that it sees
+    const bool live = col < rows;
+    uint32_t head_in_group;
+    const int token = static_cast<int>(fast_div(live ? col : 0, a.group, head_in_group));
+    const int head = kvh * group + static_cast<int>(head_in_group);
+    int row_lo, row_hi;
+    attn_bounds(a, s, s.pos0 + token, row_lo, row_hi);
+    if (!live) {
+        row_hi = 0;
+    }
+    // keys outside [all_lo, all_hi) are not seen by every row
+    int all_lo, all_hi;
+    attn_bounds(a, s, s.pos0, unused, all_hi);
+    attn_bounds(a, s, s.pos0 + s.nq - 1, all_lo, unused);
+
+    // Q^T: the elements that the pieces of K bring in the same steps
+    half8 q[kSteps];
+    const T *qp = static_cast<const T *>(a.q) + (s.first + token) * a.q_ts + head * a.q_hs;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const int d0 = kQuant ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+        half8 x = {};
+        if (live && d0 < a.head_dim) {
+            x = *reinterpret_cast<const half8 *>(qp + d0);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = static_cast<T>(static_cast<float>(x[e]) * a.sign);
+        }
+        q[i] = x;
+    }
+
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        o[i] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    float vmax = 0x1p-100f;  // int8: what the sums o are in units of
+
+    u32x4 kx[2][kPieces], vx[2][kPieces];
+    float sk = 0.0f, sv = 0.0f;  // int8: the scales of key lane % 32
+    bool kept[2];
+    auto fetch = [&](int j0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const KeyRow r = attn_key(a, table, kvh, j0 + 16 * t + col, hi);
+            kept[t] = r.kept;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int d0 = (4 * i + g) * kElems;
+                u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                if (r.kept && d0 < a.head_dim) {
+                    x = *reinterpret_cast<const u32x4 *>(kbase + r.at + d0);
+                    y = *reinterpret_cast<const u32x4 *>(vbase + r.at + d0);
+                }
+                kx[t][i] = x;
+                vx[t][i] = y;
+            }
+            if constexpr (kQuant) {
+                if (t == ((lane >> 4) & 1)) {
+                    const long long at =
+                        (static_cast<long long>(r.kept ? r.page : 0) * a.kv_heads + kvh) * a.page.d + r.offset;
+                    sk = r.kept ? a.scale_k[at] : 0.0f;
+                    sv = r.kept ? a.scale_v[at] : 0.0f;
+                }
+            }
+        }
+    };
+
+    int j0 = lo + 32 * wave;
+    if (j0 < hi) {
+        fetch(j0);
+    }
+    for (; j0 < hi; j0 += kAttnFewRowStep) {
+        // S^T
+        f32x4 st[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            st[t] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                if constexpr (kQuant) {
+                    half8 h[2];
+                    int8_to_half(kx[t][i], h);
+                    st[t] = mfma16(h[0], q[2 * i], st[t]);
+                    st[t] = mfma16(h[1], q[2 * i + 1], st[t]);
+                } else {
+                    st[t] = mfma16(__builtin_bit_cast(half8, kx[t][i]), q[i], st[t]);
+                }
+            }
+        }
+        // V into LDS
+        wave_lds_fence();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            char *row = mine + (16 * t + col) * kStride;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                if constexpr (kQuant) {
+                    half8 h[2];
+                    int8_to_half(vx[t][i], h);
+                    *reinterpret_cast<half8 *>(row + 128 * i + 32 * g) = h[0];
+                    *reinterpret_cast<half8 *>(row + 128 * i + 32 * g + 16) = h[1];
+                } else {
+                    *reinterpret_cast<u32x4 *>(row + 64 * i + 16 * g) = vx[t][i];
+                }
+            }
+        }
+        float *scales = reinterpret_cast<float *>(mine + 32 * kStride);
+        float unit = vmax;
+        if constexpr (kQuant) {
+            if (lane < 32) {
+                scales[lane] = sk;
+                scales[32 + lane] = sv;
+            }
+            // the largest finite scale of a value so far
+            float top = __builtin_isfinite(sv) ? sv : 0.0f;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                top = fmaxf(top, __shfl_xor(top, off));
+            }
+            unit = fmaxf(unit, top);
+        }
+        const unsigned long long kept0 = __ballot(kept[0]), kept1 = __ballot(kept[1]);
+        const uint32_t keptmask = static_cast<uint32_t>(kept0 & 0xffff) |
+                                  (static_cast<uint32_t>(kept1 & 0xffff) << 16);
+        const int jt = j0;
+        bool bad = false;
+        const bool mixed = jt < all_lo || jt + 32 > all_hi;
+        if constexpr (!kQuant) {
+            if (mixed) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            bad |= any_not_finite<T>(vx[t][i][e]);
+                        }
+                    }
+                }
+                bad = __any(bad);
+            }
+        }
+        wave_lds_fence();
+        if (j0 + kAttnFewRowStep < hi) {
+            fetch(j0 + kAttnFewRowStep);
+        }
+
+        // softmax of this lane's 8 keys: 16 t + 4 g + r
+        float top = m;
+        uint32_t seen = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 ks = 1.0f;
+            if constexpr (kQuant) {
+                ks = *reinterpret_cast<f32x4 *>(scales + 16 * t + 4 * g);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = 16 * t + 4 * g + r;
+                const bool see =
+                    ((keptmask >> key) & 1) != 0 && jt + key >= row_lo && jt + key < row_hi;
+                seen |= static_cast<uint32_t>(see) << (4 * t + r);
+                float x = st[t][r];
+                if constexpr (kQuant) {
+                    x *= ks[r];
+                }
+                st[t][r] = see ? x * a.scale : -INFINITY;
+                // a NaN stays one: exp2 of it, below
+                top = fmaxf(top, st[t][r]);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float base = top == -INFINITY ? 0.0f : top;
+        float alpha = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= alpha;
+        // int8: values as whole numbers, their scales on the probabilities, in units of the largest scale
+        const float per_unit = kQuant ? 1.0f / unit : 1.0f;
+        if constexpr (kQuant) {
+            alpha *= vmax * per_unit;
+            vmax = unit;
+        }
+        half8 p;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 vsc = 1.0f;
+            if constexpr (kQuant) {
+                vsc = *reinterpret_cast<f32x4 *>(scales + 32 + 16 * t + 4 * g);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float e = __builtin_amdgcn_exp2f(st[t][r] - base);
+                l += e;
+                if constexpr (kQuant) {
+                    e = ((seen >> (4 * t + r)) & 1) ? e * (vsc[r] * per_unit) : 0.0f;
+                }
+                p[4 * t + r] = static_cast<T>(e);
+            }
+        }
+        // O^T
+        half8 see1;
+        if (!kQuant && bad) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                see1[e] = static_cast<T>((seen >> e) & 1 ? 1.0f : 0.0f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const char *at = mine + (4 * g + (col >> 2)) * kStride + 32 * i + 8 * (lane & 3);
+            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 16 * kStride);
+            u32x4 x = {x0[0], x0[1], x1[0], x1[1]};
+            o[i] = o[i] * alpha;
+            if (!kQuant && bad) {
+                u32x4 clean, code;
+                split_not_finite<T>(x, clean, code);
+                const f32x4 count =
+                    mfma16(__builtin_bit_cast(half8, code), see1, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                x = clean;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    o[i][r] += not_finite_term(count[r]);
+                }
+            }
+            o[i] = mfma16(__builtin_bit_cast(half8, x), p, o[i]);
+        }
+    }
+
+    // the four waves meet: sums of the lanes of a row, then of the waves
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    wave_lds_fence();
+    float *mo = reinterpret_cast<float *>(mine);  // [16][DP]
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = kQuant ? o[i] * vmax : o[i];
+    }
+    if (lane < 16) {
+        s_m[wave][lane] = m;
+        s_l[wave][lane] = l;
+    }
+    __syncthreads();
+    const int r = tid >> 4, d0 = (tid & 15) * (DP / 16);
+    if (r >= rows) {
+        return;
+    }
+    const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float sum = 0.0f, acc[DP / 16] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(s_m[w][r] - base);
+        sum += s_l[w][r] * f;
+        const float *from = reinterpret_cast<const float *>(lds + w * Tile::kWaveBytes) + r * DP + d0;
+#pragma unroll
+        for (int e = 0; e < DP / 16; e += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(from + e);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                acc[e + c] += x[c] * f;
+            }
+        }
+    }
+    const int out_token = static_cast<int>(fast_div(r, a.group, head_in_group));
+    attn_put<T, DP / 16>(a, split, splits, s.first + out_token, kvh * group + static_cast<int>(head_in_group),
+                         d0, acc, mm, sum);
+}
+
+}  // namespace
+}  // namespace tqt

@@ -1,0 +1,88 @@
+// Joining the parts that several workgroups have of a row: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, with
+// the parts taken in the order of the keys. Bound by latency at few rows, by the parts' bytes (at most 3% of the
+// cache's at 256 keys a split) at many.
+#pragma once
+
+#include "attn_common.hpp"
+
+namespace tqt {
+namespace {
+
+// One workgroup per row; head_dim / 4 threads along the row, as many such groups as fit over the splits.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
+{
+    __shared__ int s_seq;
+    __shared__ f32x4 s_acc[256];
+    __shared__ float s_sum[256];
+    const int tid = threadIdx.x;
+    const int token = static_cast<int>(blockIdx.x), head = static_cast<int>(blockIdx.y);
+    if (tid == 0) {
+        s_seq = -1;
+    }
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += 256) {
+        if (a.q_start[b] <= token && token < a.q_start[b + 1]) {
+            s_seq = b;
+        }
+    }
+    __syncthreads();
+    const int b = s_seq;
+    if (b < 0) {
+        return;
+    }
+    const AttnSeq s = attn_seq(a, b);
+    const int i = token - s.first;
+    if (i >= s.nq || s.nq * static_cast<int>(a.group.d) > kAttnFewRows) {
+        return;
+    }
+    int first, last, unused;
+    attn_bounds(a, s, s.pos0, first, unused);
+    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
+    const int splits = attn_splits(first, last, a.few_chunk);
+    if (splits == 1) {
+        return;
+    }
+    const long long row = static_cast<long long>(token) * a.q_heads + head;
+    const long long step = static_cast<long long>(a.q_tokens) * a.q_heads;
+    const int across = a.head_dim / 4, groups = 256 / across;
+    const int group = tid / across, at = tid - group * across;
+    float m = -INFINITY;
+    for (int k = tid & 63; k < splits; k += 64) {
+        m = fmaxf(m, a.part_ml[2 * (k * step + row)]);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        m = fmaxf(m, __shfl_xor(m, off));
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    f32x4 acc = 0.0f;
+    float sum = 0.0f;
+    if (group < groups) {
+        // consecutive splits to one group: the sums' order is that of the keys
+        const int each = (splits + groups - 1) / groups;
+        const int k1 = min(splits, (group + 1) * each);
+#pragma unroll 4
+        for (int k = group * each; k < k1; ++k) {
+            const long long r = k * step + row;
+            const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
+            sum += a.part_ml[2 * r + 1] * f;
+            acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
+        }
+    }
+    s_acc[tid] = acc;
+    s_sum[tid] = sum;
+    __syncthreads();
+    if (tid >= across) {
+        return;
+    }
+    for (int k = 1; k < groups; ++k) {
+        acc += s_acc[k * across + tid];
+        sum += s_sum[k * across + tid];
+    }
+    const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
+    attn_put<T, 4>(a, 0, 1, token, head, 4 * tid, out, m, sum);
+}
+
+}  // namespace
+}  // namespace tqt

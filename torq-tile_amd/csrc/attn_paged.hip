@@ -1,5 +1,7 @@
 // Attention of new tokens over a paged cache on gfx950: the entry points and their checks.
 #include "attn_common.hpp"
+#include "attn_few_row.hpp"
+#include "attn_join.hpp"
 #include "tqt_attn_paged_gfx950.h"
 
 #include <cmath>
@@ -27,7 +29,7 @@ __global__ __launch_bounds__(256) void attn_row_kernel(AttnArgs a)
     }
     const AttnSeq s = attn_seq(a, b);
     const int i = token - s.first;
-    if (i >= a.max_q_len) {
+    if (i >= a.max_q_len || s.nq * static_cast<int>(a.group.d) <= kAttnFewRows) {
         return;
     }
     int lo, hi;
@@ -37,7 +39,7 @@ __global__ __launch_bounds__(256) void attn_row_kernel(AttnArgs a)
     const T *qp = static_cast<const T *>(a.q) + token * a.q_ts + head * a.q_hs;
     for (int e = 0; e < 4; ++e) {
         const int d = lane + 64 * e;
-        q[e] = d < a.head_dim ? static_cast<float>(qp[d]) : 0.0f;
+        q[e] = d < a.head_dim ? static_cast<float>(qp[d]) * a.sign : 0.0f;
         o[e] = 0.0f;
     }
     for (int j = lo; j < hi; ++j) {
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(256) void attn_row_kernel(AttnArgs a)
         dot *= a.scale;
         const float mn = dot > m ? dot : m;
         const float base = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = expf(m - base), p = expf(dot - base);
+        const float alpha = exp2f(m - base), p = exp2f(dot - base);
         l = l * alpha + p;
         m = mn;
         for (int e = 0; e < 4; ++e) {
@@ -78,12 +80,34 @@ __global__ __launch_bounds__(256) void attn_row_kernel(AttnArgs a)
     for (int e = 0; e < 4; ++e) {
         const int d = lane + 64 * e;
         if (d < a.head_dim) {
-            dp[d] = static_cast<T>(m == -INFINITY ? 0.0f : o[e] / l);
+            dp[d] = static_cast<T>(l == 0.0f ? 0.0f : o[e] / l);
         }
     }
     if (a.lse != nullptr && lane == 0) {
-        a.lse[static_cast<long long>(token) * a.q_heads + head] = m == -INFINITY ? m : m + logf(l);
+        a.lse[static_cast<long long>(token) * a.q_heads + head] = (m + log2f(l)) * 0.69314718f;
     }
+}
+
+bool attn_empty(const tqt_attn_paged_params *p)
+{
+    return p->batch == 0 || p->q_tokens == 0 || p->q_heads == 0 || p->max_q_len == 0;
+}
+
+// The checks that the sizes alone decide.
+const char *attn_size_error(const tqt_attn_paged_params *p)
+{
+    const size_t top = 1u << 31;
+    if (p->batch >= (1u << 16) || p->q_tokens >= top || p->q_heads >= (1u << 16) || p->max_q_len >= top ||
+        p->max_kv_len >= top || p->ld_table >= top || p->q_tokens * p->q_heads >= top) {
+        return "batch, q_tokens, q_heads, max_q_len, max_kv_len or ld_table too large";
+    }
+    if (p->kv.head_dim == 0 || p->kv.kv_heads == 0 || p->q_heads % p->kv.kv_heads != 0) {
+        return "q_heads % kv_heads != 0";
+    }
+    if (p->max_q_len * (p->q_heads / p->kv.kv_heads) >= top) {
+        return "max_q_len * (q_heads / kv_heads) exceeds 2^31-1";
+    }
+    return nullptr;
 }
 
 const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool quant)
@@ -91,22 +115,14 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
     if (p == nullptr) {
         return "params == NULL";
     }
-    if (p->batch == 0 || p->q_tokens == 0 || p->q_heads == 0) {
+    if (attn_empty(p)) {
         return nullptr;
-    }
-    const size_t top = 1u << 31;
-    if (p->batch >= (1u << 24) || p->q_tokens >= top || p->q_heads >= (1u << 16) || p->max_q_len >= top ||
-        p->max_kv_len >= top || p->ld_table >= top) {
-        return "batch, q_tokens, q_heads, max_q_len, max_kv_len or ld_table too large";
     }
     if (const char *e = paged_kv_error(p->kv, cache_bytes, quant)) {
         return e;
     }
-    if (p->q_heads % p->kv.kv_heads != 0) {
-        return "q_heads % kv_heads != 0";
-    }
-    if (p->max_q_len * (p->q_heads / p->kv.kv_heads) >= top) {
-        return "max_q_len * (q_heads / kv_heads) exceeds 2^31-1";
+    if (const char *e = attn_size_error(p)) {
+        return e;
     }
     if (p->max_kv_len > p->ld_table * p->kv.page_size) {
         return "max_kv_len > ld_table * page_size";
@@ -132,6 +148,29 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
     return nullptr;
 }
 
+// What a call launches, from its sizes (which have been checked).
+struct AttnPlan
+{
+    bool run_few, run_tile;
+    AttnSplit few;
+    int splits;      // of the kernel that has more
+    long long rows;  // of Q, times query heads
+};
+
+AttnPlan attn_plan(const tqt_attn_paged_params *p)
+{
+    AttnPlan plan;
+    const long long group = p->q_heads / p->kv.kv_heads;
+    const long long window = static_cast<long long>(std::min<size_t>(p->window, 1u << 31));
+    plan.rows = static_cast<long long>(p->q_tokens) * p->q_heads;
+    plan.run_few = group <= kAttnFewRows;
+    plan.run_tile = static_cast<long long>(p->max_q_len) * group > kAttnFewRows;
+    const long long few_q = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
+    plan.few = attn_few_row_split(p->batch, p->kv.kv_heads, attn_span(few_q, p->max_kv_len, window));
+    plan.splits = plan.run_few ? plan.few.splits : 1;
+    return plan;
+}
+
 template <typename T, typename C>
 bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *where)
 {
@@ -140,7 +179,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     }
     const char *error = attn_error(p, sizeof(C), std::is_same<C, int8_t>::value);
     TQT_REQUIRE(error == nullptr, error);
-    if (p->batch == 0 || p->q_tokens == 0 || p->q_heads == 0 || p->max_q_len == 0) {
+    if (attn_empty(p)) {
         return false;
     }
     AttnArgs a = {};
@@ -172,14 +211,35 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.head_dim = static_cast<int>(p->kv.head_dim);
     a.max_q_len = static_cast<int>(p->max_q_len);
     a.max_kv_len = static_cast<int>(p->max_kv_len);
-    a.scale = p->scale;
+    a.sign = p->scale > 0.0f ? 1.0f : p->scale < 0.0f ? -1.0f : 0.0f;
+    a.scale = p->scale == 0.0f ? 1.0f : std::fabs(p->scale) * 1.4426950408889634f;
     a.causal = p->causal != 0;
     // a window past every length is none
     a.window = p->window < (1u << 31) ? static_cast<int>(p->window) : 0;
-    const long long rows = static_cast<long long>(a.q_tokens) * a.q_heads;
-    TQT_REQUIRE(rows < (1ll << 31), "too many rows");
-    hipLaunchKernelGGL((attn_row_kernel<T, C>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0,
-                       stream, a);
+    const AttnPlan plan = attn_plan(p);
+    a.few_chunk = plan.few.chunk;
+    a.part_o = static_cast<float *>(p->workspace);
+    a.part_ml = a.part_o + plan.rows * plan.splits * a.head_dim;
+    if (plan.run_few) {
+        const dim3 grid(plan.few.splits, a.kv_heads, a.batch);
+        if (a.head_dim <= 64) {
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 64>), grid, dim3(256), 0, stream, a);
+        } else if (a.head_dim <= 128) {
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 128>), grid, dim3(256), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 256>), grid, dim3(256), 0, stream, a);
+        }
+        check_launch(where);
+    }
+    if (plan.run_tile) {
+        const long long rows = static_cast<long long>(a.q_tokens) * a.q_heads;
+        hipLaunchKernelGGL((attn_row_kernel<T, C>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256),
+                           0, stream, a);
+        check_launch(where);
+    }
+    if (plan.splits > 1) {
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(a.q_tokens, a.q_heads), dim3(256), 0, stream, a);
+    }
     check_launch(where);
     return true;
 }
@@ -191,9 +251,14 @@ using namespace tqt;
 
 extern "C" {
 
-size_t tqt_get_workspace_size_attn_paged_gfx950(const struct tqt_attn_paged_params *)
+size_t tqt_get_workspace_size_attn_paged_gfx950(const struct tqt_attn_paged_params *params)
 {
-    return 0;
+    if (params == nullptr || attn_size_error(params) != nullptr || attn_empty(params)) {
+        return 0;
+    }
+    const AttnPlan plan = attn_plan(params);
+    // a part of every row and split: its sums, its maximum and its sum of probabilities
+    return plan.splits > 1 ? static_cast<size_t>(plan.rows) * plan.splits * (params->kv.head_dim + 2) * 4 : 0;
 }
 
 #define TQT_ATTN_ENTRIES(NAME, T, C)                                                                  \

@@ -1,0 +1,46 @@
+// Rules of the attention over a paged cache: which kernel takes a sequence, and how its keys are split.
+// Plain C++ without HIP, so that a host program can evaluate them as the launcher does.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+namespace tqt {
+
+// Rows of one key head that the few-row kernel takes: (new tokens) x (query heads per key head), as many
+// as its matrix instruction has columns.
+constexpr int kAttnFewRows = 16;
+
+// Keys that a workgroup of the few-row kernel takes in one step (four waves, 32 each).
+constexpr int kAttnFewRowStep = 128;
+
+struct AttnSplit
+{
+    int chunk, splits;
+};
+
+// Keys that the queries of one sequence may see at most.
+constexpr long long attn_span(long long max_q_len, long long max_kv_len, long long window)
+{
+    return window > 0 ? std::min(max_kv_len, window + max_q_len - 1) : max_kv_len;
+}
+
+// The few-row kernel reads each key once, so it is bound by the cache's bytes: what matters is that every CU
+// has workgroups. A span of the keys is a workgroup; spans get shorter until there are about
+// four for each of the 256 CUs, but keep 256 keys (two steps of a workgroup).
+constexpr long long kAttnFewRowWorkgroups = 1024;
+constexpr int kAttnFewRowLeast = 256;
+
+inline AttnSplit attn_few_row_split(long long batch, long long kv_heads, long long span)
+{
+    const long long want = std::max(1ll, kAttnFewRowWorkgroups / std::max(1ll, batch * kv_heads));
+    long long chunk = (span + want - 1) / want;
+    chunk = std::max<long long>(kAttnFewRowLeast, (chunk + kAttnFewRowStep - 1) / kAttnFewRowStep *
+                                                      kAttnFewRowStep);
+    AttnSplit s;
+    s.chunk = static_cast<int>(chunk);
+    s.splits = static_cast<int>(std::max(1ll, (span + chunk - 1) / chunk));
+    return s;
+}
+
+}  // namespace tqt
