@@ -35,7 +35,7 @@ struct AttnArgs
     float scale, sign;
     int causal, window;  // window 0: none
     // the split of the keys over workgroups: spans of so many keys, joined from the workspace's f32 sums
-    int few_chunk;
+    int few_chunk, tile_chunk, tile_rows;
     float *part_o;   // [splits][q_tokens * q_heads][head_dim], not divided by the sum
     float *part_ml;  // [splits][q_tokens * q_heads][2]: maximum (log2) and sum
 };
@@ -71,7 +71,18 @@ __device__ __forceinline__ void attn_bounds(const AttnArgs &a, const AttnSeq &s,
 // Workgroups that share the keys [first, last) of some rows.
 __device__ __forceinline__ int attn_splits(int first, int last, int chunk)
 {
-    return max(1, (last - first + chunk - 1) / chunk);
+    return last > first ? (last - first - 1) / chunk + 1 : 1;
+}
+
+// The keys that a tile of `m` rows may see, from a multiple of 64 on.
+__device__ __forceinline__ void attn_tile_span(const AttnArgs &a, const AttnSeq &s, int tile, int m, int &first,
+                                               int &last)
+{
+    int unused;
+    const int end = min((tile + 1) * m, s.nq * static_cast<int>(a.group.d)) - 1;
+    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(tile * m, a.group)), first, unused);
+    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(end, a.group)), unused, last);
+    first &= ~63;
 }
 
 // N elements of a row's sums from d0 on (d0 + N <= head_dim or d0 >= head_dim): the result where one

@@ -33,13 +33,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
     }
     const AttnSeq s = attn_seq(a, b);
     const int i = token - s.first;
-    if (i >= s.nq || s.nq * static_cast<int>(a.group.d) > kAttnFewRows) {
+    if (i >= s.nq) {
         return;
     }
-    int first, last, unused;
-    attn_bounds(a, s, s.pos0, first, unused);
-    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
-    const int splits = attn_splits(first, last, a.few_chunk);
+    const int heads = static_cast<int>(a.group.d);
+    int first, last, unused, chunk = a.few_chunk;
+    if (s.nq * heads <= kAttnFewRows) {
+        attn_bounds(a, s, s.pos0, first, unused);
+        attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
+    } else {
+        uint32_t head_in_group;
+        fast_div(head, a.group, head_in_group);
+        attn_tile_span(a, s, (i * heads + static_cast<int>(head_in_group)) / a.tile_rows, a.tile_rows, first,
+                       last);
+        chunk = a.tile_chunk;
+    }
+    const int splits = attn_splits(first, last, chunk);
     if (splits == 1) {
         return;
     }

@@ -2,6 +2,7 @@
 #include "attn_common.hpp"
 #include "attn_few_row.hpp"
 #include "attn_join.hpp"
+#include "attn_tile.hpp"
 #include "tqt_attn_paged_gfx950.h"
 
 #include <cmath>
@@ -9,84 +10,6 @@
 
 namespace tqt {
 namespace {
-
-// One wave per row: lanes along the head, keys one after another with the running maximum and sum.
-template <typename T, typename C>
-__global__ __launch_bounds__(256) void attn_row_kernel(AttnArgs a)
-{
-    const int lane = threadIdx.x & 63;
-    const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (item >= static_cast<long long>(a.q_tokens) * a.q_heads) {
-        return;
-    }
-    const int token = static_cast<int>(item / a.q_heads), head = static_cast<int>(item % a.q_heads);
-    int b = 0;
-    while (b < a.batch && a.q_start[b + 1] <= token) {
-        ++b;
-    }
-    if (b == a.batch || token < a.q_start[b]) {
-        return;
-    }
-    const AttnSeq s = attn_seq(a, b);
-    const int i = token - s.first;
-    if (i >= a.max_q_len || s.nq * static_cast<int>(a.group.d) <= kAttnFewRows) {
-        return;
-    }
-    int lo, hi;
-    attn_bounds(a, s, s.pos0 + i, lo, hi);
-    const int kvh = fast_div(head, a.group);
-    float q[4], o[4], m = -INFINITY, l = 0.0f;
-    const T *qp = static_cast<const T *>(a.q) + token * a.q_ts + head * a.q_hs;
-    for (int e = 0; e < 4; ++e) {
-        const int d = lane + 64 * e;
-        q[e] = d < a.head_dim ? static_cast<float>(qp[d]) * a.sign : 0.0f;
-        o[e] = 0.0f;
-    }
-    for (int j = lo; j < hi; ++j) {
-        uint32_t offset;
-        const uint32_t pi = fast_div(j, a.page, offset);
-        const int page = a.table[b * a.ld_table + pi];
-        if (page < 0 || page >= a.num_pages) {
-            continue;
-        }
-        const long long at = page * a.page_stride + offset * a.token_stride + kvh * a.head_stride;
-        const C *kp = static_cast<const C *>(a.k) + at, *vp = static_cast<const C *>(a.v) + at;
-        float dot = 0.0f;
-        for (int e = 0; e < 4; ++e) {
-            const int d = lane + 64 * e;
-            dot += d < a.head_dim ? q[e] * static_cast<float>(kp[d]) : 0.0f;
-        }
-        for (int off = 32; off > 0; off >>= 1) {
-            dot += __shfl_xor(dot, off);
-        }
-        float vs = 1.0f;
-        if (std::is_same<C, int8_t>::value) {
-            const long long sc = (static_cast<long long>(page) * a.kv_heads + kvh) * a.page.d + offset;
-            dot *= a.scale_k[sc];
-            vs = a.scale_v[sc];
-        }
-        dot *= a.scale;
-        const float mn = dot > m ? dot : m;
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = exp2f(m - base), p = exp2f(dot - base);
-        l = l * alpha + p;
-        m = mn;
-        for (int e = 0; e < 4; ++e) {
-            const int d = lane + 64 * e;
-            o[e] = o[e] * alpha + (d < a.head_dim ? p * vs * static_cast<float>(vp[d]) : 0.0f);
-        }
-    }
-    T *dp = static_cast<T *>(a.d) + token * a.d_ts + head * a.d_hs;
-    for (int e = 0; e < 4; ++e) {
-        const int d = lane + 64 * e;
-        if (d < a.head_dim) {
-            dp[d] = static_cast<T>(l == 0.0f ? 0.0f : o[e] / l);
-        }
-    }
-    if (a.lse != nullptr && lane == 0) {
-        a.lse[static_cast<long long>(token) * a.q_heads + head] = (m + log2f(l)) * 0.69314718f;
-    }
-}
 
 bool attn_empty(const tqt_attn_paged_params *p)
 {
@@ -98,7 +21,7 @@ const char *attn_size_error(const tqt_attn_paged_params *p)
 {
     const size_t top = 1u << 31;
     if (p->batch >= (1u << 16) || p->q_tokens >= top || p->q_heads >= (1u << 16) || p->max_q_len >= top ||
-        p->max_kv_len >= top || p->ld_table >= top || p->q_tokens * p->q_heads >= top) {
+        p->max_kv_len >= top / 2 || p->ld_table >= top || p->q_tokens * p->q_heads >= top) {
         return "batch, q_tokens, q_heads, max_q_len, max_kv_len or ld_table too large";
     }
     if (p->kv.head_dim == 0 || p->kv.kv_heads == 0 || p->q_heads % p->kv.kv_heads != 0) {
@@ -152,7 +75,8 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
 struct AttnPlan
 {
     bool run_few, run_tile;
-    AttnSplit few;
+    AttnSplit few, tile;
+    long long tiles;
     int splits;      // of the kernel that has more
     long long rows;  // of Q, times query heads
 };
@@ -167,7 +91,11 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     plan.run_tile = static_cast<long long>(p->max_q_len) * group > kAttnFewRows;
     const long long few_q = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
     plan.few = attn_few_row_split(p->batch, p->kv.kv_heads, attn_span(few_q, p->max_kv_len, window));
-    plan.splits = plan.run_few ? plan.few.splits : 1;
+    plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
+    plan.tile = attn_tile_split(plan.tiles, p->kv.kv_heads,
+                                attn_span(std::min<long long>(p->max_q_len, kAttnTileRows / group + 2),
+                                          p->max_kv_len, window));
+    plan.splits = std::max(plan.run_few ? plan.few.splits : 1, plan.run_tile ? plan.tile.splits : 1);
     return plan;
 }
 
@@ -218,6 +146,8 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.window = p->window < (1u << 31) ? static_cast<int>(p->window) : 0;
     const AttnPlan plan = attn_plan(p);
     a.few_chunk = plan.few.chunk;
+    a.tile_chunk = plan.tile.chunk;
+    a.tile_rows = kAttnTileRows;
     a.part_o = static_cast<float *>(p->workspace);
     a.part_ml = a.part_o + plan.rows * plan.splits * a.head_dim;
     if (plan.run_few) {
@@ -232,9 +162,14 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         check_launch(where);
     }
     if (plan.run_tile) {
-        const long long rows = static_cast<long long>(a.q_tokens) * a.q_heads;
-        hipLaunchKernelGGL((attn_row_kernel<T, C>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256),
-                           0, stream, a);
+        const dim3 grid(a.kv_heads, static_cast<unsigned>(plan.tiles), plan.tile.splits);
+        if (a.head_dim <= 64) {
+            hipLaunchKernelGGL((attn_tile_kernel<T, C, 64, 4>), grid, dim3(256), 0, stream, a);
+        } else if (a.head_dim <= 128) {
+            hipLaunchKernelGGL((attn_tile_kernel<T, C, 128, 4>), grid, dim3(256), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((attn_tile_kernel<T, C, 256, 4>), grid, dim3(256), 0, stream, a);
+        }
         check_launch(where);
     }
     if (plan.splits > 1) {

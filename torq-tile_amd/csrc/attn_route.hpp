@@ -43,4 +43,33 @@ inline AttnSplit attn_few_row_split(long long batch, long long kv_heads, long lo
     return s;
 }
 
+// The tile kernel is bound by the matrix cores. Its workgroups (two fit a CU) should fill the chip: where
+// the tiles are fewer, their keys are split, in spans of at least 256.
+constexpr int kAttnTileRows = 128;
+constexpr long long kAttnTileWorkgroups = 512;
+constexpr int kAttnTileLeast = 256;
+
+// Tiles of all sequences at most, from the host's bounds.
+inline long long attn_tiles(long long batch, long long q_tokens, long long max_q_len, long long group)
+{
+    const long long each = (max_q_len * group + kAttnTileRows - 1) / kAttnTileRows;
+    return std::min(batch * each, q_tokens * group / kAttnTileRows + batch);
+}
+
+inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long span)
+{
+    const long long want = std::max(1ll, kAttnTileWorkgroups / std::max(1ll, tiles * kv_heads));
+    long long chunk = (span + want - 1) / want;
+    chunk = std::max<long long>(kAttnTileLeast, (chunk + 63) / 64 * 64);
+    AttnSplit s;
+    s.chunk = static_cast<int>(chunk);
+    // a tile's span begins at a multiple of 64: up to 63 keys more
+    s.splits = static_cast<int>(std::max(1ll, (span + 63 + chunk - 1) / chunk));
+    if (want == 1) {
+        s.chunk = static_cast<int>((span + 127) / 64 * 64);
+        s.splits = 1;
+    }
+    return s;
+}
+
 }  // namespace tqt

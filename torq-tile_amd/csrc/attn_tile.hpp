@@ -1,0 +1,469 @@
+// Attention of many rows: tiles of 32 rows a wave, 32 NW a workgroup, against 64 keys at a time. A row is a
+// (token, query head) pair of one key head, so the heads of a group share the keys that a tile reads.
+//
+// Bound by the matrix cores: 4 d flops per row and key. As in the few-row kernel the first product is
+// S^T = K Q^T, so a lane holds 32 of a tile's 64 scores of one row (its neighbour 32 lanes on holds the others),
+// the statistics are one value a lane, and P^T is the second operand of O^T = V^T P^T without leaving the
+// registers. K and V go from memory to LDS directly (16 bytes a lane, a tile ahead of their use, two
+// stages), keys past the end and pages that are not kept from a block of zeros.
+//
+// LDS layout of a tile: [key / 16][piece / 4][key % 16][4 pieces of 16 bytes], so that each lane of the 1 KB load
+// that fills one [16][4] block has the same key in all of its loads, and looks up one page per tile. A key's
+// pieces are at piece ^ f(key), f = 2 bit1(key) + bit2(key): the 8 keys that a 16-byte read of K takes at a
+// time and the 4 keys x 32 bytes of a column read of V each cover all 32 banks once.
+#pragma once
+
+#include "attn_common.hpp"
+
+namespace tqt {
+namespace {
+
+__device__ const u32x4 kAttnZeros = {0, 0, 0, 0};
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// The workgroup's sequence and tile among all of the batch's: tiles of a sequence are taken from its last
+// rows on, which see the most keys.
+__device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int m, int &b, int &tile)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < a.batch) {
+            const AttnSeq s = attn_seq(a, b0 + lane);
+            const int rows = s.nq * static_cast<int>(a.group.d);
+            n = rows > kAttnFewRows ? (rows + m - 1) / m : 0;
+        }
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int x = __shfl_up(upto, off);
+            upto += lane >= off ? x : 0;
+        }
+        const unsigned long long past = __ballot(before + upto > index);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            b = b0 + at;
+            tile = before + __shfl(upto, at) - 1 - index;
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
+}
+
+template <typename T, typename C, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(AttnArgs a)
+{
+    typedef typename Half8<T>::type half8;
+    constexpr bool kQuant = std::is_same<C, int8_t>::value;
+    constexpr int kGroups = DP / 32;                // blocks of 4 pieces along a row
+    constexpr int kTileBytes = 64 * DP * 2;         // of K or V
+    constexpr int kM = 32 * NW;
+    __shared__ __attribute__((aligned(1024))) int8_t lds[4 * kTileBytes];  // [stage][K, V]
+    __shared__ int s_kept[2][4];
+    __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [stage][K, V]
+
+    const int kvh = blockIdx.x, split = blockIdx.z;
+    int b, tile;
+    if (!attn_find_tile(a, blockIdx.y, kM, b, tile)) {
+        return;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    const AttnSeq s = attn_seq(a, b);
+    const int group = static_cast<int>(a.group.d);
+    int first, last;
+    attn_tile_span(a, s, tile, kM, first, last);
+    const int splits = attn_splits(first, last, a.tile_chunk);
+    if (split >= splits) {
+        return;
+    }
+    const int lo = first + split * a.tile_chunk, hi = min(last, lo + a.tile_chunk);
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int32_t *table = a.table + b * a.ld_table;
+    const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
+
+    // this lane's row, and the keys that it sees
+    const int rows = s.nq * group;
+    const int row = tile * kM + 32 * wave + col;
+    const bool live = row < rows;
+    uint32_t head_in_group;
+    const int token = static_cast<int>(fast_div(live ? row : rows - 1, a.group, head_in_group));
+    const int head = kvh * group + static_cast<int>(head_in_group);
+    int row_lo, row_hi;
+    attn_bounds(a, s, s.pos0 + token, row_lo, row_hi);
+    // the keys that every row of the wave sees, and those that any does
+    const int wave_row0 = tile * kM + 32 * wave;
+    const int token0 = static_cast<int>(fast_div(min(wave_row0, rows - 1), a.group));
+    const int token1 = static_cast<int>(fast_div(min(wave_row0 + 31, rows - 1), a.group));
+    int all_lo, all_hi, any_lo, any_hi;
+    attn_bounds(a, s, s.pos0 + token0, any_lo, all_hi);
+    attn_bounds(a, s, s.pos0 + token1, all_lo, any_hi);
+    if (wave_row0 >= rows) {
+        any_hi = 0;  // nothing but the loads
+    }
+
+    half8 q[DP / 16];
+    const T *qp = static_cast<const T *>(a.q) + (s.first + token) * a.q_ts + head * a.q_hs;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+        half8 x = {};
+        if (16 * i < a.head_dim) {
+            x = *reinterpret_cast<const half8 *>(qp + 16 * i + 8 * h);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = static_cast<T>(static_cast<float>(x[e]) * a.sign);
+        }
+        q[i] = x;
+    }
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        o[i] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    float unit = 0x1p-100f;  // int8: what the sums o are in units of
+
+    // loads: this lane's key of a tile is 16 x block + lane / 4
+    constexpr int kBlocks = 4 / NW > 0 ? 4 / NW : 1;  // 16-key blocks a wave loads
+    const int piece = (lane & 3) ^ ((((lane >> 3) & 1) << 1) | ((lane >> 4) & 1));
+    KeyRow next[kBlocks];
+    auto look_up = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            next[i] = attn_key(a, table, kvh, j0 + 16 * (wave * kBlocks + i) + (lane >> 2), hi);
+        }
+    };
+    // int8 tiles pass through registers, where they become 16-bit whole numbers
+    constexpr int kRaw = kQuant ? DP / 64 : 1;
+    u32x4 raw_k[kBlocks][kRaw], raw_v[kBlocks][kRaw];
+    float raw_sk[kBlocks], raw_sv[kBlocks];
+    auto load_raw = [&]() {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+#pragma unroll
+            for (int c = 0; c < kRaw; ++c) {
+                const int d0 = 64 * c + 16 * (lane & 3);
+                u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                if (next[i].kept && d0 < a.head_dim) {
+                    x = *reinterpret_cast<const u32x4 *>(kbase + next[i].at + d0);
+                    y = *reinterpret_cast<const u32x4 *>(vbase + next[i].at + d0);
+                }
+                raw_k[i][c] = x;
+                raw_v[i][c] = y;
+            }
+            const long long at = (static_cast<long long>(next[i].kept ? next[i].page : 0) * a.kv_heads + kvh) *
+                                     a.page.d + next[i].offset;
+            raw_sk[i] = next[i].kept ? a.scale_k[at] : 0.0f;
+            raw_sv[i] = next[i].kept ? a.scale_v[at] : 0.0f;
+        }
+    };
+    unsigned long long raw_kept[kBlocks];
+    auto note_kept = [&]() {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            raw_kept[i] = __ballot(next[i].kept);
+        }
+    };
+    auto store_raw = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int block = wave * kBlocks + i;
+            int8_t *to = lds + stage * 2 * kTileBytes + block * kGroups * 1024 + (lane >> 2) * 64;
+            const int f = (((lane >> 3) & 1) << 1) | ((lane >> 4) & 1);
+#pragma unroll
+            for (int c = 0; c < kRaw; ++c) {
+                half8 x[2], y[2];
+                int8_to_half(raw_k[i][c], x);
+                int8_to_half(raw_v[i][c], y);
+                int8_t *at = to + (2 * c + ((lane >> 1) & 1)) * 1024;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int place = ((2 * (lane & 1) + e) ^ f) * 16;
+                    *reinterpret_cast<half8 *>(at + place) = x[e];
+                    *reinterpret_cast<half8 *>(at + kTileBytes + place) = y[e];
+                }
+            }
+            if ((lane & 3) == 0) {
+                s_scale[stage][0][16 * block + (lane >> 2)] = raw_sk[i];
+                s_scale[stage][1][16 * block + (lane >> 2)] = raw_sv[i];
+            }
+            if (lane == 0) {
+                s_kept[stage][block] = raw_kept[i] == ~0ull;
+            }
+        }
+    };
+    auto load = [&](int stage) {
+        const int8_t *zeros = reinterpret_cast<const int8_t *>(&kAttnZeros);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int block = wave * kBlocks + i;
+            int8_t *to = lds + stage * 2 * kTileBytes + block * kGroups * 1024;
+            const unsigned long long kept = __ballot(next[i].kept);
+            if (lane == 0) {
+                s_kept[stage][block] = kept == ~0ull;
+            }
+#pragma unroll
+            for (int c = 0; c < kGroups; ++c) {
+                const int d0 = 32 * c + 8 * piece;
+                const bool in = next[i].kept && d0 < a.head_dim;
+                const int8_t *kp = in ? reinterpret_cast<const int8_t *>(kbase + next[i].at + d0) : zeros;
+                const int8_t *vp = in ? reinterpret_cast<const int8_t *>(vbase + next[i].at + d0) : zeros;
+                dma_lds16(kp, to + c * 1024);
+                dma_lds16(vp, to + kTileBytes + c * 1024);
+            }
+        }
+    };
+
+    // operand addresses within a stage
+    const int fk = (((col >> 1) & 1) << 1) | ((col >> 2) & 1);
+    const int k_at = (col >> 4) * kGroups * 1024 + (col & 15) * 64 + ((h ^ (fk & 1)) | (fk & 2)) * 16;
+    const int vr = 4 * h + ((lane >> 2) & 3);
+    const int fv = (((vr >> 1) & 1) << 1) | ((vr >> 2) & 1);
+    const int v_at = kTileBytes + vr * 64 + (((((lane >> 4) & 1) << 1) | ((lane >> 1) & 1)) ^ fv) * 16 +
+                     (lane & 1) * 8;
+
+    auto step = [&](int j0, int stage, auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        const int8_t *base = lds + stage * 2 * kTileBytes;
+        f32x16 st[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            st[t] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const half8 k = *reinterpret_cast<const half8 *>(
+                    base + (k_at ^ (32 * (i & 1))) + (2 * t * kGroups + (i >> 1)) * 1024);
+                st[t] = mfma32(k, q[i], st[t]);
+            }
+        }
+        if constexpr (kQuant) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 x =
+                        *reinterpret_cast<const f32x4 *>(&s_scale[stage][0][32 * t + 2 * r + 4 * h]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        st[t][r + c] *= x[c];
+                    }
+                }
+            }
+        }
+        uint32_t seen[2] = {0, 0};
+        if constexpr (kMasked) {
+            // which of the tile's keys are kept is looked up again: tiles at the edges only
+            const KeyRow kr = attn_key(a, table, kvh, j0 + lane, hi);
+            const unsigned long long kept = __ballot(kr.kept);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t kept32 = static_cast<uint32_t>(kept >> (32 * t));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = 8 * (r >> 2) + 4 * h + (r & 3);
+                    const int j = j0 + 32 * t + key;
+                    const bool see = ((kept32 >> key) & 1) != 0 && j >= row_lo && j < row_hi;
+                    seen[t] |= static_cast<uint32_t>(see) << r;
+                    st[t][r] = see ? st[t][r] : -INFINITY;
+                }
+            }
+        }
+        float top = m;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                top = fmaxf(top, st[t][r]);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // m is in units of the unscaled product
+        const float base_s = top == -INFINITY ? 0.0f : top * a.scale;
+        float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.scale, -base_s));
+        m = top;
+        const float alpha_l = alpha;
+        float per_unit = 1.0f;
+        if constexpr (kQuant) {
+            // values are whole numbers here, their scales on the probabilities, in units of the largest
+            const float mine = s_scale[stage][1][lane];
+            float most = __builtin_isfinite(mine) ? mine : 0.0f;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                most = fmaxf(most, __shfl_xor(most, off));
+            }
+            most = fmaxf(most, unit);
+            per_unit = 1.0f / most;
+            alpha *= unit * per_unit;
+            unit = most;
+        }
+        half8 p[4];
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r4 = 0; r4 < 16; r4 += 4) {
+                f32x4 vs = 1.0f;
+                if constexpr (kQuant) {
+                    vs = *reinterpret_cast<const f32x4 *>(&s_scale[stage][1][32 * t + 2 * r4 + 4 * h]);
+                }
+#pragma unroll
+                for (int r = r4; r < r4 + 4; ++r) {
+                    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
+                    sum += e;
+                    if constexpr (kQuant) {
+                        e *= vs[r - r4] * per_unit;
+                        if constexpr (kMasked) {
+                            e = (seen[t] >> r) & 1 ? e : 0.0f;
+                        }
+                    }
+                    p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+                }
+            }
+        }
+        l = __builtin_fmaf(l, alpha_l, sum);
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                o[i] = o[i] * alpha;
+            }
+        }
+        auto value = [&](int i, int u) {
+            const int8_t *at = base + v_at + (u * kGroups + i) * 1024;
+            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
+            return u32x4{x0[0], x0[1], x1[0], x1[1]};
+        };
+        if constexpr (kMasked && !kQuant) {
+            // 0 times the tile's values is NaN where one is no number
+            f32x16 zero = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    zero = mfma32(__builtin_bit_cast(half8, value(i, u)), half8{}, zero);
+                }
+            }
+            bool bad = false;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                bad |= zero[r] != zero[r];
+            }
+            if (__any(bad)) {
+                for (int u = 0; u < 4; ++u) {
+                    half8 see1, pu = p[0];
+                    uint32_t bits = seen[u >> 1] >> (8 * (u & 1));
+#pragma unroll
+                    for (int x = 1; x < 4; ++x) {
+                        pu = u == x ? p[x] : pu;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        see1[e] = static_cast<T>((bits >> e) & 1 ? 1.0f : 0.0f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) {
+                        u32x4 clean, code;
+                        split_not_finite<T>(value(i, u), clean, code);
+                        f32x16 count = 0.0f;
+                        count = mfma32(__builtin_bit_cast(half8, code), see1, count);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            o[i][r] += not_finite_term(count[r]);
+                        }
+                        o[i] = mfma32(__builtin_bit_cast(half8, clean), pu, o[i]);
+                    }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                o[i] = mfma32(__builtin_bit_cast(half8, value(i, u)), p[u], o[i]);
+            }
+        }
+    };
+
+    if (lo < hi) {
+        if (wave * kBlocks < 4) {
+            look_up(lo);
+            if constexpr (kQuant) {
+                load_raw();
+                note_kept();
+                look_up(lo + 64);
+                store_raw(0);
+            } else {
+                load(0);
+                look_up(lo + 64);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    int stage = 0;
+    for (int j0 = lo; j0 < hi; j0 += 64, stage ^= 1) {
+        const bool more = wave * kBlocks < 4 && j0 + 64 < hi;
+        if (more) {
+            if constexpr (kQuant) {
+                load_raw();
+                note_kept();
+            } else {
+                load(stage ^ 1);
+            }
+            look_up(j0 + 128);
+        }
+        if (j0 < any_hi && j0 + 64 > any_lo) {
+            const bool kept = s_kept[stage][0] && s_kept[stage][1] && s_kept[stage][2] && s_kept[stage][3];
+            if (kept && j0 >= all_lo && j0 + 64 <= all_hi) {
+                step(j0, stage, std::false_type());
+            } else {
+                step(j0, stage, std::true_type());
+            }
+        }
+        if constexpr (kQuant) {
+            if (more) {
+                store_raw(stage ^ 1);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+
+    if (!live) {
+        return;
+    }
+    l += __shfl_xor(l, 32);
+    const float m2 = m == -INFINITY ? m : m * a.scale;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            float out[4] = {o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            if constexpr (kQuant) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    out[e] *= unit;
+                }
+            }
+            attn_put<T, 4>(a, split, splits, s.first + token, head, 32 * i + 2 * r + 4 * h, out, m2, l);
+        }
+    }
+}
+
+}  // namespace
+}  // namespace tqt
