@@ -123,6 +123,9 @@ __device__ __forceinline__ void attn_put(const AttnArgs &a, int split, int split
 }
 
 // Element offset of a key's row of one key head, or -1: past `hi`, or on no page of the cache.
+// 512 zero bytes: a row of keys that are not there.
+__device__ const u32x4 kAttnZeros[32] = {};
+
 struct KeyRow
 {
     long long at;
@@ -180,6 +183,18 @@ __device__ __forceinline__ void wave_lds_fence()
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The larger of this lane's value and that of lane ^ 32. The swap is inline asm: with the builtin the compiler
+// drops the maximum of its two results (each lane then has the lower half's value). Two wait states lie
+// between a vector instruction's write and the swap.
+__device__ __forceinline__ float max_across_halves(float x)
+{
+    float y = x;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+#endif
+    return fmaxf(x, y);
 }
 
 // 16 int8 as 16-bit floats, exactly: [0] the first 8, [1] the others.

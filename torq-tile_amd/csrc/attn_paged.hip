@@ -163,12 +163,20 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     }
     if (plan.run_tile) {
         const dim3 grid(a.kv_heads, static_cast<unsigned>(plan.tiles), plan.tile.splits);
+        auto launch = [&](auto dp) {
+            constexpr int kDP = decltype(dp)::value;
+            if (a.head_dim == kDP) {
+                hipLaunchKernelGGL((attn_tile_kernel<T, C, kDP, 4, true>), grid, dim3(256), 0, stream, a);
+            } else {
+                hipLaunchKernelGGL((attn_tile_kernel<T, C, kDP, 4, false>), grid, dim3(256), 0, stream, a);
+            }
+        };
         if (a.head_dim <= 64) {
-            hipLaunchKernelGGL((attn_tile_kernel<T, C, 64, 4>), grid, dim3(256), 0, stream, a);
+            launch(std::integral_constant<int, 64>());
         } else if (a.head_dim <= 128) {
-            hipLaunchKernelGGL((attn_tile_kernel<T, C, 128, 4>), grid, dim3(256), 0, stream, a);
+            launch(std::integral_constant<int, 128>());
         } else {
-            hipLaunchKernelGGL((attn_tile_kernel<T, C, 256, 4>), grid, dim3(256), 0, stream, a);
+            launch(std::integral_constant<int, 256>());
         }
         check_launch(where);
     }

@@ -18,8 +18,6 @@
 namespace tqt {
 namespace {
 
-__device__ const u32x4 kAttnZeros = {0, 0, 0, 0};
-
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c)
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -60,7 +58,7 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
     return false;
 }
 
-template <typename T, typename C, int DP, int NW>
+template <typename T, typename C, int DP, int NW, bool kFull>
 __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(AttnArgs a)
 {
     typedef typename Half8<T>::type half8;
@@ -69,7 +67,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     constexpr int kTileBytes = 64 * DP * 2;         // of K or V
     constexpr int kM = 32 * NW;
     __shared__ __attribute__((aligned(1024))) int8_t lds[4 * kTileBytes];  // [stage][K, V]
-    __shared__ int s_kept[2][4];
+    __shared__ __attribute__((aligned(16))) int s_kept[2][4];
     __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [stage][K, V]
 
     const int kvh = blockIdx.x, split = blockIdx.z;
@@ -104,16 +102,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     const int head = kvh * group + static_cast<int>(head_in_group);
     int row_lo, row_hi;
     attn_bounds(a, s, s.pos0 + token, row_lo, row_hi);
-    // the keys that every row of the wave sees, and those that any does
-    const int wave_row0 = tile * kM + 32 * wave;
-    const int token0 = static_cast<int>(fast_div(min(wave_row0, rows - 1), a.group));
-    const int token1 = static_cast<int>(fast_div(min(wave_row0 + 31, rows - 1), a.group));
-    int all_lo, all_hi, any_lo, any_hi;
-    attn_bounds(a, s, s.pos0 + token0, any_lo, all_hi);
-    attn_bounds(a, s, s.pos0 + token1, all_lo, any_hi);
-    if (wave_row0 >= rows) {
-        any_hi = 0;  // nothing but the loads
-    }
+    // the keys that every row of the workgroup sees
+    int all_lo, all_hi, unused;
+    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(tile * kM, a.group)), unused, all_hi);
+    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(min((tile + 1) * kM, rows) - 1, a.group)), all_lo,
+                unused);
 
     half8 q[DP / 16];
     const T *qp = static_cast<const T *>(a.q) + (s.first + token) * a.q_ts + head * a.q_hs;
@@ -139,7 +132,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     float unit = 0x1p-100f;  // int8: what the sums o are in units of
 
     // loads: this lane's key of a tile is 16 x block + lane / 4
-    constexpr int kBlocks = 4 / NW > 0 ? 4 / NW : 1;  // 16-key blocks a wave loads
+    constexpr int kBlocks = 4 / NW;  // 16-key blocks a wave loads
     const int piece = (lane & 3) ^ ((((lane >> 3) & 1) << 1) | ((lane >> 4) & 1));
     KeyRow next[kBlocks];
     auto look_up = [&](int j0) {
@@ -208,7 +201,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         }
     };
     auto load = [&](int stage) {
-        const int8_t *zeros = reinterpret_cast<const int8_t *>(&kAttnZeros);
+        const int8_t *zeros = reinterpret_cast<const int8_t *>(kAttnZeros);
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
             const int block = wave * kBlocks + i;
@@ -217,14 +210,15 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             if (lane == 0) {
                 s_kept[stage][block] = kept == ~0ull;
             }
+            const int8_t *kp = next[i].kept ? reinterpret_cast<const int8_t *>(kbase + next[i].at) : zeros;
+            const int8_t *vp = next[i].kept ? reinterpret_cast<const int8_t *>(vbase + next[i].at) : zeros;
+            kp += 16 * piece;
+            vp += 16 * piece;
 #pragma unroll
             for (int c = 0; c < kGroups; ++c) {
-                const int d0 = 32 * c + 8 * piece;
-                const bool in = next[i].kept && d0 < a.head_dim;
-                const int8_t *kp = in ? reinterpret_cast<const int8_t *>(kbase + next[i].at + d0) : zeros;
-                const int8_t *vp = in ? reinterpret_cast<const int8_t *>(vbase + next[i].at + d0) : zeros;
-                dma_lds16(kp, to + c * 1024);
-                dma_lds16(vp, to + kTileBytes + c * 1024);
+                const bool in = kFull || 32 * c + 8 * piece < a.head_dim;
+                dma_lds16(in ? kp + 64 * c : zeros, to + c * 1024);
+                dma_lds16(in ? vp + 64 * c : zeros, to + kTileBytes + c * 1024);
             }
         }
     };
@@ -237,15 +231,44 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     const int v_at = kTileBytes + vr * 64 + (((((lane >> 4) & 1) << 1) | ((lane >> 1) & 1)) ^ fv) * 16 +
                      (lane & 1) * 8;
 
-    auto step = [&](int j0, int stage, auto masked) {
-        constexpr bool kMasked = decltype(masked)::value;
+    if (lo < hi) {
+        look_up(lo);
+        if constexpr (kQuant) {
+            load_raw();
+            note_kept();
+            look_up(lo + 64);
+            store_raw(0);
+        } else {
+            load(0);
+            look_up(lo + 64);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    int stage = 0;
+    for (int j0 = lo; j0 < hi; j0 += 64, stage ^= 1) {
+        const bool more = j0 + 64 < hi;
+        if (more) {
+            if constexpr (kQuant) {
+                load_raw();
+                note_kept();
+            } else {
+                load(stage ^ 1);
+            }
+            look_up(j0 + 128);
+        }
+        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[stage]);
+        const bool mixed = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) == 0 ||
+                           j0 < all_lo || j0 + 64 > all_hi;
         const int8_t *base = lds + stage * 2 * kTileBytes;
+
         f32x16 st[2];
+        st[0] = 0.0f;
+        st[1] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            st[t] = 0.0f;
+        for (int i = 0; i < DP / 16; ++i) {
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
+            for (int t = 0; t < 2; ++t) {
                 const half8 k = *reinterpret_cast<const half8 *>(
                     base + (k_at ^ (32 * (i & 1))) + (2 * t * kGroups + (i >> 1)) * 1024);
                 st[t] = mfma32(k, q[i], st[t]);
@@ -265,25 +288,28 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                 }
             }
         }
-        uint32_t seen[2] = {0, 0};
-        if constexpr (kMasked) {
+        uint32_t seen[2] = {~0u, ~0u};
+        if (mixed) {
             // which of the tile's keys are kept is looked up again: tiles at the edges only
             const KeyRow kr = attn_key(a, table, kvh, j0 + lane, hi);
             const unsigned long long kept = __ballot(kr.kept);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint32_t kept32 = static_cast<uint32_t>(kept >> (32 * t));
+                // keys [row_lo, row_hi) of the 32, those kept, and of them this half-wave's: 4 of every 8
+                const int below = min(max(row_lo - j0 - 32 * t, 0), 32);
+                const int upto = min(max(row_hi - j0 - 32 * t, 0), 32);
+                uint32_t in = static_cast<uint32_t>(kept >> (32 * t));
+                in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
+                in >>= 4 * h;
+                seen[t] = (in & 0xfu) | ((in >> 4) & 0xf0u) | ((in >> 8) & 0xf00u) | ((in >> 12) & 0xf000u);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = 8 * (r >> 2) + 4 * h + (r & 3);
-                    const int j = j0 + 32 * t + key;
-                    const bool see = ((kept32 >> key) & 1) != 0 && j >= row_lo && j < row_hi;
-                    seen[t] |= static_cast<uint32_t>(see) << r;
-                    st[t][r] = see ? st[t][r] : -INFINITY;
+                    st[t][r] = (seen[t] >> r) & 1 ? st[t][r] : -INFINITY;
                 }
             }
         }
-        float top = m;
+
+        float top = st[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -291,12 +317,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                 top = fmaxf(top, st[t][r]);
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // m is in units of the unscaled product
+        top = max_across_halves(top);
+        // m, in units of the unscaled product, follows the maximum only when that has grown by more than a
+        // factor of 2^8 in the probabilities: until then they stay below 256 and the sums as they are
+        top = (top - m) * a.scale > 8.0f ? top : m;
         const float base_s = top == -INFINITY ? 0.0f : top * a.scale;
         float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.scale, -base_s));
         m = top;
-        const float alpha_l = alpha;
+        l *= alpha;
         float per_unit = 1.0f;
         if constexpr (kQuant) {
             // values are whole numbers here, their scales on the probabilities, in units of the largest
@@ -311,8 +339,14 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             alpha *= unit * per_unit;
             unit = most;
         }
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                o[i] = o[i] * alpha;
+            }
+        }
         half8 p[4];
-        float sum = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -324,115 +358,68 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
 #pragma unroll
                 for (int r = r4; r < r4 + 4; ++r) {
                     float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
-                    sum += e;
+                    sum[t] += e;
                     if constexpr (kQuant) {
                         e *= vs[r - r4] * per_unit;
-                        if constexpr (kMasked) {
-                            e = (seen[t] >> r) & 1 ? e : 0.0f;
-                        }
+                        e = (seen[t] >> r) & 1 ? e : 0.0f;
                     }
                     p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
                 }
             }
         }
-        l = __builtin_fmaf(l, alpha_l, sum);
-        if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                o[i] = o[i] * alpha;
-            }
-        }
+        l += sum[0] + sum[1];
+
         auto value = [&](int i, int u) {
             const int8_t *at = base + v_at + (u * kGroups + i) * 1024;
             const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
             return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
-        if constexpr (kMasked && !kQuant) {
-            // 0 times the tile's values is NaN where one is no number
-            f32x16 zero = 0.0f;
+        if constexpr (!kQuant) {
+            if (mixed) {
+                // values that are no numbers, which not every row may meet: all waves look at their share
+                u32x4 *share = reinterpret_cast<u32x4 *>(lds + stage * 2 * kTileBytes + kTileBytes) + tid;
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < kTileBytes / 16; i += 64 * NW) {
+                    const u32x4 x = share[i];
+                    bad |= any_not_finite<T>(x[0]) || any_not_finite<T>(x[1]) || any_not_finite<T>(x[2]) ||
+                           any_not_finite<T>(x[3]);
+                }
+                if (__syncthreads_or(bad)) {
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t bits = seen[u >> 1] >> (8 * (u & 1));
+                        half8 see1;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            see1[e] = static_cast<T>((bits >> e) & 1 ? 1.0f : 0.0f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) {
+                            u32x4 clean, code;
+                            split_not_finite<T>(value(i, u), clean, code);
+                            f32x16 count = 0.0f;
+                            count = mfma32(__builtin_bit_cast(half8, code), see1, count);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                o[i][r] += not_finite_term(count[r]);
+                            }
+                        }
+                    }
+                    __syncthreads();
+                    for (int i = 0; i < kTileBytes / 16; i += 64 * NW) {
+                        u32x4 clean, code;
+                        split_not_finite<T>(share[i], clean, code);
+                        share[i] = clean;
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    zero = mfma32(__builtin_bit_cast(half8, value(i, u)), half8{}, zero);
-                }
-            }
-            bool bad = false;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                bad |= zero[r] != zero[r];
-            }
-            if (__any(bad)) {
-                for (int u = 0; u < 4; ++u) {
-                    half8 see1, pu = p[0];
-                    uint32_t bits = seen[u >> 1] >> (8 * (u & 1));
-#pragma unroll
-                    for (int x = 1; x < 4; ++x) {
-                        pu = u == x ? p[x] : pu;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        see1[e] = static_cast<T>((bits >> e) & 1 ? 1.0f : 0.0f);
-                    }
-#pragma unroll
-                    for (int i = 0; i < DP / 32; ++i) {
-                        u32x4 clean, code;
-                        split_not_finite<T>(value(i, u), clean, code);
-                        f32x16 count = 0.0f;
-                        count = mfma32(__builtin_bit_cast(half8, code), see1, count);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            o[i][r] += not_finite_term(count[r]);
-                        }
-                        o[i] = mfma32(__builtin_bit_cast(half8, clean), pu, o[i]);
-                    }
-                }
-                return;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
                 o[i] = mfma32(__builtin_bit_cast(half8, value(i, u)), p[u], o[i]);
-            }
-        }
-    };
-
-    if (lo < hi) {
-        if (wave * kBlocks < 4) {
-            look_up(lo);
-            if constexpr (kQuant) {
-                load_raw();
-                note_kept();
-                look_up(lo + 64);
-                store_raw(0);
-            } else {
-                load(0);
-                look_up(lo + 64);
-            }
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-    }
-    int stage = 0;
-    for (int j0 = lo; j0 < hi; j0 += 64, stage ^= 1) {
-        const bool more = wave * kBlocks < 4 && j0 + 64 < hi;
-        if (more) {
-            if constexpr (kQuant) {
-                load_raw();
-                note_kept();
-            } else {
-                load(stage ^ 1);
-            }
-            look_up(j0 + 128);
-        }
-        if (j0 < any_hi && j0 + 64 > any_lo) {
-            const bool kept = s_kept[stage][0] && s_kept[stage][1] && s_kept[stage][2] && s_kept[stage][3];
-            if (kept && j0 >= all_lo && j0 + 64 <= all_hi) {
-                step(j0, stage, std::false_type());
-            } else {
-                step(j0, stage, std::true_type());
             }
         }
         if constexpr (kQuant) {
