@@ -133,16 +133,35 @@ struct KeyRow
     bool kept;
 };
 
-__device__ __forceinline__ KeyRow attn_key(const AttnArgs &a, const int32_t *table, int head, int j, int hi)
+// A key's page, asked for: the entry is on its way and nothing waits for it yet.
+struct PageAsked
 {
-    KeyRow r;
+    int page, offset;
+};
+
+__device__ __forceinline__ PageAsked attn_ask_page(const AttnArgs &a, const int32_t *table, int j, int hi)
+{
+    PageAsked r;
     uint32_t offset;
     const uint32_t pi = fast_div(static_cast<uint32_t>(j), a.page, offset);
     r.page = j < hi ? table[pi] : -1;
     r.offset = static_cast<int>(offset);
+    return r;
+}
+
+__device__ __forceinline__ KeyRow attn_key(const AttnArgs &a, PageAsked p, int head)
+{
+    KeyRow r;
+    r.page = p.page;
+    r.offset = p.offset;
     r.kept = r.page >= 0 && r.page < a.num_pages;
     r.at = r.kept ? r.page * a.page_stride + r.offset * a.token_stride + head * a.head_stride : 0;
     return r;
+}
+
+__device__ __forceinline__ KeyRow attn_key(const AttnArgs &a, const int32_t *table, int head, int j, int hi)
+{
+    return attn_key(a, attn_ask_page(a, table, j, hi), head);
 }
 
 // 8 values of a 16-bit type as a matrix operand, and the two shapes of product used.

@@ -135,10 +135,17 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     constexpr int kBlocks = 4 / NW;  // 16-key blocks a wave loads
     const int piece = (lane & 3) ^ ((((lane >> 3) & 1) << 1) | ((lane >> 4) & 1));
     KeyRow next[kBlocks];
-    auto look_up = [&](int j0) {
+    PageAsked asked[kBlocks];
+    auto ask = [&](int j0) {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
-            next[i] = attn_key(a, table, kvh, j0 + 16 * (wave * kBlocks + i) + (lane >> 2), hi);
+            asked[i] = attn_ask_page(a, table, j0 + 16 * (wave * kBlocks + i) + (lane >> 2), hi);
+        }
+    };
+    auto resolve = [&]() {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            next[i] = attn_key(a, asked[i], kvh);
         }
     };
     // int8 tiles pass through registers, where they become 16-bit whole numbers
@@ -232,17 +239,18 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                      (lane & 1) * 8;
 
     if (lo < hi) {
-        look_up(lo);
+        ask(lo);
+        resolve();
+        ask(lo + 64);
         if constexpr (kQuant) {
             load_raw();
             note_kept();
-            look_up(lo + 64);
             store_raw(0);
         } else {
             load(0);
-            look_up(lo + 64);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        resolve();
         __syncthreads();
     }
     int stage = 0;
@@ -255,7 +263,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             } else {
                 load(stage ^ 1);
             }
-            look_up(j0 + 128);
+            ask(j0 + 128);
         }
         const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[stage]);
         const bool mixed = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) == 0 ||
@@ -265,14 +273,31 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         f32x16 st[2];
         st[0] = 0.0f;
         st[1] = 0.0f;
+        // operands are read from LDS a group of four ahead of their products
+        auto key = [&](int i, int t) {
+            return *reinterpret_cast<const u32x4 *>(base + (k_at ^ (32 * (i & 1))) +
+                                                    (2 * t * kGroups + (i >> 1)) * 1024);
+        };
+        u32x4 x[2][4];
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
+        for (int e = 0; e < 4; ++e) {
+            x[0][e] = key(e >> 1, e & 1);
+        }
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const half8 k = *reinterpret_cast<const half8 *>(
-                    base + (k_at ^ (32 * (i & 1))) + (2 * t * kGroups + (i >> 1)) * 1024);
-                st[t] = mfma32(k, q[i], st[t]);
+        for (int i = 0; i < DP / 16; i += 2) {
+            const int now = (i >> 1) & 1;
+            if (i + 2 < DP / 16) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[now ^ 1][e] = key(i + 2 + (e >> 1), e & 1);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                st[e & 1] = mfma32(__builtin_bit_cast(half8, x[now][e]), q[i + (e >> 1)], st[e & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (kQuant) {
 #pragma unroll
@@ -309,6 +334,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
         }
 
+        auto value = [&](int i, int u) {
+            const int8_t *at = base + v_at + (u * kGroups + i) * 1024;
+            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
+            return u32x4{x0[0], x0[1], x1[0], x1[1]};
+        };
         float top = st[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -369,11 +399,6 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         }
         l += sum[0] + sum[1];
 
-        auto value = [&](int i, int u) {
-            const int8_t *at = base + v_at + (u * kGroups + i) * 1024;
-            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
-            return u32x4{x0[0], x0[1], x1[0], x1[1]};
-        };
         if constexpr (!kQuant) {
             if (mixed) {
                 // values that are no numbers, which not every row may meet: all waves look at their share
@@ -415,12 +440,28 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                 }
             }
         }
+        constexpr int kAhead = kGroups < 4 ? kGroups : 4, kParts = 4 * kGroups / kAhead;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int e = 0; e < kAhead; ++e) {
+            x[0][e] = value(e % kGroups, e / kGroups);
+        }
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                o[i] = mfma32(__builtin_bit_cast(half8, value(i, u)), p[u], o[i]);
+        for (int n = 0; n < kParts; ++n) {
+            if (n + 1 < kParts) {
+#pragma unroll
+                for (int e = 0; e < kAhead; ++e) {
+                    const int at = (n + 1) * kAhead + e;
+                    x[(n + 1) & 1][e] = value(at % kGroups, at / kGroups);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e) {
+                const int at = n * kAhead + e;
+                o[at % kGroups] =
+                    mfma32(__builtin_bit_cast(half8, x[n & 1][e]), p[at / kGroups], o[at % kGroups]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (kQuant) {
             if (more) {
@@ -428,6 +469,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        resolve();
         __syncthreads();
     }
 
