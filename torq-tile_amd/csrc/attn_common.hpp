@@ -36,6 +36,7 @@ struct AttnArgs
     int causal, window;  // window 0: none
     // the split of the keys over workgroups: spans of so many keys, joined from the workspace's f32 sums
     int few_chunk, tile_chunk, tile_rows;
+    int few_rows;  // sequences of at most so many rows to a key head are the few-row kernel's
     float *part_o;   // [splits][q_tokens * q_heads][head_dim], not divided by the sum
     float *part_ml;  // [splits][q_tokens * q_heads][2]: maximum (log2) and sum
 };

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
     const AttnSeq s = attn_seq(a, b);
     const int group = static_cast<int>(a.group.d);
     const int rows = s.nq * group;
-    if (rows == 0 || rows > kAttnFewRows) {
+    if (rows == 0 || rows > a.few_rows) {
         return;
     }
     // the keys that any row sees

@@ -8,50 +8,63 @@
 namespace tqt {
 namespace {
 
-// One workgroup per row; head_dim / 4 threads along the row, as many such groups as fit over the splits.
+// One workgroup per row; head_dim / 4 threads along the row, as many such groups as fit over the splits. The
+// first `few` workgroups of a head are the rows that the few-row kernel may have (its sequences have at most
+// a.few_rows / group tokens), the others are all rows of Q, for the tile kernel's.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few)
 {
     __shared__ int s_seq;
     __shared__ f32x4 s_acc[256];
     __shared__ float s_sum[256];
-    const int tid = threadIdx.x;
-    const int token = static_cast<int>(blockIdx.x), head = static_cast<int>(blockIdx.y);
-    if (tid == 0) {
-        s_seq = -1;
-    }
-    __syncthreads();
-    for (int b = tid; b < a.batch; b += 256) {
-        if (a.q_start[b] <= token && token < a.q_start[b + 1]) {
-            s_seq = b;
+    const int tid = threadIdx.x, head = static_cast<int>(blockIdx.y);
+    const int heads = static_cast<int>(a.group.d);
+    int b, token;
+    const bool tiles = static_cast<int>(blockIdx.x) >= few;
+    if (tiles) {
+        token = static_cast<int>(blockIdx.x) - few;
+        if (tid == 0) {
+            s_seq = -1;
         }
-    }
-    __syncthreads();
-    const int b = s_seq;
-    if (b < 0) {
-        return;
+        __syncthreads();
+        for (int x = tid; x < a.batch; x += 256) {
+            if (a.q_start[x] <= token && token < a.q_start[x + 1]) {
+                s_seq = x;
+            }
+        }
+        __syncthreads();
+        b = s_seq;
+        if (b < 0) {
+            return;
+        }
+    } else {
+        const int each = few / a.batch;
+        b = static_cast<int>(blockIdx.x) / each;
+        token = static_cast<int>(blockIdx.x) - b * each;
     }
     const AttnSeq s = attn_seq(a, b);
-    const int i = token - s.first;
-    if (i >= s.nq) {
+    if (tiles) {
+        token -= s.first;
+    }
+    if (token >= s.nq || (s.nq * heads > a.few_rows) != tiles) {
         return;
     }
-    const int heads = static_cast<int>(a.group.d);
     int first, last, unused, chunk = a.few_chunk;
-    if (s.nq * heads <= kAttnFewRows) {
-        attn_bounds(a, s, s.pos0, first, unused);
-        attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
-    } else {
+    if (tiles) {
         uint32_t head_in_group;
         fast_div(head, a.group, head_in_group);
-        attn_tile_span(a, s, (i * heads + static_cast<int>(head_in_group)) / a.tile_rows, a.tile_rows, first,
-                       last);
+        attn_tile_span(a, s, (token * heads + static_cast<int>(head_in_group)) / a.tile_rows, a.tile_rows,
+                       first, last);
         chunk = a.tile_chunk;
+    } else {
+        attn_bounds(a, s, s.pos0, first, unused);
+        attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
     }
     const int splits = attn_splits(first, last, chunk);
     if (splits == 1) {
         return;
     }
+    token += s.first;
     const long long row = static_cast<long long>(token) * a.q_heads + head;
     const long long step = static_cast<long long>(a.q_tokens) * a.q_heads;
     const int across = a.head_dim / 4, groups = 256 / across;

@@ -87,7 +87,11 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     const long long group = p->q_heads / p->kv.kv_heads;
     const long long window = static_cast<long long>(std::min<size_t>(p->window, 1u << 31));
     plan.rows = static_cast<long long>(p->q_tokens) * p->q_heads;
-    plan.run_few = group <= kAttnFewRows;
+    // where the bounds say that every sequence has max_q_len tokens, or there is one, its length decides;
+    // a shorter one after all is the tile kernel's
+    const bool alike = p->batch == 1 || p->q_tokens == p->batch * p->max_q_len;
+    plan.run_few = group <= kAttnFewRows &&
+                   (!alike || static_cast<long long>(p->max_q_len) * group <= kAttnFewRows);
     plan.run_tile = static_cast<long long>(p->max_q_len) * group > kAttnFewRows;
     const long long few_q = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
     plan.few = attn_few_row_split(p->batch, p->kv.kv_heads, attn_span(few_q, p->max_kv_len, window));
@@ -148,6 +152,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.few_chunk = plan.few.chunk;
     a.tile_chunk = plan.tile.chunk;
     a.tile_rows = kAttnTileRows;
+    a.few_rows = plan.run_few ? kAttnFewRows : 0;
     a.part_o = static_cast<float *>(p->workspace);
     a.part_ml = a.part_o + plan.rows * plan.splits * a.head_dim;
     if (plan.run_few) {
@@ -180,8 +185,10 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         }
         check_launch(where);
     }
-    if (plan.splits > 1) {
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(a.q_tokens, a.q_heads), dim3(256), 0, stream, a);
+    const int few = plan.run_few && plan.few.splits > 1 ? a.batch * (kAttnFewRows / static_cast<int>(a.group.d)) : 0;
+    const int joined = few + (plan.run_tile && plan.tile.splits > 1 ? a.q_tokens : 0);
+    if (joined > 0) {
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(joined, a.q_heads), dim3(256), 0, stream, a, few);
     }
     check_launch(where);
     return true;

@@ -38,7 +38,7 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
         if (b0 + lane < a.batch) {
             const AttnSeq s = attn_seq(a, b0 + lane);
             const int rows = s.nq * static_cast<int>(a.group.d);
-            n = rows > kAttnFewRows ? (rows + m - 1) / m : 0;
+            n = rows > a.few_rows ? (rows + m - 1) / m : 0;
         }
         int upto = n;
 #pragma unroll
@@ -283,6 +283,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         for (int e = 0; e < 4; ++e) {
             x[0][e] = key(e >> 1, e & 1);
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < DP / 16; i += 2) {
             const int now = (i >> 1) & 1;
@@ -299,6 +300,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (kQuant) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -445,6 +447,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         for (int e = 0; e < kAhead; ++e) {
             x[0][e] = value(e % kGroups, e / kGroups);
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int n = 0; n < kParts; ++n) {
             if (n + 1 < kParts) {
@@ -463,6 +466,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (kQuant) {
             if (more) {
                 store_raw(stage ^ 1);
