@@ -27,8 +27,8 @@ struct FewRowTile
     static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 256 : 0);
 };
 
-template <typename T, typename C, int DP>
-__global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(AttnArgs a)
+template <typename T, typename C, int DP, bool kFull>
+__global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(C) == 1 && DP > 64 ? 1 : 0)) void attn_few_row_kernel(AttnArgs a)
 {
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
@@ -100,24 +100,31 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
     float m = -INFINITY, l = 0.0f;
     float vmax = 0x1p-100f;  // int8: what the sums o are in units of
 
+    // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
     u32x4 kx[2][kPieces], vx[2][kPieces];
     float sk = 0.0f, sv = 0.0f;  // int8: the scales of key lane % 32
+    PageAsked asked[2];
     bool kept[2];
-    auto fetch = [&](int j0) {
+    auto ask = [&](int j) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const KeyRow r = attn_key(a, table, kvh, j0 + 16 * t + col, hi);
+            asked[t] = attn_ask_page(a, table, j + 16 * t + col, hi);
+        }
+    };
+    auto fetch = [&]() {
+        const C *zeros = reinterpret_cast<const C *>(kAttnZeros);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const KeyRow r = attn_key(a, asked[t], kvh);
             kept[t] = r.kept;
+            const C *kp = (r.kept ? kbase + r.at : zeros) + g * kElems;
+            const C *vp = (r.kept ? vbase + r.at : zeros) + g * kElems;
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                const int d0 = (4 * i + g) * kElems;
-                u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                if (r.kept && d0 < a.head_dim) {
-                    x = *reinterpret_cast<const u32x4 *>(kbase + r.at + d0);
-                    y = *reinterpret_cast<const u32x4 *>(vbase + r.at + d0);
-                }
-                kx[t][i] = x;
-                vx[t][i] = y;
+                const int d0 = 4 * i * kElems;
+                const bool in = kFull || d0 + g * kElems < a.head_dim;
+                kx[t][i] = *reinterpret_cast<const u32x4 *>(in ? kp + d0 : zeros);
+                vx[t][i] = *reinterpret_cast<const u32x4 *>(in ? vp + d0 : zeros);
             }
             if constexpr (kQuant) {
                 if (t == ((lane >> 4) & 1)) {
@@ -132,7 +139,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
 
     int j0 = lo + 32 * wave;
     if (j0 < hi) {
-        fetch(j0);
+        ask(j0);
+        fetch();
+        ask(j0 + kAttnFewRowStep);
     }
     for (; j0 < hi; j0 += kAttnFewRowStep) {
         // S^T
@@ -207,12 +216,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
         }
         wave_lds_fence();
         if (j0 + kAttnFewRowStep < hi) {
-            fetch(j0 + kAttnFewRowStep);
+            fetch();
+            ask(j0 + 2 * kAttnFewRowStep);
         }
 
         // softmax of this lane's 8 keys: 16 t + 4 g + r
         float top = m;
-        uint32_t seen = 0;
+        uint32_t seen = 0, in = keptmask;
+        {
+            const int below = min(max(row_lo - jt, 0), 32), upto = min(max(row_hi - jt, 0), 32);
+            in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 ks = 1.0f;
@@ -222,8 +236,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int key = 16 * t + 4 * g + r;
-                const bool see =
-                    ((keptmask >> key) & 1) != 0 && jt + key >= row_lo && jt + key < row_hi;
+                const bool see = (in >> key) & 1;
                 seen |= static_cast<uint32_t>(see) << (4 * t + r);
                 float x = st[t][r];
                 if constexpr (kQuant) {
@@ -263,32 +276,48 @@ __global__ __launch_bounds__(256, DP == 256 ? 2 : 3) void attn_few_row_kernel(At
                 p[4 * t + r] = static_cast<T>(e);
             }
         }
-        // O^T
-        half8 see1;
-        if (!kQuant && bad) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                see1[e] = static_cast<T>((seen >> e) & 1 ? 1.0f : 0.0f);
-            }
-        }
+        const char *columns = mine + (4 * g + (col >> 2)) * kStride + 8 * (lane & 3);
+        auto value = [&](int i) {
+            const u32x2 x0 = lds_read_column4(columns + 32 * i);
+            const u32x2 x1 = lds_read_column4(columns + 32 * i + 16 * kStride);
+            return u32x4{x0[0], x0[1], x1[0], x1[1]};
+        };
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            const char *at = mine + (4 * g + (col >> 2)) * kStride + 32 * i + 8 * (lane & 3);
-            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 16 * kStride);
-            u32x4 x = {x0[0], x0[1], x1[0], x1[1]};
             o[i] = o[i] * alpha;
-            if (!kQuant && bad) {
-                u32x4 clean, code;
-                split_not_finite<T>(x, clean, code);
-                const f32x4 count =
-                    mfma16(__builtin_bit_cast(half8, code), see1, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                x = clean;
+        }
+        if constexpr (!kQuant) {
+            if (bad) {
+                half8 see1;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    o[i][r] += not_finite_term(count[r]);
+                for (int e = 0; e < 8; ++e) {
+                    see1[e] = static_cast<T>((seen >> e) & 1 ? 1.0f : 0.0f);
                 }
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    u32x4 clean, code;
+                    split_not_finite<T>(value(i), clean, code);
+                    const f32x4 count =
+                        mfma16(__builtin_bit_cast(half8, code), see1, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        o[i][r] += not_finite_term(count[r]);
+                    }
+                }
+                wave_lds_fence();
+                for (int i = lane; i < 32 * DP / 8; i += 64) {
+                    u32x4 *at = reinterpret_cast<u32x4 *>(mine + (i / (DP / 8)) * kStride + 16 * (i % (DP / 8)));
+                    u32x4 clean, code;
+                    split_not_finite<T>(*at, clean, code);
+                    *at = clean;
+                }
+                wave_lds_fence();
             }
-            o[i] = mfma16(__builtin_bit_cast(half8, x), p, o[i]);
+        }
+        // O^T
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            o[i] = mfma16(__builtin_bit_cast(half8, value(i)), p, o[i]);
         }
     }
 

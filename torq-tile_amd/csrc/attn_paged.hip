@@ -103,6 +103,26 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     return plan;
 }
 
+// Calls f with the padded head_dim (64, 128 or 256) and whether it is the head's own.
+template <typename F>
+void by_head_dim(int head_dim, F f)
+{
+    auto with = [&](auto dp) {
+        if (head_dim == dp.value) {
+            f(dp, std::true_type());
+        } else {
+            f(dp, std::false_type());
+        }
+    };
+    if (head_dim <= 64) {
+        with(std::integral_constant<int, 64>());
+    } else if (head_dim <= 128) {
+        with(std::integral_constant<int, 128>());
+    } else {
+        with(std::integral_constant<int, 256>());
+    }
+}
+
 template <typename T, typename C>
 bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *where)
 {
@@ -157,32 +177,18 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.part_ml = a.part_o + plan.rows * plan.splits * a.head_dim;
     if (plan.run_few) {
         const dim3 grid(plan.few.splits, a.kv_heads, a.batch);
-        if (a.head_dim <= 64) {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 64>), grid, dim3(256), 0, stream, a);
-        } else if (a.head_dim <= 128) {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 128>), grid, dim3(256), 0, stream, a);
-        } else {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, 256>), grid, dim3(256), 0, stream, a);
-        }
+        by_head_dim(a.head_dim, [&](auto dp, auto full) {
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value>), grid, dim3(256), 0, stream,
+                               a);
+        });
         check_launch(where);
     }
     if (plan.run_tile) {
         const dim3 grid(a.kv_heads, static_cast<unsigned>(plan.tiles), plan.tile.splits);
-        auto launch = [&](auto dp) {
-            constexpr int kDP = decltype(dp)::value;
-            if (a.head_dim == kDP) {
-                hipLaunchKernelGGL((attn_tile_kernel<T, C, kDP, 4, true>), grid, dim3(256), 0, stream, a);
-            } else {
-                hipLaunchKernelGGL((attn_tile_kernel<T, C, kDP, 4, false>), grid, dim3(256), 0, stream, a);
-            }
-        };
-        if (a.head_dim <= 64) {
-            launch(std::integral_constant<int, 64>());
-        } else if (a.head_dim <= 128) {
-            launch(std::integral_constant<int, 128>());
-        } else {
-            launch(std::integral_constant<int, 256>());
-        }
+        by_head_dim(a.head_dim, [&](auto dp, auto full) {
+            hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value>), grid, dim3(256), 0, stream,
+                               a);
+        });
         check_launch(where);
     }
     const int few = plan.run_few && plan.few.splits > 1 ? a.batch * (kAttnFewRows / static_cast<int>(a.group.d)) : 0;
