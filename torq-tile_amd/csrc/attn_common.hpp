@@ -34,11 +34,14 @@ struct AttnArgs
     // sign of the caller's scale.
     float scale, sign;
     int causal, window;  // window 0: none
-    // the split of the keys over workgroups: spans of so many keys, joined from the workspace's f32 sums
-    int few_chunk, tile_chunk, tile_rows;
     int few_rows;  // sequences of at most so many rows to a key head are the few-row kernel's
-    float *part_o;   // [splits][q_tokens * q_heads][head_dim], not divided by the sum
-    float *part_ml;  // [splits][q_tokens * q_heads][2]: maximum (log2) and sum
+    // Parts of rows whose keys several workgroups have, in the workspace: f32 sums not divided by the sum of
+    // probabilities, and (maximum in log2, sum). The few-row kernel's come first: workgroup w's are 2 w (of a
+    // sequence that began before its run) and 2 w + 1 (of one that ends after it), kAttnFewRows rows each;
+    // then the tile kernel's, [split][row of Q][query head], each of tile_chunk keys.
+    float *part_o;   // [][head_dim]
+    float *part_ml;  // [][2]
+    int few_workgroups, tile_chunk, tile_rows;
 };
 
 // A sequence of the batch, with every length brought inside what the host checked.
@@ -87,24 +90,21 @@ __device__ __forceinline__ void attn_tile_span(const AttnArgs &a, const AttnSeq 
 }
 
 // N elements of a row's sums from d0 on (d0 + N <= head_dim or d0 >= head_dim): the result where one
-// workgroup has all of its keys, else this split's part. sum == 0: no key, or scores of -infinity alone.
+// workgroup has all of its keys (part < 0), else a part. sum == 0: no key, or scores of -infinity alone.
 template <typename T, int N>
-__device__ __forceinline__ void attn_put(const AttnArgs &a, int split, int splits, int token, int head, int d0,
+__device__ __forceinline__ void attn_put(const AttnArgs &a, long long part, int token, int head, int d0,
                                          const float (&acc)[N], float m, float sum)
 {
-    const long long row = static_cast<long long>(token) * a.q_heads + head;
-    if (splits > 1) {
-        const long long at = static_cast<long long>(split) * a.q_tokens * a.q_heads + row;
+    if (part >= 0) {
         if (d0 < a.head_dim) {
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                *reinterpret_cast<f32x4 *>(a.part_o + at * a.head_dim + d0 + e) =
-                    f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+            for (int e = 0; e < N; ++e) {
+                a.part_o[part * a.head_dim + d0 + e] = acc[e];
             }
         }
         if (d0 == 0) {
-            a.part_ml[2 * at] = m;
-            a.part_ml[2 * at + 1] = sum;
+            a.part_ml[2 * part] = m;
+            a.part_ml[2 * part + 1] = sum;
         }
         return;
     }
@@ -119,8 +119,54 @@ __device__ __forceinline__ void attn_put(const AttnArgs &a, int split, int split
         *reinterpret_cast<out_vec *>(static_cast<T *>(a.d) + token * a.d_ts + head * a.d_hs + d0) = y;
     }
     if (a.lse != nullptr && d0 == 0) {
-        a.lse[row] = (m + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+        a.lse[static_cast<long long>(token) * a.q_heads + head] =
+            (m + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
     }
+}
+
+// The few-row kernel's work of one sequence: the keys [first, last) that its rows see, in units.
+struct FewRowWork
+{
+    int first, last, units;  // units of one key head; 0: the sequence is not the few-row kernel's
+};
+
+__device__ __forceinline__ FewRowWork few_row_work(const AttnArgs &a, const AttnSeq &s)
+{
+    FewRowWork w;
+    int unused;
+    attn_bounds(a, s, s.pos0, w.first, unused);
+    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, w.last);
+    const int rows = s.nq * static_cast<int>(a.group.d);
+    w.units = rows == 0 || rows > a.few_rows ? 0 : attn_splits(w.first, w.last, kAttnFewRowUnit);
+    return w;
+}
+
+// This lane's share of a sum over the batch: the units of sequence b0 + lane.
+__device__ __forceinline__ int few_row_units(const AttnArgs &a, int b0, int lane)
+{
+    return b0 + lane < a.batch
+               ? few_row_work(a, attn_seq(a, b0 + lane)).units * a.kv_heads
+               : 0;
+}
+
+__device__ __forceinline__ int wave_inclusive_sum(int x, int lane)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(x, off);
+        x += lane >= off ? y : 0;
+    }
+    return x;
+}
+
+// Units of a workgroup's run, from all of the batch's (every lane of a wave calls this).
+__device__ __forceinline__ int few_row_run(const AttnArgs &a, int lane, int &total)
+{
+    total = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        total += __shfl(wave_inclusive_sum(few_row_units(a, b0, lane), lane), 63);
+    }
+    return (total + a.few_workgroups - 1) / a.few_workgroups;
 }
 
 // Element offset of a key's row of one key head, or -1: past `hi`, or on no page of the cache.

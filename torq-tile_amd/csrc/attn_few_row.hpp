@@ -28,38 +28,54 @@ struct FewRowTile
 };
 
 template <typename T, typename C, int DP, bool kFull>
-__global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(C) == 1 && DP > 64 ? 1 : 0)) void attn_few_row_kernel(AttnArgs a)
+__global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn_few_row_kernel(AttnArgs a)
 {
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
     constexpr bool kQuant = Tile::kQuant;
     constexpr int kPieces = Tile::kPieces, kSteps = DP / 32, kStride = Tile::kStride;
     constexpr int kElems = 16 / static_cast<int>(sizeof(C));  // elements of a piece
-    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::kWaveBytes];
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ __attribute__((aligned(16))) char lds[kAttnFewRowWaves * Tile::kWaveBytes];
+    __shared__ float s_m[kAttnFewRowWaves][16], s_l[kAttnFewRowWaves][16];
 
-    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int col = lane & 15, g = lane >> 4;
-    const AttnSeq s = attn_seq(a, b);
     const int group = static_cast<int>(a.group.d);
+    char *mine = lds + wave * Tile::kWaveBytes;
+    int total;
+    const int run = few_row_run(a, lane, total);
+    int unit = static_cast<int>(blockIdx.x) * run;
+    const int end = min(unit + run, total);
+
+    // one sequence and key head after another, each as far as the run goes
+    while (unit < end) {
+    int b = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int n = few_row_units(a, b0, lane), upto = before + wave_inclusive_sum(n, lane);
+        const unsigned long long past = __ballot(upto > unit);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            b = b0 + at;
+            before = __shfl(upto - n, at);
+            break;
+        }
+        before = __shfl(upto, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const AttnSeq s = attn_seq(a, b);
+    const FewRowWork work = few_row_work(a, s);
     const int rows = s.nq * group;
-    if (rows == 0 || rows > a.few_rows) {
-        return;
-    }
-    // the keys that any row sees
-    int first, last, unused;
-    attn_bounds(a, s, s.pos0, first, unused);
-    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
-    const int splits = attn_splits(first, last, a.few_chunk);
-    if (split >= splits) {
-        return;
-    }
-    const int lo = first + split * a.few_chunk, hi = min(last, lo + a.few_chunk);
+    const int in_seq = __builtin_amdgcn_readfirstlane(unit - before);
+    const int kvh = in_seq / work.units, unit0 = in_seq - kvh * work.units;
+    const int unit1 = min(work.units, unit0 + (end - unit));
+    unit += unit1 - unit0;
+    const int lo = work.first + unit0 * kAttnFewRowUnit;
+    const int hi = unit1 == work.units ? work.last : lo + (unit1 - unit0) * kAttnFewRowUnit;
+    const bool whole = unit1 - unit0 == work.units;
+    const long long part = whole ? -1 : (2ll * blockIdx.x + (unit0 == 0)) * kAttnFewRows;
     const int32_t *table = a.table + b * a.ld_table;
     const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
-    char *mine = lds + wave * Tile::kWaveBytes;
-
     // this lane's row, and the keys that it sees
     const bool live = col < rows;
     uint32_t head_in_group;
@@ -71,7 +87,7 @@ __global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(
         row_hi = 0;
     }
     // keys outside [all_lo, all_hi) are not seen by every row
-    int all_lo, all_hi;
+    int all_lo, all_hi, unused;
     attn_bounds(a, s, s.pos0, unused, all_hi);
     attn_bounds(a, s, s.pos0 + s.nq - 1, all_lo, unused);
 
@@ -141,9 +157,9 @@ __global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(
     if (j0 < hi) {
         ask(j0);
         fetch();
-        ask(j0 + kAttnFewRowStep);
+        ask(j0 + kAttnFewRowUnit);
     }
-    for (; j0 < hi; j0 += kAttnFewRowStep) {
+    for (; j0 < hi; j0 += kAttnFewRowUnit) {
         // S^T
         f32x4 st[2];
 #pragma unroll
@@ -215,9 +231,9 @@ __global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(
             }
         }
         wave_lds_fence();
-        if (j0 + kAttnFewRowStep < hi) {
+        if (j0 + kAttnFewRowUnit < hi) {
             fetch();
-            ask(j0 + 2 * kAttnFewRowStep);
+            ask(j0 + 2 * kAttnFewRowUnit);
         }
 
         // softmax of this lane's 8 keys: 16 t + 4 g + r
@@ -335,30 +351,32 @@ __global__ __launch_bounds__(256, (DP == 256 ? 1 : DP == 128 ? 2 : 3) + (sizeof(
         s_l[wave][lane] = l;
     }
     __syncthreads();
-    const int r = tid >> 4, d0 = (tid & 15) * (DP / 16);
-    if (r >= rows) {
-        return;
-    }
-    const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float sum = 0.0f, acc[DP / 16] = {};
+    constexpr int kThreads = 4 * kAttnFewRowWaves, kOut = DP / kThreads;  // threads along a row, elements of each
+    const int r = tid / kThreads, d0 = (tid % kThreads) * kOut;
+    if (r < rows) {
+    float mm = s_m[0][r];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 1; w < kAttnFewRowWaves; ++w) {
+        mm = fmaxf(mm, s_m[w][r]);
+    }
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float sum = 0.0f, acc[kOut] = {};
+#pragma unroll
+    for (int w = 0; w < kAttnFewRowWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(s_m[w][r] - base);
         sum += s_l[w][r] * f;
         const float *from = reinterpret_cast<const float *>(lds + w * Tile::kWaveBytes) + r * DP + d0;
 #pragma unroll
-        for (int e = 0; e < DP / 16; e += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(from + e);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                acc[e + c] += x[c] * f;
-            }
+        for (int e = 0; e < kOut; ++e) {
+            acc[e] += from[e] * f;
         }
     }
     const int out_token = static_cast<int>(fast_div(r, a.group, head_in_group));
-    attn_put<T, DP / 16>(a, split, splits, s.first + out_token, kvh * group + static_cast<int>(head_in_group),
-                         d0, acc, mm, sum);
+    attn_put<T, kOut>(a, part < 0 ? -1 : part + r, s.first + out_token,
+                      kvh * group + static_cast<int>(head_in_group), d0, acc, mm, sum);
+    }
+    __syncthreads();
+    }
 }
 
 }  // namespace

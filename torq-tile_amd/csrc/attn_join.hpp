@@ -8,39 +8,40 @@
 namespace tqt {
 namespace {
 
-// One workgroup per row; head_dim / 4 threads along the row, as many such groups as fit over the splits. The
-// first `few` workgroups of a head are the rows that the few-row kernel may have (its sequences have at most
-// a.few_rows / group tokens), the others are all rows of Q, for the tile kernel's.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few)
+// kWaves waves per row, head_dim / 4 threads along it and as many such groups as fit over the splits: one wave
+// (four rows a workgroup) where the parts are few, four where they are many. The first `few` rows of a head are
+// those that the few-row kernel may have (`each` tokens of every sequence), the others are all rows of Q, for
+// the tile kernel's.
+template <typename T, int kWaves>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int each, int rows)
 {
-    __shared__ int s_seq;
-    __shared__ f32x4 s_acc[256];
-    __shared__ float s_sum[256];
-    const int tid = threadIdx.x, head = static_cast<int>(blockIdx.y);
+    __shared__ f32x4 s_acc[kWaves > 1 ? 256 : 1];
+    __shared__ float s_sum[kWaves > 1 ? 256 : 1];
+    const int tid = threadIdx.x, lane = tid & 63;
     const int heads = static_cast<int>(a.group.d);
-    int b, token;
-    const bool tiles = static_cast<int>(blockIdx.x) >= few;
+    const int item = __builtin_amdgcn_readfirstlane(
+        static_cast<int>(blockIdx.x) * (4 / kWaves) + (kWaves > 1 ? 0 : tid >> 6));
+    if (item >= rows * a.q_heads) {
+        return;
+    }
+    const int at_row = item / a.q_heads, head = item - at_row * a.q_heads;
+    const bool tiles = at_row >= few;
+    int b = 0, token = at_row - few;
     if (tiles) {
-        token = static_cast<int>(blockIdx.x) - few;
-        if (tid == 0) {
-            s_seq = -1;
+        int found = -1;
+        for (int x0 = 0; x0 < a.batch && found < 0; x0 += 64) {
+            const int x = x0 + lane;
+            const unsigned long long here =
+                __ballot(x < a.batch && a.q_start[x] <= token && token < a.q_start[x + 1]);
+            found = here != 0 ? x0 + __builtin_ctzll(here) : -1;
         }
-        __syncthreads();
-        for (int x = tid; x < a.batch; x += 256) {
-            if (a.q_start[x] <= token && token < a.q_start[x + 1]) {
-                s_seq = x;
-            }
-        }
-        __syncthreads();
-        b = s_seq;
-        if (b < 0) {
+        if (found < 0) {
             return;
         }
+        b = found;
     } else {
-        const int each = few / a.batch;
-        b = static_cast<int>(blockIdx.x) / each;
-        token = static_cast<int>(blockIdx.x) - b * each;
+        b = at_row / each;
+        token = at_row - b * each;
     }
     const AttnSeq s = attn_seq(a, b);
     if (tiles) {
@@ -49,29 +50,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few)
     if (token >= s.nq || (s.nq * heads > a.few_rows) != tiles) {
         return;
     }
-    int first, last, unused, chunk = a.few_chunk;
+    // the row's parts: part0, then from part1 on every `step` rows of the workspace
+    uint32_t in_group;
+    const int kvh = static_cast<int>(fast_div(head, a.group, in_group));
+    int parts;
+    long long part0, part1, step;
     if (tiles) {
-        uint32_t head_in_group;
-        fast_div(head, a.group, head_in_group);
-        attn_tile_span(a, s, (token * heads + static_cast<int>(head_in_group)) / a.tile_rows, a.tile_rows,
-                       first, last);
-        chunk = a.tile_chunk;
+        int first, last;
+        attn_tile_span(a, s, (token * heads + static_cast<int>(in_group)) / a.tile_rows, a.tile_rows, first,
+                       last);
+        parts = attn_splits(first, last, a.tile_chunk);
+        step = static_cast<long long>(a.q_tokens) * a.q_heads;
+        part0 = 2ll * a.few_workgroups * kAttnFewRows +
+                static_cast<long long>(s.first + token) * a.q_heads + head;
+        part1 = part0 + step;
     } else {
-        attn_bounds(a, s, s.pos0, first, unused);
-        attn_bounds(a, s, s.pos0 + s.nq - 1, unused, last);
+        const int units = few_row_work(a, s).units;
+        int total, before = 0;
+        const int run = few_row_run(a, lane, total);
+        for (int b0 = 0; b0 <= b; b0 += 64) {
+            before += __shfl(wave_inclusive_sum(b0 + lane < b ? few_row_units(a, b0, lane) : 0, lane), 63);
+        }
+        before += kvh * units;
+        const int w0 = before / run, w1 = (before + units - 1) / run;
+        parts = w1 - w0 + 1;
+        const int r = token * heads + static_cast<int>(in_group);
+        part0 = (2ll * w0 + 1) * kAttnFewRows + r;
+        part1 = 2ll * (w0 + 1) * kAttnFewRows + r;
+        step = 2 * kAttnFewRows;
     }
-    const int splits = attn_splits(first, last, chunk);
-    if (splits == 1) {
+    if (parts == 1) {
         return;
     }
     token += s.first;
-    const long long row = static_cast<long long>(token) * a.q_heads + head;
-    const long long step = static_cast<long long>(a.q_tokens) * a.q_heads;
-    const int across = a.head_dim / 4, groups = 256 / across;
-    const int group = tid / across, at = tid - group * across;
+    const int across = a.head_dim / 4, groups = 64 * kWaves / across;
+    const int me = kWaves > 1 ? tid : lane;
+    const int group = me / across, at = me - group * across;
     float m = -INFINITY;
-    for (int k = tid & 63; k < splits; k += 64) {
-        m = fmaxf(m, a.part_ml[2 * (k * step + row)]);
+    for (int k = lane; k < parts; k += 64) {
+        m = fmaxf(m, a.part_ml[2 * (k == 0 ? part0 : part1 + (k - 1) * step)]);
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
@@ -81,29 +98,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few)
     f32x4 acc = 0.0f;
     float sum = 0.0f;
     if (group < groups) {
-        // consecutive splits to one group: the sums' order is that of the keys
-        const int each = (splits + groups - 1) / groups;
-        const int k1 = min(splits, (group + 1) * each);
-#pragma unroll 4
-        for (int k = group * each; k < k1; ++k) {
-            const long long r = k * step + row;
+        // consecutive parts to one group: the sums' order is that of the keys
+        const int per = (parts + groups - 1) / groups;
+        const int k1 = min(parts, (group + 1) * per);
+#pragma unroll 8
+        for (int k = group * per; k < k1; ++k) {
+            const long long r = k == 0 ? part0 : part1 + (k - 1) * step;
             const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
             sum += a.part_ml[2 * r + 1] * f;
             acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
         }
     }
-    s_acc[tid] = acc;
-    s_sum[tid] = sum;
-    __syncthreads();
-    if (tid >= across) {
+    if constexpr (kWaves > 1) {
+        s_acc[tid] = acc;
+        s_sum[tid] = sum;
+        __syncthreads();
+    }
+    const f32x4 own = acc;
+    const float own_sum = sum;
+    for (int k = 1; k < groups; ++k) {
+        if constexpr (kWaves > 1) {
+            if (tid < across) {
+                acc += s_acc[k * across + tid];
+                sum += s_sum[k * across + tid];
+            }
+        } else {
+            // every group's sums in turn, to the first
+            const int from = k * across + at;
+            sum += __shfl(own_sum, from);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[e] += __shfl(own[e], from);
+            }
+        }
+    }
+    if (me >= across) {
         return;
     }
-    for (int k = 1; k < groups; ++k) {
-        acc += s_acc[k * across + tid];
-        sum += s_sum[k * across + tid];
-    }
     const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
-    attn_put<T, 4>(a, 0, 1, token, head, 4 * tid, out, m, sum);
+    attn_put<T, 4>(a, -1, token, head, 4 * at, out, m, sum);
 }
 
 }  // namespace

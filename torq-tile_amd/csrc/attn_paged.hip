@@ -30,6 +30,10 @@ const char *attn_size_error(const tqt_attn_paged_params *p)
     if (p->max_q_len * (p->q_heads / p->kv.kv_heads) >= top) {
         return "max_q_len * (q_heads / kv_heads) exceeds 2^31-1";
     }
+    if (static_cast<long long>(p->batch) * static_cast<long long>(p->kv.kv_heads) *
+            static_cast<long long>(p->max_kv_len / kAttnFewRowUnit + 1) >= (1ll << 31)) {
+        return "batch * kv_heads * max_kv_len too large";
+    }
     return nullptr;
 }
 
@@ -75,31 +79,49 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
 struct AttnPlan
 {
     bool run_few, run_tile;
-    AttnSplit few, tile;
+    int few_workgroups;    // 0: no few-row kernel
+    bool few_many;         // parts for a row of the few-row kernel
+    long long few_tokens;  // of a sequence of the few-row kernel, at most
     long long tiles;
-    int splits;      // of the kernel that has more
-    long long rows;  // of Q, times query heads
+    AttnSplit tile;
+    long long parts;  // rows of the workspace
 };
+
+// Workgroups of the few-row kernel that a CU holds, by their registers.
+int few_row_per_cu(size_t head_dim)
+{
+    const char *e = getenv("FPC");
+    return e ? atoi(e) : head_dim > 128 ? 1 : head_dim > 64 ? 2 : 3;
+}
 
 AttnPlan attn_plan(const tqt_attn_paged_params *p)
 {
-    AttnPlan plan;
+    AttnPlan plan = {};
     const long long group = p->q_heads / p->kv.kv_heads;
     const long long window = static_cast<long long>(std::min<size_t>(p->window, 1u << 31));
-    plan.rows = static_cast<long long>(p->q_tokens) * p->q_heads;
     // where the bounds say that every sequence has max_q_len tokens, or there is one, its length decides;
     // a shorter one after all is the tile kernel's
     const bool alike = p->batch == 1 || p->q_tokens == p->batch * p->max_q_len;
     plan.run_few = group <= kAttnFewRows &&
                    (!alike || static_cast<long long>(p->max_q_len) * group <= kAttnFewRows);
     plan.run_tile = static_cast<long long>(p->max_q_len) * group > kAttnFewRows;
-    const long long few_q = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
-    plan.few = attn_few_row_split(p->batch, p->kv.kv_heads, attn_span(few_q, p->max_kv_len, window));
+    plan.few_tokens = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
+    if (plan.run_few) {
+        const long long heads = static_cast<long long>(p->batch) * p->kv.kv_heads;
+        const long long span = attn_span(plan.few_tokens, p->max_kv_len, window);
+        plan.few_workgroups = attn_few_row_workgroups(
+            heads * std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit),
+            few_row_per_cu(p->kv.head_dim));
+        plan.few_many = plan.few_workgroups > heads * kAttnJoinManyParts;
+    }
     plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
     plan.tile = attn_tile_split(plan.tiles, p->kv.kv_heads,
                                 attn_span(std::min<long long>(p->max_q_len, kAttnTileRows / group + 2),
                                           p->max_kv_len, window));
-    plan.splits = std::max(plan.run_few ? plan.few.splits : 1, plan.run_tile ? plan.tile.splits : 1);
+    plan.parts = 2ll * plan.few_workgroups * kAttnFewRows;
+    if (plan.run_tile && plan.tile.splits > 1) {
+        plan.parts += plan.tile.splits * static_cast<long long>(p->q_tokens) * p->q_heads;
+    }
     return plan;
 }
 
@@ -169,17 +191,16 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     // a window past every length is none
     a.window = p->window < (1u << 31) ? static_cast<int>(p->window) : 0;
     const AttnPlan plan = attn_plan(p);
-    a.few_chunk = plan.few.chunk;
+    a.few_workgroups = plan.few_workgroups;
     a.tile_chunk = plan.tile.chunk;
     a.tile_rows = kAttnTileRows;
     a.few_rows = plan.run_few ? kAttnFewRows : 0;
     a.part_o = static_cast<float *>(p->workspace);
-    a.part_ml = a.part_o + plan.rows * plan.splits * a.head_dim;
+    a.part_ml = a.part_o + plan.parts * a.head_dim;
     if (plan.run_few) {
-        const dim3 grid(plan.few.splits, a.kv_heads, a.batch);
         by_head_dim(a.head_dim, [&](auto dp, auto full) {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value>), grid, dim3(256), 0, stream,
-                               a);
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value>), dim3(plan.few_workgroups),
+                               dim3(64 * kAttnFewRowWaves), 0, stream, a);
         });
         check_launch(where);
     }
@@ -191,10 +212,19 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         });
         check_launch(where);
     }
-    const int few = plan.run_few && plan.few.splits > 1 ? a.batch * (kAttnFewRows / static_cast<int>(a.group.d)) : 0;
-    const int joined = few + (plan.run_tile && plan.tile.splits > 1 ? a.q_tokens : 0);
-    if (joined > 0) {
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3(joined, a.q_heads), dim3(256), 0, stream, a, few);
+    const bool join_tile = plan.run_tile && plan.tile.splits > 1;
+    if (plan.few_workgroups > 1 || join_tile) {
+        const int each = static_cast<int>(plan.few_tokens), few = plan.run_few ? a.batch * each : 0;
+        const int rows = few + (join_tile ? a.q_tokens : 0);
+        const long long items = static_cast<long long>(rows) * a.q_heads;
+        TQT_REQUIRE(items < (1ll << 31), "too many rows");
+        if (plan.few_many || plan.tile.splits > kAttnJoinManyParts) {
+            hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3(static_cast<unsigned>(items)), dim3(256), 0,
+                               stream, a, few, each, rows);
+        } else {
+            hipLaunchKernelGGL((attn_join_kernel<T, 1>), dim3(static_cast<unsigned>((items + 3) / 4)),
+                               dim3(256), 0, stream, a, few, each, rows);
+        }
     }
     check_launch(where);
     return true;
@@ -213,8 +243,7 @@ size_t tqt_get_workspace_size_attn_paged_gfx950(const struct tqt_attn_paged_para
         return 0;
     }
     const AttnPlan plan = attn_plan(params);
-    // a part of every row and split: its sums, its maximum and its sum of probabilities
-    return plan.splits > 1 ? static_cast<size_t>(plan.rows) * plan.splits * (params->kv.head_dim + 2) * 4 : 0;
+    return static_cast<size_t>(plan.parts) * (params->kv.head_dim + 2) * 4;
 }
 
 #define TQT_ATTN_ENTRIES(NAME, T, C)                                                                  \

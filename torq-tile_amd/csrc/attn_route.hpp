@@ -11,37 +11,27 @@ namespace tqt {
 // as its matrix instruction has columns.
 constexpr int kAttnFewRows = 16;
 
-// Keys that a workgroup of the few-row kernel takes in one step (four waves, 32 each).
-constexpr int kAttnFewRowStep = 128;
-
-struct AttnSplit
-{
-    int chunk, splits;
-};
-
 // Keys that the queries of one sequence may see at most.
 constexpr long long attn_span(long long max_q_len, long long max_kv_len, long long window)
 {
     return window > 0 ? std::min(max_kv_len, window + max_q_len - 1) : max_kv_len;
 }
 
-// The few-row kernel reads each key once, so it is bound by the cache's bytes: what matters is that every CU
-// has workgroups. A span of the keys is a workgroup; spans get shorter until there are about
-// four for each of the 256 CUs, but keep 256 keys (two steps of a workgroup).
-constexpr long long kAttnFewRowWorkgroups = 1024;
-constexpr int kAttnFewRowLeast = 256;
+// The few-row kernel reads each key once, so it is bound by the cache's bytes: every CU should have them in
+// flight all the time, whatever the lengths are. Its keys are cut into units of so many for each key head, and
+// the workgroups that fit the chip at once take equal runs of units, across sequences.
+constexpr int kAttnFewRowWaves = 4;
+constexpr int kAttnFewRowUnit = 32 * kAttnFewRowWaves;
 
-inline AttnSplit attn_few_row_split(long long batch, long long kv_heads, long long span)
+// Workgroups of the few-row kernel for a call of at most so many units.
+inline int attn_few_row_workgroups(long long units, int per_cu)
 {
-    const long long want = std::max(1ll, kAttnFewRowWorkgroups / std::max(1ll, batch * kv_heads));
-    long long chunk = (span + want - 1) / want;
-    chunk = std::max<long long>(kAttnFewRowLeast, (chunk + kAttnFewRowStep - 1) / kAttnFewRowStep *
-                                                      kAttnFewRowStep);
-    AttnSplit s;
-    s.chunk = static_cast<int>(chunk);
-    s.splits = static_cast<int>(std::max(1ll, (span + chunk - 1) / chunk));
-    return s;
+    return static_cast<int>(std::max(1ll, std::min(units, 256ll * per_cu)));
 }
+
+// Whether the join of the few-row kernel's parts takes four waves for a row instead of one: at more parts
+// than so many.
+constexpr int kAttnJoinManyParts = 16;
 
 // The tile kernel is bound by the matrix cores. Its workgroups (two fit a CU) should fill the chip: where
 // the tiles are fewer, their keys are split, in spans of at least 256.
@@ -55,6 +45,11 @@ inline long long attn_tiles(long long batch, long long q_tokens, long long max_q
     const long long each = (max_q_len * group + kAttnTileRows - 1) / kAttnTileRows;
     return std::min(batch * each, q_tokens * group / kAttnTileRows + batch);
 }
+
+struct AttnSplit
+{
+    int chunk, splits;
+};
 
 inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long span)
 {

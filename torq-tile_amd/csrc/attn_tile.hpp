@@ -482,6 +482,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     }
     l += __shfl_xor(l, 32);
     const float m2 = m == -INFINITY ? m : m * a.scale;
+    const long long part = splits == 1 ? -1
+                                       : 2ll * a.few_workgroups * kAttnFewRows +
+                                             (static_cast<long long>(split) * a.q_tokens + s.first + token) *
+                                                 a.q_heads +
+                                             head;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) {
 #pragma unroll
@@ -493,7 +498,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                     out[e] *= unit;
                 }
             }
-            attn_put<T, 4>(a, split, splits, s.first + token, head, 32 * i + 2 * r + 4 * h, out, m2, l);
+            attn_put<T, 4>(a, part, s.first + token, head, 32 * i + 2 * r + 4 * h, out, m2, l);
         }
     }
 }
