@@ -141,32 +141,58 @@ __device__ __forceinline__ FewRowWork few_row_work(const AttnArgs &a, const Attn
     return w;
 }
 
-// This lane's share of a sum over the batch: the units of sequence b0 + lane.
-__device__ __forceinline__ int few_row_units(const AttnArgs &a, int b0, int lane)
+// Sum of the lanes up to and with this one, of which those from n on hold 0 (and lane 63 the total).
+__device__ __forceinline__ int wave_inclusive_sum(int x, int lane, int n)
 {
-    return b0 + lane < a.batch
-               ? few_row_work(a, attn_seq(a, b0 + lane)).units * a.kv_heads
-               : 0;
-}
-
-__device__ __forceinline__ int wave_inclusive_sum(int x, int lane)
-{
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
+    n = min(n, 64);
+    for (int off = 1; off < n; off <<= 1) {
         const int y = __shfl_up(x, off);
         x += lane >= off ? y : 0;
     }
-    return x;
+    return lane < n ? x : __builtin_amdgcn_readlane(x, n - 1);
 }
 
-// Units of a workgroup's run, from all of the batch's (every lane of a wave calls this).
-__device__ __forceinline__ int few_row_run(const AttnArgs &a, int lane, int &total)
+// The few-row kernel's units of all sequences in order, each times kv_heads. A wave holds 64 sequences at a
+// time, one a lane.
+struct FewRowBatch
+{
+    AttnSeq s;       // sequence b0 + lane
+    FewRowWork work;
+    int b0;
+    int upto;        // units of sequences up to and with this lane's
+};
+
+__device__ __forceinline__ void few_row_batch(const AttnArgs &a, int b0, int before, int lane, FewRowBatch &x)
+{
+    const bool in = b0 + lane < a.batch;
+    x.s = attn_seq(a, in ? b0 + lane : 0);
+    x.work = few_row_work(a, x.s);
+    x.b0 = b0;
+    x.upto = before + wave_inclusive_sum(in ? x.work.units * a.kv_heads : 0, lane, a.batch - b0);
+}
+
+// Units of a workgroup's run (all lanes of a wave call this); leaves the last 64 sequences in x.
+__device__ __forceinline__ int few_row_run(const AttnArgs &a, int lane, int &total, FewRowBatch &x)
 {
     total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        total += __shfl(wave_inclusive_sum(few_row_units(a, b0, lane), lane), 63);
+        few_row_batch(a, b0, total, lane, x);
+        total = __shfl(x.upto, 63);
     }
     return (total + a.few_workgroups - 1) / a.few_workgroups;
+}
+
+// One lane's sequence and work for the whole wave.
+__device__ __forceinline__ void few_row_pick(const FewRowBatch &x, int at, AttnSeq &s, FewRowWork &w)
+{
+    s.first = __builtin_amdgcn_readlane(x.s.first, at);
+    s.q_len = __builtin_amdgcn_readlane(x.s.q_len, at);
+    s.kv_len = __builtin_amdgcn_readlane(x.s.kv_len, at);
+    s.nq = __builtin_amdgcn_readlane(x.s.nq, at);
+    s.pos0 = __builtin_amdgcn_readlane(x.s.pos0, at);
+    w.first = __builtin_amdgcn_readlane(x.work.first, at);
+    w.last = __builtin_amdgcn_readlane(x.work.last, at);
+    w.units = __builtin_amdgcn_readlane(x.work.units, at);
 }
 
 // Element offset of a key's row of one key head, or -1: past `hi`, or on no page of the cache.

@@ -42,29 +42,31 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
     const int col = lane & 15, g = lane >> 4;
     const int group = static_cast<int>(a.group.d);
     char *mine = lds + wave * Tile::kWaveBytes;
+    const int wg = static_cast<int>(blockIdx.x);
     int total;
-    const int run = few_row_run(a, lane, total);
-    int unit = static_cast<int>(blockIdx.x) * run;
+    FewRowBatch batch;
+    const int run = few_row_run(a, lane, total, batch);
+    int unit = wg * run;
     const int end = min(unit + run, total);
 
     // one sequence and key head after another, each as far as the run goes
     while (unit < end) {
-    int b = 0;
-    int before = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int n = few_row_units(a, b0, lane), upto = before + wave_inclusive_sum(n, lane);
-        const unsigned long long past = __ballot(upto > unit);
-        if (past != 0) {
-            const int at = __builtin_ctzll(past);
-            b = b0 + at;
-            before = __shfl(upto - n, at);
-            break;
+    if (a.batch > 64) {
+        int before = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 64) {
+            few_row_batch(a, b0, before, lane, batch);
+            before = __shfl(batch.upto, 63);
+            if (before > unit) {
+                break;
+            }
         }
-        before = __shfl(upto, 63);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    const AttnSeq s = attn_seq(a, b);
-    const FewRowWork work = few_row_work(a, s);
+    const int in_batch = __builtin_ctzll(__ballot(batch.upto > unit));
+    const int b = batch.b0 + in_batch;
+    AttnSeq s;
+    FewRowWork work;
+    few_row_pick(batch, in_batch, s, work);
+    const int before = __builtin_amdgcn_readlane(batch.upto, in_batch) - work.units * a.kv_heads;
     const int rows = s.nq * group;
     const int in_seq = __builtin_amdgcn_readfirstlane(unit - before);
     const int kvh = in_seq / work.units, unit0 = in_seq - kvh * work.units;
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
     const int lo = work.first + unit0 * kAttnFewRowUnit;
     const int hi = unit1 == work.units ? work.last : lo + (unit1 - unit0) * kAttnFewRowUnit;
     const bool whole = unit1 - unit0 == work.units;
-    const long long part = whole ? -1 : (2ll * blockIdx.x + (unit0 == 0)) * kAttnFewRows;
+    const long long part = whole ? -1 : (2ll * wg + (unit0 == 0)) * kAttnFewRows;
     const int32_t *table = a.table + b * a.ld_table;
     const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
     // this lane's row, and the keys that it sees

@@ -26,26 +26,36 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int
     }
     const int at_row = item / a.q_heads, head = item - at_row * a.q_heads;
     const bool tiles = at_row >= few;
-    int b = 0, token = at_row - few;
+    AttnSeq s;
+    int token, units = 0, run = 1, before = 0;
     if (tiles) {
-        int found = -1;
-        for (int x0 = 0; x0 < a.batch && found < 0; x0 += 64) {
+        token = at_row - few;
+        int b = -1;
+        for (int x0 = 0; x0 < a.batch && b < 0; x0 += 64) {
             const int x = x0 + lane;
             const unsigned long long here =
                 __ballot(x < a.batch && a.q_start[x] <= token && token < a.q_start[x + 1]);
-            found = here != 0 ? x0 + __builtin_ctzll(here) : -1;
+            b = here != 0 ? x0 + __builtin_ctzll(here) : -1;
         }
-        if (found < 0) {
+        if (b < 0) {
             return;
         }
-        b = found;
-    } else {
-        b = at_row / each;
-        token = at_row - b * each;
-    }
-    const AttnSeq s = attn_seq(a, b);
-    if (tiles) {
+        s = attn_seq(a, b);
         token -= s.first;
+    } else {
+        const int b = at_row / each;
+        token = at_row - b * each;
+        FewRowBatch batch;
+        FewRowWork work;
+        int total;
+        run = few_row_run(a, lane, total, batch);
+        for (int b0 = 0; a.batch > 64 && b0 <= b; b0 += 64) {
+            few_row_batch(a, b0, before, lane, batch);
+            before = __shfl(batch.upto, 63);
+        }
+        few_row_pick(batch, b & 63, s, work);
+        units = work.units;
+        before = __builtin_amdgcn_readlane(batch.upto, b & 63) - units * a.kv_heads;
     }
     if (token >= s.nq || (s.nq * heads > a.few_rows) != tiles) {
         return;
@@ -65,12 +75,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int
                 static_cast<long long>(s.first + token) * a.q_heads + head;
         part1 = part0 + step;
     } else {
-        const int units = few_row_work(a, s).units;
-        int total, before = 0;
-        const int run = few_row_run(a, lane, total);
-        for (int b0 = 0; b0 <= b; b0 += 64) {
-            before += __shfl(wave_inclusive_sum(b0 + lane < b ? few_row_units(a, b0, lane) : 0, lane), 63);
-        }
         before += kvh * units;
         const int w0 = before / run, w1 = (before + units - 1) / run;
         parts = w1 - w0 + 1;

@@ -90,8 +90,7 @@ struct AttnPlan
 // Workgroups of the few-row kernel that a CU holds, by their registers.
 int few_row_per_cu(size_t head_dim)
 {
-    const char *e = getenv("FPC");
-    return e ? atoi(e) : head_dim > 128 ? 1 : head_dim > 64 ? 2 : 3;
+    return head_dim > 128 ? 1 : 2;
 }
 
 AttnPlan attn_plan(const tqt_attn_paged_params *p)
