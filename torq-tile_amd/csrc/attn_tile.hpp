@@ -66,9 +66,9 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     constexpr int kGroups = DP / 32;                // blocks of 4 pieces along a row
     constexpr int kTileBytes = 64 * DP * 2;         // of K or V
     constexpr int kM = 32 * NW;
-    __shared__ __attribute__((aligned(1024))) int8_t lds[4 * kTileBytes];  // [stage][K, V]
-    __shared__ __attribute__((aligned(16))) int s_kept[2][4];
-    __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [stage][K, V]
+    __shared__ __attribute__((aligned(1024))) int8_t lds[4 * kTileBytes];  // K of even and odd tiles, V of both
+    __shared__ __attribute__((aligned(16))) int s_kept[4][4];              // [tile % 4][16-key block]
+    __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [K, V][tile % 2]
 
     const int kvh = blockIdx.x, split = blockIdx.z;
     int b, tile;
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     // loads: this lane's key of a tile is 16 x block + lane / 4
     constexpr int kBlocks = 4 / NW;  // 16-key blocks a wave loads
     const int piece = (lane & 3) ^ ((((lane >> 3) & 1) << 1) | ((lane >> 4) & 1));
-    KeyRow next[kBlocks];
+    KeyRow k_next[kBlocks], v_next[kBlocks];
     PageAsked asked[kBlocks];
     auto ask = [&](int j0) {
 #pragma unroll
@@ -145,87 +145,71 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     auto resolve = [&]() {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
-            next[i] = attn_key(a, asked[i], kvh);
+            v_next[i] = k_next[i];
+            k_next[i] = attn_key(a, asked[i], kvh);
         }
     };
-    // int8 tiles pass through registers, where they become 16-bit whole numbers
-    constexpr int kRaw = kQuant ? DP / 64 : 1;
-    u32x4 raw_k[kBlocks][kRaw], raw_v[kBlocks][kRaw];
-    float raw_sk[kBlocks], raw_sv[kBlocks];
-    auto load_raw = [&]() {
+    auto note_kept = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
-#pragma unroll
-            for (int c = 0; c < kRaw; ++c) {
-                const int d0 = 64 * c + 16 * (lane & 3);
-                u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                if (next[i].kept && d0 < a.head_dim) {
-                    x = *reinterpret_cast<const u32x4 *>(kbase + next[i].at + d0);
-                    y = *reinterpret_cast<const u32x4 *>(vbase + next[i].at + d0);
-                }
-                raw_k[i][c] = x;
-                raw_v[i][c] = y;
-            }
-            const long long at = (static_cast<long long>(next[i].kept ? next[i].page : 0) * a.kv_heads + kvh) *
-                                     a.page.d + next[i].offset;
-            raw_sk[i] = next[i].kept ? a.scale_k[at] : 0.0f;
-            raw_sv[i] = next[i].kept ? a.scale_v[at] : 0.0f;
-        }
-    };
-    unsigned long long raw_kept[kBlocks];
-    auto note_kept = [&]() {
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            raw_kept[i] = __ballot(next[i].kept);
-        }
-    };
-    auto store_raw = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-            const int block = wave * kBlocks + i;
-            int8_t *to = lds + stage * 2 * kTileBytes + block * kGroups * 1024 + (lane >> 2) * 64;
-            const int f = (((lane >> 3) & 1) << 1) | ((lane >> 4) & 1);
-#pragma unroll
-            for (int c = 0; c < kRaw; ++c) {
-                half8 x[2], y[2];
-                int8_to_half(raw_k[i][c], x);
-                int8_to_half(raw_v[i][c], y);
-                int8_t *at = to + (2 * c + ((lane >> 1) & 1)) * 1024;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int place = ((2 * (lane & 1) + e) ^ f) * 16;
-                    *reinterpret_cast<half8 *>(at + place) = x[e];
-                    *reinterpret_cast<half8 *>(at + kTileBytes + place) = y[e];
-                }
-            }
-            if ((lane & 3) == 0) {
-                s_scale[stage][0][16 * block + (lane >> 2)] = raw_sk[i];
-                s_scale[stage][1][16 * block + (lane >> 2)] = raw_sv[i];
-            }
+            const unsigned long long kept = __ballot(k_next[i].kept);
             if (lane == 0) {
-                s_kept[stage][block] = raw_kept[i] == ~0ull;
+                s_kept[tile & 3][wave * kBlocks + i] = kept == ~0ull;
             }
         }
     };
-    auto load = [&](int stage) {
+    // 16-bit rows go to LDS directly, `which` (0: K, 1: V) of an even or odd tile
+    auto load = [&](const KeyRow (&from)[kBlocks], const C *source, int which, int tile) {
         const int8_t *zeros = reinterpret_cast<const int8_t *>(kAttnZeros);
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
-            const int block = wave * kBlocks + i;
-            int8_t *to = lds + stage * 2 * kTileBytes + block * kGroups * 1024;
-            const unsigned long long kept = __ballot(next[i].kept);
-            if (lane == 0) {
-                s_kept[stage][block] = kept == ~0ull;
-            }
-            const int8_t *kp = next[i].kept ? reinterpret_cast<const int8_t *>(kbase + next[i].at) : zeros;
-            const int8_t *vp = next[i].kept ? reinterpret_cast<const int8_t *>(vbase + next[i].at) : zeros;
-            kp += 16 * piece;
-            vp += 16 * piece;
+            int8_t *to = lds + (2 * which + (tile & 1)) * kTileBytes + (wave * kBlocks + i) * kGroups * 1024;
+            const int8_t *p =
+                (from[i].kept ? reinterpret_cast<const int8_t *>(source + from[i].at) : zeros) + 16 * piece;
 #pragma unroll
             for (int c = 0; c < kGroups; ++c) {
                 const bool in = kFull || 32 * c + 8 * piece < a.head_dim;
-                dma_lds16(in ? kp + 64 * c : zeros, to + c * 1024);
-                dma_lds16(in ? vp + 64 * c : zeros, to + kTileBytes + c * 1024);
+                dma_lds16(in ? p + 64 * c : zeros, to + c * 1024);
+            }
+        }
+    };
+    // int8 rows pass through registers, where they become 16-bit whole numbers
+    constexpr int kRaw = kQuant ? DP / 64 : 1;
+    u32x4 raw[2][kBlocks][kRaw];
+    float raw_scale[2][kBlocks];
+    auto load_raw = [&](const KeyRow (&from)[kBlocks], const C *source, const float *scales, int which) {
+        const C *zeros = reinterpret_cast<const C *>(kAttnZeros);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const C *p = (from[i].kept ? source + from[i].at : zeros) + 16 * (lane & 3);
+#pragma unroll
+            for (int c = 0; c < kRaw; ++c) {
+                const bool in = kFull || 64 * c + 16 * (lane & 3) < a.head_dim;
+                raw[which][i][c] = *reinterpret_cast<const u32x4 *>(in ? p + 64 * c : zeros);
+            }
+            const long long at = (static_cast<long long>(from[i].page) * a.kv_heads + kvh) * a.page.d +
+                                 from[i].offset;
+            raw_scale[which][i] = *(from[i].kept ? scales + at : reinterpret_cast<const float *>(kAttnZeros));
+        }
+    };
+    auto store_raw = [&](int which, int tile) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const int block = wave * kBlocks + i;
+            int8_t *to = lds + (2 * which + (tile & 1)) * kTileBytes + block * kGroups * 1024 + (lane >> 2) * 64;
+            const int f = (((lane >> 3) & 1) << 1) | ((lane >> 4) & 1);
+#pragma unroll
+            for (int c = 0; c < kRaw; ++c) {
+                half8 x[2];
+                int8_to_half(raw[which][i][c], x);
+                int8_t *at = to + (2 * c + ((lane >> 1) & 1)) * 1024;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    *reinterpret_cast<half8 *>(at + ((2 * (lane & 1) + e) ^ f) * 16) = x[e];
+                }
+            }
+            if ((lane & 3) == 0) {
+                s_scale[which][tile & 1][16 * block + (lane >> 2)] = raw_scale[which][i];
             }
         }
     };
@@ -235,86 +219,49 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     const int k_at = (col >> 4) * kGroups * 1024 + (col & 15) * 64 + ((h ^ (fk & 1)) | (fk & 2)) * 16;
     const int vr = 4 * h + ((lane >> 2) & 3);
     const int fv = (((vr >> 1) & 1) << 1) | ((vr >> 2) & 1);
-    const int v_at = kTileBytes + vr * 64 + (((((lane >> 4) & 1) << 1) | ((lane >> 1) & 1)) ^ fv) * 16 +
+    const int v_at = 2 * kTileBytes + vr * 64 + (((((lane >> 4) & 1) << 1) | ((lane >> 1) & 1)) ^ fv) * 16 +
                      (lane & 1) * 8;
 
-    if (lo < hi) {
-        ask(lo);
-        resolve();
-        ask(lo + 64);
-        if constexpr (kQuant) {
-            load_raw();
-            note_kept();
-            store_raw(0);
-        } else {
-            load(0);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        resolve();
-        __syncthreads();
-    }
-    int stage = 0;
-    for (int j0 = lo; j0 < hi; j0 += 64, stage ^= 1) {
-        const bool more = j0 + 64 < hi;
-        if (more) {
-            if constexpr (kQuant) {
-                load_raw();
-                note_kept();
-            } else {
-                load(stage ^ 1);
+    auto scale_scores = [&](f32x16 (&st)[2], int parity) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(&s_scale[0][parity][32 * t + 2 * r + 4 * h]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    st[t][r + c] *= y[c];
+                }
             }
-            ask(j0 + 128);
         }
-        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[stage]);
+    };
+    // One tile: its scores are in `st`; the next one's go to `after`, their products between the exponentials
+    // of this one's (a wave issues in order, so that the two kinds have to alternate). `odd`: the tile's
+    // number's lowest bit.
+    auto step = [&](f32x16 (&st)[2], f32x16 (&after)[2], int j0, int n, auto odd) {
+        constexpr int kOdd = decltype(odd)::value;
+        const bool more = j0 + 64 < hi, more2 = j0 + 128 < hi;
+        if constexpr (kQuant) {
+            if (more2) {
+                load_raw(k_next, kbase, a.scale_k, 0);
+                note_kept(n + 2);
+            }
+            if (more) {
+                load_raw(v_next, vbase, a.scale_v, 1);
+            }
+        } else {
+            if (more2) {
+                load(k_next, kbase, 0, kOdd);
+                note_kept(n + 2);
+            }
+            if (more) {
+                load(v_next, vbase, 1, kOdd ^ 1);
+            }
+        }
+        ask(j0 + 192);
+        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[n & 3]);
         const bool mixed = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) == 0 ||
                            j0 < all_lo || j0 + 64 > all_hi;
-        const int8_t *base = lds + stage * 2 * kTileBytes;
-
-        f32x16 st[2];
-        st[0] = 0.0f;
-        st[1] = 0.0f;
-        // operands are read from LDS a group of four ahead of their products
-        auto key = [&](int i, int t) {
-            return *reinterpret_cast<const u32x4 *>(base + (k_at ^ (32 * (i & 1))) +
-                                                    (2 * t * kGroups + (i >> 1)) * 1024);
-        };
-        u32x4 x[2][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[0][e] = key(e >> 1, e & 1);
-        }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < DP / 16; i += 2) {
-            const int now = (i >> 1) & 1;
-            if (i + 2 < DP / 16) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[now ^ 1][e] = key(i + 2 + (e >> 1), e & 1);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                st[e & 1] = mfma32(__builtin_bit_cast(half8, x[now][e]), q[i + (e >> 1)], st[e & 1]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_s_setprio(0);
-        if constexpr (kQuant) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 x =
-                        *reinterpret_cast<const f32x4 *>(&s_scale[stage][0][32 * t + 2 * r + 4 * h]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        st[t][r + c] *= x[c];
-                    }
-                }
-            }
-        }
         uint32_t seen[2] = {~0u, ~0u};
         if (mixed) {
             // which of the tile's keys are kept is looked up again: tiles at the edges only
@@ -336,11 +283,23 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
         }
 
+        // operands are read from LDS a group of four ahead of their products
+        const int8_t *k_base = lds + (kOdd ^ 1) * kTileBytes, *v_base = lds + kOdd * kTileBytes;
+        auto key = [&](int i, int t) {
+            return *reinterpret_cast<const u32x4 *>(k_base + (k_at ^ (32 * (i & 1))) +
+                                                    (2 * t * kGroups + (i >> 1)) * 1024);
+        };
         auto value = [&](int i, int u) {
-            const int8_t *at = base + v_at + (u * kGroups + i) * 1024;
+            const int8_t *at = v_base + v_at + (u * kGroups + i) * 1024;
             const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
             return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
+        u32x4 x[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[0][e] = key(e >> 1, e & 1);
+        }
+
         float top = st[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -360,7 +319,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         float per_unit = 1.0f;
         if constexpr (kQuant) {
             // values are whole numbers here, their scales on the probabilities, in units of the largest
-            const float mine = s_scale[stage][1][lane];
+            const float mine = s_scale[1][kOdd][lane];
             float most = __builtin_isfinite(mine) ? mine : 0.0f;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
@@ -379,38 +338,44 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         }
         half8 p[4];
         float sum[2] = {0.0f, 0.0f};
+        after[0] = 0.0f;
+        after[1] = 0.0f;
+        constexpr int kProducts = DP / 8, kEach = kProducts > 32 ? 1 : 32 / kProducts;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int k = 0; k < kProducts; ++k) {
+            if (k % 4 == 0 && k + 4 < kProducts) {
 #pragma unroll
-            for (int r4 = 0; r4 < 16; r4 += 4) {
-                f32x4 vs = 1.0f;
-                if constexpr (kQuant) {
-                    vs = *reinterpret_cast<const f32x4 *>(&s_scale[stage][1][32 * t + 2 * r4 + 4 * h]);
-                }
-#pragma unroll
-                for (int r = r4; r < r4 + 4; ++r) {
-                    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
-                    sum[t] += e;
-                    if constexpr (kQuant) {
-                        e *= vs[r - r4] * per_unit;
-                        e = (seen[t] >> r) & 1 ? e : 0.0f;
-                    }
-                    p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+                for (int e = 0; e < 4; ++e) {
+                    x[((k >> 2) + 1) & 1][e] = key((k >> 1) + 2 + (e >> 1), e & 1);
                 }
             }
+            after[k & 1] =
+                mfma32(__builtin_bit_cast(half8, x[(k >> 2) & 1][k & 3]), q[k >> 1], after[k & 1]);
+#pragma unroll
+            for (int c = 0; c < kEach; ++c) {
+                const int t = (k * kEach + c) >> 4, r = (k * kEach + c) & 15;
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
+                sum[t] += e;
+                if constexpr (kQuant) {
+                    e *= s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)] * per_unit;
+                    e = (seen[t] >> r) & 1 ? e : 0.0f;
+                }
+                p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         l += sum[0] + sum[1];
 
         if constexpr (!kQuant) {
             if (mixed) {
                 // values that are no numbers, which not every row may meet: all waves look at their share
-                u32x4 *share = reinterpret_cast<u32x4 *>(lds + stage * 2 * kTileBytes + kTileBytes) + tid;
+                u32x4 *share = reinterpret_cast<u32x4 *>(lds + (2 + kOdd) * kTileBytes) + tid;
                 bool bad = false;
 #pragma unroll
                 for (int i = 0; i < kTileBytes / 16; i += 64 * NW) {
-                    const u32x4 x = share[i];
-                    bad |= any_not_finite<T>(x[0]) || any_not_finite<T>(x[1]) || any_not_finite<T>(x[2]) ||
-                           any_not_finite<T>(x[3]);
+                    const u32x4 y = share[i];
+                    bad |= any_not_finite<T>(y[0]) || any_not_finite<T>(y[1]) || any_not_finite<T>(y[2]) ||
+                           any_not_finite<T>(y[3]);
                 }
                 if (__syncthreads_or(bad)) {
                     for (int u = 0; u < 4; ++u) {
@@ -447,34 +412,97 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         for (int e = 0; e < kAhead; ++e) {
             x[0][e] = value(e % kGroups, e / kGroups);
         }
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int n = 0; n < kParts; ++n) {
-            if (n + 1 < kParts) {
+        for (int k = 0; k < kParts; ++k) {
+            if (k + 1 < kParts) {
 #pragma unroll
                 for (int e = 0; e < kAhead; ++e) {
-                    const int at = (n + 1) * kAhead + e;
-                    x[(n + 1) & 1][e] = value(at % kGroups, at / kGroups);
+                    const int at = (k + 1) * kAhead + e;
+                    x[(k + 1) & 1][e] = value(at % kGroups, at / kGroups);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < kAhead; ++e) {
-                const int at = n * kAhead + e;
+                const int at = k * kAhead + e;
                 o[at % kGroups] =
-                    mfma32(__builtin_bit_cast(half8, x[n & 1][e]), p[at / kGroups], o[at % kGroups]);
+                    mfma32(__builtin_bit_cast(half8, x[k & 1][e]), p[at / kGroups], o[at % kGroups]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_s_setprio(0);
         if constexpr (kQuant) {
+            scale_scores(after, kOdd ^ 1);
+            if (more2) {
+                store_raw(0, kOdd);
+            }
             if (more) {
-                store_raw(stage ^ 1);
+                store_raw(1, kOdd ^ 1);
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         resolve();
         __syncthreads();
+    };
+
+    if (lo < hi) {
+        f32x16 even[2], odd[2];
+        // K of tiles 0 and 1, V of tile 0
+        ask(lo);
+        resolve();
+        ask(lo + 64);
+        resolve();
+        note_kept(1);
+        if constexpr (kQuant) {
+            load_raw(k_next, kbase, a.scale_k, 0);
+            store_raw(0, 1);
+            load_raw(v_next, kbase, a.scale_k, 0);
+            load_raw(v_next, vbase, a.scale_v, 1);
+            store_raw(0, 0);
+            store_raw(1, 0);
+        } else {
+            load(v_next, kbase, 0, 0);
+            load(k_next, kbase, 0, 1);
+            load(v_next, vbase, 1, 0);
+        }
+        ask(lo + 128);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const unsigned long long kept = __ballot(v_next[i].kept);
+            if (lane == 0) {
+                s_kept[0][wave * kBlocks + i] = kept == ~0ull;
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        resolve();
+        __syncthreads();
+        even[0] = 0.0f;
+        even[1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const u32x4 k = *reinterpret_cast<const u32x4 *>(lds + (k_at ^ (32 * (i & 1))) +
+                                                                 (2 * t * kGroups + (i >> 1)) * 1024);
+                even[t] = mfma32(__builtin_bit_cast(half8, k), q[i], even[t]);
+            }
+        }
+        if constexpr (kQuant) {
+            scale_scores(even, 0);
+        }
+        __syncthreads();
+        for (int j0 = lo, n = 0;;) {
+            step(even, odd, j0, n, std::integral_constant<int, 0>());
+            j0 += 64;
+            if (j0 >= hi) {
+                break;
+            }
+            step(odd, even, j0, n + 1, std::integral_constant<int, 1>());
+            j0 += 64;
+            n += 2;
+            if (j0 >= hi) {
+                break;
+            }
+        }
     }
 
     if (!live) {
