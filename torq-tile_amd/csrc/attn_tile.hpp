@@ -340,7 +340,20 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         float sum[2] = {0.0f, 0.0f};
         after[0] = 0.0f;
         after[1] = 0.0f;
-        constexpr int kProducts = DP / 8, kEach = kProducts > 32 ? 1 : 32 / kProducts;
+        constexpr int kProducts = DP / 8, kEach = 32 / kProducts;
+        auto use = [&](int k) {
+#pragma unroll
+            for (int c = 0; c < kEach; ++c) {
+                const int t = (k * kEach + c) >> 4, r = (k * kEach + c) & 15;
+                float e = st[t][r];
+                sum[t] += e;
+                if constexpr (kQuant) {
+                    e *= s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)] * per_unit;
+                    e = (seen[t] >> r) & 1 ? e : 0.0f;
+                }
+                p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+            }
+        };
 #pragma unroll
         for (int k = 0; k < kProducts; ++k) {
             if (k % 4 == 0 && k + 4 < kProducts) {
@@ -351,19 +364,18 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             }
             after[k & 1] =
                 mfma32(__builtin_bit_cast(half8, x[(k >> 2) & 1][k & 3]), q[k >> 1], after[k & 1]);
+            // exponentials of this step's scores, and what the last step's are for
 #pragma unroll
             for (int c = 0; c < kEach; ++c) {
                 const int t = (k * kEach + c) >> 4, r = (k * kEach + c) & 15;
-                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
-                sum[t] += e;
-                if constexpr (kQuant) {
-                    e *= s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)] * per_unit;
-                    e = (seen[t] >> r) & 1 ? e : 0.0f;
-                }
-                p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+                st[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
+            }
+            if (k > 0) {
+                use(k - 1);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        use(kProducts - 1);
         l += sum[0] + sum[1];
 
         if constexpr (!kQuant) {
