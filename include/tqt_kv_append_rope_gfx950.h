@@ -15,7 +15,7 @@
  *   f16_f32, bf16_f32       results of the f32 GEMMs, rounded once; Q_out has the cache's type
  *   qsi8dx_f16, qsi8dx_bf16 an int8 cache, symmetric with one f32 scale for each token and head in
  *                           scale_k, scale_v [num_pages][kv_heads][page_size]: amax = max |x| of the
- *                           (rotated, f32) row, scale = amax / 127 (1 for a row of zeros),
+ *                           (rotated, f32) row, scale = amax * f32(1 / 127) (1 for a row of zeros),
  *                           q = clamp(nearbyint(x / scale), -127, 127). A row with a NaN or an infinity
  *                           gets a scale that is one, so it reads back as NaN. Q_out has Q's type.
  *

@@ -56,7 +56,7 @@ def rope(x, positions, table, rot, interleaved, inverse=False, dtype=np.float64)
 def quantize_rows(rows):
     """Symmetric int8 of f32 rows [..., d], as the library defines it: (q, scale)."""
     amax = np.abs(rows).max(-1)
-    scale = (amax / np.float32(127)).astype(np.float32)
+    scale = (amax * (np.float32(1) / np.float32(127))).astype(np.float32)
     zero = scale == 0
     scale = np.where(zero, np.float32(1), scale)
     with np.errstate(over="ignore"):

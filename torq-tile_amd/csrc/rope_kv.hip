@@ -77,27 +77,40 @@ __device__ __forceinline__ float nan_max(float m, float a)
     return a > m || a != a ? a : m;
 }
 
+// The scale of a row of an int8 cache; `zero`: every q is 0 (a scale that is 0 in f32 too).
 struct QuantRow
 {
-    float scale;
-    bool zero;
+    float scale, inverse;
+    bool zero, plain;
 };
 
-// The scale of a row of an int8 cache; `zero`: every q is 0 (an amax whose 127th part is 0 in f32 too).
 __device__ __forceinline__ QuantRow quant_row(float amax)
 {
     QuantRow r;
-    r.scale = amax / 127.0f;
+    r.scale = amax * (1.0f / 127.0f);
     r.zero = r.scale == 0.0f;
     if (r.zero) {
         r.scale = 1.0f;
     }
+    r.inverse = 1.0f / r.scale;
+    r.plain = r.scale >= 0x1p-100f && r.scale <= 0x1p100f;
     return r;
 }
 
-__device__ __forceinline__ int8_t quant_value(float x, QuantRow r)
+// nearbyint(x / scale). The quotient is correctly rounded without a division: from the correctly rounded inverse,
+// two corrections by the exact remainder (the second starts within an ulp), where none of them underflows; a
+// quotient below 2^-40, whose remainder may, rounds to 0 either way.
+__device__ __forceinline__ int8_t quant_value(float x, const QuantRow &r)
 {
-    const float q = fminf(fmaxf(rintf(x / r.scale), -127.0f), 127.0f);
+    float y;
+    if (r.plain) {
+        y = x * r.inverse;
+        y = __builtin_fmaf(__builtin_fmaf(-y, r.scale, x), r.inverse, y);
+        y = __builtin_fmaf(__builtin_fmaf(-y, r.scale, x), r.inverse, y);
+    } else {
+        y = x / r.scale;
+    }
+    const float q = fminf(fmaxf(rintf(y), -127.0f), 127.0f);
     return r.zero ? static_cast<int8_t>(0) : static_cast<int8_t>(q);
 }
 
@@ -210,7 +223,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a, int
     }
 #pragma unroll
     for (int j = 0; j < HPT; ++j) {
-        QuantRow quant = {1.0f, true};
+        QuantRow quant = {1.0f, 1.0f, true, true};
         if constexpr (kQuant) {
             float amax = 0.0f;
 #pragma unroll
@@ -292,7 +305,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_any_kernel(RopeArgs a, int 
         const int pos = a.positions[token];
         t = pos >= 0 && pos < a.max_pos ? a.table + static_cast<long long>(pos) * r : nullptr;
     }
-    QuantRow quant = {1.0f, true};
+    QuantRow quant = {1.0f, 1.0f, true, true};
     float amax = 0.0f;
     // an int8 row is gone through twice: its amax, then its values
     for (int pass = kQuant && !query ? 0 : 1; pass < 2; ++pass) {
