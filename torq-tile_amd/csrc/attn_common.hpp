@@ -289,6 +289,35 @@ __device__ __forceinline__ float max_across_halves(float x)
     return fmaxf(x, y);
 }
 
+// x * y, and 0 where x or y is 0, whatever the other is.
+__device__ __forceinline__ float mul_zero_wins(float x, float y)
+{
+    float z = 0.0f;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(z) : "v"(x), "v"(y));
+#endif
+    return z;
+}
+
+// The largest of a wave's values (none of them NaN): rotations within rows of 16, then across the rows.
+__device__ __forceinline__ float wave_max(float x)
+{
+    auto rotated = [](float y, auto by) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y),
+                                                                     0x120 + decltype(by)::value, 0xf, 0xf,
+                                                                     false));
+    };
+    x = fmaxf(x, rotated(x, std::integral_constant<int, 1>()));
+    x = fmaxf(x, rotated(x, std::integral_constant<int, 2>()));
+    x = fmaxf(x, rotated(x, std::integral_constant<int, 4>()));
+    x = fmaxf(x, rotated(x, std::integral_constant<int, 8>()));
+    const int y = __builtin_bit_cast(int, x);
+    return fmaxf(fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 0)),
+                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 16))),
+                 fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 32)),
+                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 48))));
+}
+
 // 16 int8 as 16-bit floats, exactly: [0] the first 8, [1] the others.
 __device__ __forceinline__ void int8_to_half(u32x4 x, f16x8 (&y)[2])
 {

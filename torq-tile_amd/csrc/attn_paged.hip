@@ -124,23 +124,20 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     return plan;
 }
 
-// Calls f with the padded head_dim (64, 128 or 256) and whether it is the head's own.
-template <typename F>
+// Calls f with the first of the sizes that holds head_dim, and whether it is the head's own.
+template <int kSize, int... kMore, typename F>
 void by_head_dim(int head_dim, F f)
 {
-    auto with = [&](auto dp) {
-        if (head_dim == dp.value) {
-            f(dp, std::true_type());
-        } else {
-            f(dp, std::false_type());
+    if constexpr (sizeof...(kMore) > 0) {
+        if (head_dim > kSize) {
+            by_head_dim<kMore...>(head_dim, f);
+            return;
         }
-    };
-    if (head_dim <= 64) {
-        with(std::integral_constant<int, 64>());
-    } else if (head_dim <= 128) {
-        with(std::integral_constant<int, 128>());
+    }
+    if (head_dim == kSize) {
+        f(std::integral_constant<int, kSize>(), std::true_type());
     } else {
-        with(std::integral_constant<int, 256>());
+        f(std::integral_constant<int, kSize>(), std::false_type());
     }
 }
 
@@ -197,7 +194,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.part_o = static_cast<float *>(p->workspace);
     a.part_ml = a.part_o + plan.parts * a.head_dim;
     if (plan.run_few) {
-        by_head_dim(a.head_dim, [&](auto dp, auto full) {
+        by_head_dim<64, 128, 256>(a.head_dim, [&](auto dp, auto full) {
             hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value>), dim3(plan.few_workgroups),
                                dim3(64 * kAttnFewRowWaves), 0, stream, a);
         });
@@ -205,7 +202,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     }
     if (plan.run_tile) {
         const dim3 grid(a.kv_heads, static_cast<unsigned>(plan.tiles), plan.tile.splits);
-        by_head_dim(a.head_dim, [&](auto dp, auto full) {
+        by_head_dim<64, 96, 128, 192, 256>(a.head_dim, [&](auto dp, auto full) {
             hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value>), grid, dim3(256), 0, stream,
                                a);
         });

@@ -59,10 +59,14 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
 }
 
 template <typename T, typename C, int DP, int NW, bool kFull>
-__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(AttnArgs a)
+__global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnArgs a)
 {
-    typedef typename Half8<T>::type half8;
     constexpr bool kQuant = std::is_same<C, int8_t>::value;
+    // The second product's type: int8 values are whole numbers in f16, which costs less than bf16 and rounds
+    // the probabilities less.
+    typedef typename std::conditional<kQuant, _Float16, T>::type P;
+    typedef typename Half8<T>::type half8;
+    typedef typename Half8<P>::type prob8;
     constexpr int kGroups = DP / 32;                // blocks of 4 pieces along a row
     constexpr int kTileBytes = 64 * DP * 2;         // of K or V
     constexpr int kM = 32 * NW;
@@ -128,8 +132,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     for (int i = 0; i < DP / 32; ++i) {
         o[i] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
-    float unit = 0x1p-100f;  // int8: what the sums o are in units of
+    // Sums of 2^(s - ref) and 2^(s - ref) v. `ref`, in log2, follows the maximum of s (int8: of s and log2 of the
+    // tile's largest value scale, so that probability times scale stays as small) only when that has grown
+    // by more than 8: until then the probabilities stay below 256 and the sums as they are.
+    float ref = -INFINITY, l = 0.0f;
+    bool repair = false;  // values that are no numbers were taken out of tiles that not every row sees
 
     // loads: this lane's key of a tile is 16 x block + lane / 4
     constexpr int kBlocks = 4 / NW;  // 16-key blocks a wave loads
@@ -174,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         }
     };
     // int8 rows pass through registers, where they become 16-bit whole numbers
-    constexpr int kRaw = kQuant ? DP / 64 : 1;
+    constexpr int kRaw = kQuant ? (DP + 63) / 64 : 1;
     u32x4 raw[2][kBlocks][kRaw];
     float raw_scale[2][kBlocks];
     auto load_raw = [&](const KeyRow (&from)[kBlocks], const C *source, const float *scales, int which) {
@@ -184,7 +191,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             const C *p = (from[i].kept ? source + from[i].at : zeros) + 16 * (lane & 3);
 #pragma unroll
             for (int c = 0; c < kRaw; ++c) {
-                const bool in = kFull || 64 * c + 16 * (lane & 3) < a.head_dim;
+                const bool in = (kFull && DP % 64 == 0) || 64 * c + 16 * (lane & 3) < a.head_dim;
                 raw[which][i][c] = *reinterpret_cast<const u32x4 *>(in ? p + 64 * c : zeros);
             }
             const long long at = (static_cast<long long>(from[i].page) * a.kv_heads + kvh) * a.page.d +
@@ -192,7 +199,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             raw_scale[which][i] = *(from[i].kept ? scales + at : reinterpret_cast<const float *>(kAttnZeros));
         }
     };
-    auto store_raw = [&](int which, int tile) {
+    auto store_raw = [&](auto half, int which, int tile) {
+        typedef decltype(half) H;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
             const int block = wave * kBlocks + i;
@@ -200,12 +208,16 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             const int f = (((lane >> 3) & 1) << 1) | ((lane >> 4) & 1);
 #pragma unroll
             for (int c = 0; c < kRaw; ++c) {
-                half8 x[2];
+                H x[2];
                 int8_to_half(raw[which][i][c], x);
-                int8_t *at = to + (2 * c + ((lane >> 1) & 1)) * 1024;
+                const int place = 2 * c + ((lane >> 1) & 1);
+                if (DP % 64 != 0 && place >= kGroups) {
+                    continue;
+                }
+                int8_t *at = to + place * 1024;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    *reinterpret_cast<half8 *>(at + ((2 * (lane & 1) + e) ^ f) * 16) = x[e];
+                    *reinterpret_cast<H *>(at + ((2 * (lane & 1) + e) ^ f) * 16) = x[e];
                 }
             }
             if ((lane & 3) == 0) {
@@ -222,6 +234,22 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     const int v_at = 2 * kTileBytes + vr * 64 + (((((lane >> 4) & 1) << 1) | ((lane >> 1) & 1)) ^ fv) * 16 +
                      (lane & 1) * 8;
 
+    // Bit r of seen[t]: whether this lane's row sees the key of its score r of half t of a tile. Which keys are
+    // kept is looked up again: this is for tiles at the edges.
+    auto see = [&](int j0, uint32_t (&seen)[2]) {
+        const KeyRow kr = attn_key(a, table, kvh, j0 + lane, hi);
+        const unsigned long long kept = __ballot(kr.kept);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            // keys [row_lo, row_hi) of the 32, those kept, and of them this half-wave's: 4 of every 8
+            const int below = min(max(row_lo - j0 - 32 * t, 0), 32);
+            const int upto = min(max(row_hi - j0 - 32 * t, 0), 32);
+            uint32_t in = static_cast<uint32_t>(kept >> (32 * t));
+            in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
+            in >>= 4 * h;
+            seen[t] = (in & 0xfu) | ((in >> 4) & 0xf0u) | ((in >> 8) & 0xf00u) | ((in >> 12) & 0xf000u);
+        }
+    };
     auto scale_scores = [&](f32x16 (&st)[2], int parity) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -262,20 +290,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[n & 3]);
         const bool mixed = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) == 0 ||
                            j0 < all_lo || j0 + 64 > all_hi;
-        uint32_t seen[2] = {~0u, ~0u};
         if (mixed) {
-            // which of the tile's keys are kept is looked up again: tiles at the edges only
-            const KeyRow kr = attn_key(a, table, kvh, j0 + lane, hi);
-            const unsigned long long kept = __ballot(kr.kept);
+            uint32_t seen[2];
+            see(j0, seen);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                // keys [row_lo, row_hi) of the 32, those kept, and of them this half-wave's: 4 of every 8
-                const int below = min(max(row_lo - j0 - 32 * t, 0), 32);
-                const int upto = min(max(row_hi - j0 - 32 * t, 0), 32);
-                uint32_t in = static_cast<uint32_t>(kept >> (32 * t));
-                in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
-                in >>= 4 * h;
-                seen[t] = (in & 0xfu) | ((in >> 4) & 0xf0u) | ((in >> 8) & 0xf00u) | ((in >> 12) & 0xf000u);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     st[t][r] = (seen[t] >> r) & 1 ? st[t][r] : -INFINITY;
@@ -308,51 +327,41 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                 top = fmaxf(top, st[t][r]);
             }
         }
-        top = max_across_halves(top);
-        // m, in units of the unscaled product, follows the maximum only when that has grown by more than a
-        // factor of 2^8 in the probabilities: until then they stay below 256 and the sums as they are
-        top = (top - m) * a.scale > 8.0f ? top : m;
-        const float base_s = top == -INFINITY ? 0.0f : top * a.scale;
-        float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, a.scale, -base_s));
-        m = top;
-        l *= alpha;
-        float per_unit = 1.0f;
+        float want = max_across_halves(top) * a.scale;
         if constexpr (kQuant) {
-            // values are whole numbers here, their scales on the probabilities, in units of the largest
             const float mine = s_scale[1][kOdd][lane];
-            float most = __builtin_isfinite(mine) ? mine : 0.0f;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                most = fmaxf(most, __shfl_xor(most, off));
-            }
-            most = fmaxf(most, unit);
-            per_unit = 1.0f / most;
-            alpha *= unit * per_unit;
-            unit = most;
+            want += __builtin_amdgcn_logf(wave_max(fmaxf(__builtin_isfinite(mine) ? mine : 0.0f, 0x1p-100f)));
         }
+        want = want - ref > 8.0f ? want : ref;
+        const float base_s = want == -INFINITY ? 0.0f : want;
+        const float alpha = __builtin_amdgcn_exp2f(ref - base_s);
+        ref = want;
+        l *= alpha;
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
                 o[i] = o[i] * alpha;
             }
         }
-        half8 p[4];
+        prob8 p[4];
         float sum[2] = {0.0f, 0.0f};
         after[0] = 0.0f;
         after[1] = 0.0f;
-        constexpr int kProducts = DP / 8, kEach = 32 / kProducts;
-        auto use = [&](int k) {
+        constexpr int kProducts = DP / 8;
+        auto each = [&](int k, auto f) {  // the scores of step k
 #pragma unroll
-            for (int c = 0; c < kEach; ++c) {
-                const int t = (k * kEach + c) >> 4, r = (k * kEach + c) & 15;
-                float e = st[t][r];
-                sum[t] += e;
-                if constexpr (kQuant) {
-                    e *= s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)] * per_unit;
-                    e = (seen[t] >> r) & 1 ? e : 0.0f;
-                }
-                p[2 * t + (r >> 3)][r & 7] = static_cast<T>(e);
+            for (int c = 32 * k / kProducts; c < 32 * (k + 1) / kProducts; ++c) {
+                f(c >> 4, c & 15);
             }
+        };
+        auto use = [&](int t, int r) {
+            float e = st[t][r];
+            sum[t] += e;
+            if constexpr (kQuant) {
+                // 0 times a scale that is no number is 0: the row does not see the key
+                e = mul_zero_wins(e, s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)]);
+            }
+            p[2 * t + (r >> 3)][r & 7] = static_cast<P>(e);
         };
 #pragma unroll
         for (int k = 0; k < kProducts; ++k) {
@@ -365,17 +374,15 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             after[k & 1] =
                 mfma32(__builtin_bit_cast(half8, x[(k >> 2) & 1][k & 3]), q[k >> 1], after[k & 1]);
             // exponentials of this step's scores, and what the last step's are for
-#pragma unroll
-            for (int c = 0; c < kEach; ++c) {
-                const int t = (k * kEach + c) >> 4, r = (k * kEach + c) & 15;
+            each(k, [&](int t, int r) {
                 st[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
-            }
+            });
             if (k > 0) {
-                use(k - 1);
+                each(k - 1, use);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        use(kProducts - 1);
+        each(kProducts - 1, use);
         l += sum[0] + sum[1];
 
         if constexpr (!kQuant) {
@@ -390,36 +397,17 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
                            any_not_finite<T>(y[3]);
                 }
                 if (__syncthreads_or(bad)) {
-                    for (int u = 0; u < 4; ++u) {
-                        const uint32_t bits = seen[u >> 1] >> (8 * (u & 1));
-                        half8 see1;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            see1[e] = static_cast<T>((bits >> e) & 1 ? 1.0f : 0.0f);
-                        }
-#pragma unroll
-                        for (int i = 0; i < DP / 32; ++i) {
-                            u32x4 clean, code;
-                            split_not_finite<T>(value(i, u), clean, code);
-                            f32x16 count = 0.0f;
-                            count = mfma32(__builtin_bit_cast(half8, code), see1, count);
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                o[i][r] += not_finite_term(count[r]);
-                            }
-                        }
-                    }
-                    __syncthreads();
                     for (int i = 0; i < kTileBytes / 16; i += 64 * NW) {
                         u32x4 clean, code;
                         split_not_finite<T>(share[i], clean, code);
                         share[i] = clean;
                     }
+                    repair = true;
                     __syncthreads();
                 }
             }
         }
-        constexpr int kAhead = kGroups < 4 ? kGroups : 4, kParts = 4 * kGroups / kAhead;
+        constexpr int kAhead = kGroups % 4 == 0 ? 4 : kGroups % 3 == 0 ? 3 : 2, kParts = 4 * kGroups / kAhead;
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) {
             x[0][e] = value(e % kGroups, e / kGroups);
@@ -438,17 +426,17 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
             for (int e = 0; e < kAhead; ++e) {
                 const int at = k * kAhead + e;
                 o[at % kGroups] =
-                    mfma32(__builtin_bit_cast(half8, x[k & 1][e]), p[at / kGroups], o[at % kGroups]);
+                    mfma32(__builtin_bit_cast(prob8, x[k & 1][e]), p[at / kGroups], o[at % kGroups]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (kQuant) {
             scale_scores(after, kOdd ^ 1);
             if (more2) {
-                store_raw(0, kOdd);
+                store_raw(half8(), 0, kOdd);
             }
             if (more) {
-                store_raw(1, kOdd ^ 1);
+                store_raw(prob8(), 1, kOdd ^ 1);
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -466,11 +454,11 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         note_kept(1);
         if constexpr (kQuant) {
             load_raw(k_next, kbase, a.scale_k, 0);
-            store_raw(0, 1);
+            store_raw(half8(), 0, 1);
             load_raw(v_next, kbase, a.scale_k, 0);
             load_raw(v_next, vbase, a.scale_v, 1);
-            store_raw(0, 0);
-            store_raw(1, 0);
+            store_raw(half8(), 0, 0);
+            store_raw(prob8(), 1, 0);
         } else {
             load(v_next, kbase, 0, 0);
             load(k_next, kbase, 0, 1);
@@ -517,11 +505,54 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
         }
     }
 
+    if constexpr (!kQuant) {
+        if (repair) {
+            // The tiles that not every row sees once more: what their values that are no numbers make of the rows
+            // that do see them.
+            for (int j0 = lo; j0 < hi; j0 += 64) {
+                ask(j0);
+                resolve();
+                load(k_next, vbase, 1, 0);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                bool all_kept = true;
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i) {
+                    all_kept &= k_next[i].kept;
+                }
+                if (__syncthreads_or(!all_kept) || j0 < all_lo || j0 + 64 > all_hi) {
+                    uint32_t seen[2];
+                    see(j0, seen);
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t bits = seen[u >> 1] >> (8 * (u & 1));
+                        half8 see1;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            see1[e] = static_cast<T>((bits >> e) & 1 ? 1.0f : 0.0f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < DP / 32; ++i) {
+                            const int8_t *at = lds + v_at + (u * kGroups + i) * 1024;
+                            const u32x2 x0 = lds_read_column4(at), x1 = lds_read_column4(at + 512);
+                            u32x4 clean, code;
+                            split_not_finite<T>(u32x4{x0[0], x0[1], x1[0], x1[1]}, clean, code);
+                            f32x16 count = 0.0f;
+                            count = mfma32(__builtin_bit_cast(half8, code), see1, count);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                o[i][r] += not_finite_term(count[r]);
+                            }
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+        }
+    }
+
     if (!live) {
         return;
     }
     l += __shfl_xor(l, 32);
-    const float m2 = m == -INFINITY ? m : m * a.scale;
     const long long part = splits == 1 ? -1
                                        : 2ll * a.few_workgroups * kAttnFewRows +
                                              (static_cast<long long>(split) * a.q_tokens + s.first + token) *
@@ -531,14 +562,8 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attn_tile_kernel(A
     for (int i = 0; i < DP / 32; ++i) {
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            float out[4] = {o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
-            if constexpr (kQuant) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    out[e] *= unit;
-                }
-            }
-            attn_put<T, 4>(a, part, s.first + token, head, 32 * i + 2 * r + 4 * h, out, m2, l);
+            const float out[4] = {o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            attn_put<T, 4>(a, part, s.first + token, head, 32 * i + 2 * r + 4 * h, out, ref, l);
         }
     }
 }
