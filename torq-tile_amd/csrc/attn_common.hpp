@@ -289,12 +289,14 @@ __device__ __forceinline__ float max_across_halves(float x)
     return fmaxf(x, y);
 }
 
-// x * y, and 0 where x or y is 0, whatever the other is.
-__device__ __forceinline__ float mul_zero_wins(float x, float y)
+// x * y, and 0 where x or y is 0, whatever the other is. `sum` holds a sum that x has gone into: it keeps the
+// instruction behind that addition, since the compiler does not insert the wait state that a result of exp2
+// needs before an instruction in inline asm.
+__device__ __forceinline__ float mul_zero_wins(float x, float y, float &sum)
 {
     float z = 0.0f;
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(z) : "v"(x), "v"(y));
+    asm("v_mul_legacy_f32 %0, %2, %3" : "=v"(z), "+v"(sum) : "v"(x), "v"(y));
 #endif
     return z;
 }

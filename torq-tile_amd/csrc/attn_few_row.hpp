@@ -33,6 +33,9 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
     constexpr bool kQuant = Tile::kQuant;
+    // the second product's type: int8 values are whole numbers in f16
+    typedef typename std::conditional<kQuant, _Float16, T>::type P;
+    typedef typename Half8<P>::type prob8;
     constexpr int kPieces = Tile::kPieces, kSteps = DP / 32, kStride = Tile::kStride;
     constexpr int kElems = 16 / static_cast<int>(sizeof(C));  // elements of a piece
     __shared__ __attribute__((aligned(16))) char lds[kAttnFewRowWaves * Tile::kWaveBytes];
@@ -115,8 +118,9 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
     for (int i = 0; i < DP / 16; ++i) {
         o[i] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
-    float vmax = 0x1p-100f;  // int8: what the sums o are in units of
+    // sums of 2^(s - ref) and 2^(s - ref) v; `ref` (log2) is the maximum of s so far, for int8 of s and log2 of
+    // the tile's largest value scale, so that probability times scale stays below 1
+    float ref = -INFINITY, l = 0.0f;
 
     // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
     u32x4 kx[2][kPieces], vx[2][kPieces];
@@ -187,29 +191,23 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 if constexpr (kQuant) {
-                    half8 h[2];
+                    prob8 h[2];
                     int8_to_half(vx[t][i], h);
-                    *reinterpret_cast<half8 *>(row + 128 * i + 32 * g) = h[0];
-                    *reinterpret_cast<half8 *>(row + 128 * i + 32 * g + 16) = h[1];
+                    *reinterpret_cast<prob8 *>(row + 128 * i + 32 * g) = h[0];
+                    *reinterpret_cast<prob8 *>(row + 128 * i + 32 * g + 16) = h[1];
                 } else {
                     *reinterpret_cast<u32x4 *>(row + 64 * i + 16 * g) = vx[t][i];
                 }
             }
         }
         float *scales = reinterpret_cast<float *>(mine + 32 * kStride);
-        float unit = vmax;
+        float scale_log = 0.0f;
         if constexpr (kQuant) {
             if (lane < 32) {
                 scales[lane] = sk;
                 scales[32 + lane] = sv;
             }
-            // the largest finite scale of a value so far
-            float top = __builtin_isfinite(sv) ? sv : 0.0f;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                top = fmaxf(top, __shfl_xor(top, off));
-            }
-            unit = fmaxf(unit, top);
+            scale_log = __builtin_amdgcn_logf(wave_max(fmaxf(__builtin_isfinite(sv) ? sv : 0.0f, 0x1p-100f)));
         }
         const unsigned long long kept0 = __ballot(kept[0]), kept1 = __ballot(kept[1]);
         const uint32_t keptmask = static_cast<uint32_t>(kept0 & 0xffff) |
@@ -239,7 +237,7 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         }
 
         // softmax of this lane's 8 keys: 16 t + 4 g + r
-        float top = m;
+        float top = -INFINITY;
         uint32_t seen = 0, in = keptmask;
         {
             const int below = min(max(row_lo - jt, 0), 32), upto = min(max(row_hi - jt, 0), 32);
@@ -267,17 +265,12 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(ref, top + scale_log);
         const float base = top == -INFINITY ? 0.0f : top;
-        float alpha = __builtin_amdgcn_exp2f(m - base);
-        m = top;
+        const float alpha = __builtin_amdgcn_exp2f(ref - base);
+        ref = top;
         l *= alpha;
-        // int8: values as whole numbers, their scales on the probabilities, in units of the largest scale
-        const float per_unit = kQuant ? 1.0f / unit : 1.0f;
-        if constexpr (kQuant) {
-            alpha *= vmax * per_unit;
-            vmax = unit;
-        }
-        half8 p;
+        prob8 p;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 vsc = 1.0f;
@@ -289,9 +282,10 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
                 float e = __builtin_amdgcn_exp2f(st[t][r] - base);
                 l += e;
                 if constexpr (kQuant) {
-                    e = ((seen >> (4 * t + r)) & 1) ? e * (vsc[r] * per_unit) : 0.0f;
+                    // 0 times a scale that is no number is 0: the row does not see the key
+                    e = mul_zero_wins(e, vsc[r], l);
                 }
-                p[4 * t + r] = static_cast<T>(e);
+                p[4 * t + r] = static_cast<P>(e);
             }
         }
         const char *columns = mine + (4 * g + (col >> 2)) * kStride + 8 * (lane & 3);
@@ -335,7 +329,7 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         // O^T
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            o[i] = mfma16(__builtin_bit_cast(half8, value(i)), p, o[i]);
+            o[i] = mfma16(__builtin_bit_cast(prob8, value(i)), p, o[i]);
         }
     }
 
@@ -346,10 +340,10 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
     float *mo = reinterpret_cast<float *>(mine);  // [16][DP]
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-        *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = kQuant ? o[i] * vmax : o[i];
+        *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = o[i];
     }
     if (lane < 16) {
-        s_m[wave][lane] = m;
+        s_m[wave][lane] = ref;
         s_l[wave][lane] = l;
     }
     __syncthreads();

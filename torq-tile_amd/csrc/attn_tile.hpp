@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(At
             sum[t] += e;
             if constexpr (kQuant) {
                 // 0 times a scale that is no number is 0: the row does not see the key
-                e = mul_zero_wins(e, s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)]);
+                e = mul_zero_wins(e, s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)], sum[t]);
             }
             p[2 * t + (r >> 3)][r & 7] = static_cast<P>(e);
         };
