@@ -1,10 +1,14 @@
-// Attention of new tokens over a paged cache on gfx950: the entry points and their checks.
+// Attention of new tokens over a paged cache on gfx950: the checks of a call, what it launches, and the entry
+// points of one type (each in a file of its own: the kernels' instances take the compiler a minute).
+#pragma once
+
 #include "attn_common.hpp"
 #include "attn_few_row.hpp"
 #include "attn_join.hpp"
 #include "attn_tile.hpp"
 #include "tqt_attn_paged_gfx950.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -27,12 +31,18 @@ const char *attn_size_error(const tqt_attn_paged_params *p)
     if (p->kv.head_dim == 0 || p->kv.kv_heads == 0 || p->q_heads % p->kv.kv_heads != 0) {
         return "q_heads % kv_heads != 0";
     }
-    if (p->max_q_len * (p->q_heads / p->kv.kv_heads) >= top) {
-        return "max_q_len * (q_heads / kv_heads) exceeds 2^31-1";
+    const size_t group = p->q_heads / p->kv.kv_heads;
+    if (p->max_q_len * group >= top - 256) {
+        return "max_q_len * (q_heads / kv_heads) too large";
     }
-    if (static_cast<long long>(p->batch) * static_cast<long long>(p->kv.kv_heads) *
-            static_cast<long long>(p->max_kv_len / kAttnFewRowUnit + 1) >= (1ll << 31)) {
-        return "batch * kv_heads * max_kv_len too large";
+    // units of the few-row kernel in 32 bits, and grids of fewer than 2^32 work-items
+    if (p->batch * p->kv.kv_heads * (p->max_kv_len / kAttnFewRowUnit + 1) >= top ||
+        p->batch * p->kv.kv_heads * kAttnFewRows >= (1u << 26)) {
+        return "batch * kv_heads or batch * kv_heads * max_kv_len too large";
+    }
+    if (attn_tiles(p->batch, p->q_tokens, p->max_q_len, group) * static_cast<long long>(p->kv.kv_heads) >=
+        (1 << 24)) {
+        return "too many rows";
     }
     return nullptr;
 }
@@ -201,7 +211,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         check_launch(where);
     }
     if (plan.run_tile) {
-        const dim3 grid(a.kv_heads, static_cast<unsigned>(plan.tiles), plan.tile.splits);
+        const dim3 grid(static_cast<unsigned>(plan.tiles * a.kv_heads), plan.tile.splits);
         by_head_dim<64, 96, 128, 192, 256>(a.head_dim, [&](auto dp, auto full) {
             hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value>), grid, dim3(256), 0, stream,
                                a);
@@ -213,7 +223,6 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         const int each = static_cast<int>(plan.few_tokens), few = plan.run_few ? a.batch * each : 0;
         const int rows = few + (join_tile ? a.q_tokens : 0);
         const long long items = static_cast<long long>(rows) * a.q_heads;
-        TQT_REQUIRE(items < (1ll << 31), "too many rows");
         if (plan.few_many || plan.tile.splits > kAttnJoinManyParts) {
             hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3(static_cast<unsigned>(items)), dim3(256), 0,
                                stream, a, few, each, rows);
@@ -228,19 +237,6 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
 
 }  // namespace
 }  // namespace tqt
-
-using namespace tqt;
-
-extern "C" {
-
-size_t tqt_get_workspace_size_attn_paged_gfx950(const struct tqt_attn_paged_params *params)
-{
-    if (params == nullptr || attn_size_error(params) != nullptr || attn_empty(params)) {
-        return 0;
-    }
-    const AttnPlan plan = attn_plan(params);
-    return static_cast<size_t>(plan.parts) * (params->kv.head_dim + 2) * 4;
-}
 
 #define TQT_ATTN_ENTRIES(NAME, T, C)                                                                  \
     const char *tqt_get_error_attn_paged_##NAME##_gfx950(const struct tqt_attn_paged_params *params)  \
@@ -259,9 +255,3 @@ size_t tqt_get_workspace_size_attn_paged_gfx950(const struct tqt_attn_paged_para
         }                                                                                             \
     }
 
-TQT_ATTN_ENTRIES(f16_f16, _Float16, _Float16)
-TQT_ATTN_ENTRIES(bf16_bf16, __bf16, __bf16)
-TQT_ATTN_ENTRIES(f16_qsi8dx, _Float16, int8_t)
-TQT_ATTN_ENTRIES(bf16_qsi8dx, __bf16, int8_t)
-
-}  // extern "C"

@@ -74,9 +74,12 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(At
     __shared__ __attribute__((aligned(16))) int s_kept[4][4];              // [tile % 4][16-key block]
     __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [K, V][tile % 2]
 
-    const int kvh = blockIdx.x, split = blockIdx.z;
+    // the key heads of a tile side by side: with 8 (or a multiple), a head's tiles are all on one XCD, whose L2
+    // its keys then pass once for them
+    const int split = blockIdx.y, index = static_cast<int>(blockIdx.x) / a.kv_heads;
+    const int kvh = static_cast<int>(blockIdx.x) - index * a.kv_heads;
     int b, tile;
-    if (!attn_find_tile(a, blockIdx.y, kM, b, tile)) {
+    if (!attn_find_tile(a, index, kM, b, tile)) {
         return;
     }
     b = __builtin_amdgcn_readfirstlane(b);
