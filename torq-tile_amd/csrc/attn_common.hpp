@@ -65,6 +65,18 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int b)
     return s;
 }
 
+// One lane's sequence for the whole wave.
+__device__ __forceinline__ AttnSeq attn_pick(const AttnSeq &x, int at)
+{
+    AttnSeq s;
+    s.first = __builtin_amdgcn_readlane(x.first, at);
+    s.q_len = __builtin_amdgcn_readlane(x.q_len, at);
+    s.kv_len = __builtin_amdgcn_readlane(x.kv_len, at);
+    s.nq = __builtin_amdgcn_readlane(x.nq, at);
+    s.pos0 = __builtin_amdgcn_readlane(x.pos0, at);
+    return s;
+}
+
 // The keys [lo, hi) that the query at `pos` may see.
 __device__ __forceinline__ void attn_bounds(const AttnArgs &a, const AttnSeq &s, int pos, int &lo, int &hi)
 {
@@ -185,11 +197,7 @@ __device__ __forceinline__ int few_row_run(const AttnArgs &a, int lane, int &tot
 // One lane's sequence and work for the whole wave.
 __device__ __forceinline__ void few_row_pick(const FewRowBatch &x, int at, AttnSeq &s, FewRowWork &w)
 {
-    s.first = __builtin_amdgcn_readlane(x.s.first, at);
-    s.q_len = __builtin_amdgcn_readlane(x.s.q_len, at);
-    s.kv_len = __builtin_amdgcn_readlane(x.s.kv_len, at);
-    s.nq = __builtin_amdgcn_readlane(x.s.nq, at);
-    s.pos0 = __builtin_amdgcn_readlane(x.s.pos0, at);
+    s = attn_pick(x.s, at);
     w.first = __builtin_amdgcn_readlane(x.work.first, at);
     w.last = __builtin_amdgcn_readlane(x.work.last, at);
     w.units = __builtin_amdgcn_readlane(x.work.units, at);

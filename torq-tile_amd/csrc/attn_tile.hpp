@@ -29,31 +29,25 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c)
 
 // The workgroup's sequence and tile among all of the batch's: tiles of a sequence are taken from its last
 // rows on, which see the most keys.
-__device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int m, int &b, int &tile)
+__device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int m, int &b, int &tile, AttnSeq &s)
 {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < a.batch) {
-            const AttnSeq s = attn_seq(a, b0 + lane);
-            const int rows = s.nq * static_cast<int>(a.group.d);
-            n = rows > a.few_rows ? (rows + m - 1) / m : 0;
-        }
-        int upto = n;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int x = __shfl_up(upto, off);
-            upto += lane >= off ? x : 0;
-        }
-        const unsigned long long past = __ballot(before + upto > index);
+        const bool in = b0 + lane < a.batch;
+        const AttnSeq mine = attn_seq(a, in ? b0 + lane : 0);
+        const int rows = mine.nq * static_cast<int>(a.group.d);
+        const int n = in && rows > a.few_rows ? (rows + m - 1) / m : 0;
+        const int upto = before + wave_inclusive_sum(n, lane, a.batch - b0);
+        const unsigned long long past = __ballot(upto > index);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
             b = b0 + at;
-            tile = before + __shfl(upto, at) - 1 - index;
+            tile = __builtin_amdgcn_readlane(upto, at) - 1 - index;
+            s = attn_pick(mine, at);
             return true;
         }
-        before += __shfl(upto, 63);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -79,12 +73,10 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(At
     const int split = blockIdx.y, index = static_cast<int>(blockIdx.x) / a.kv_heads;
     const int kvh = static_cast<int>(blockIdx.x) - index * a.kv_heads;
     int b, tile;
-    if (!attn_find_tile(a, index, kM, b, tile)) {
+    AttnSeq s;
+    if (!attn_find_tile(a, index, kM, b, tile, s)) {
         return;
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    const AttnSeq s = attn_seq(a, b);
     const int group = static_cast<int>(a.group.d);
     int first, last;
     attn_tile_span(a, s, tile, kM, first, last);
