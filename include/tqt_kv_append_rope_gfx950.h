@@ -21,8 +21,8 @@
  *
  * head_dim is a multiple of 16 up to 256; k, v and their strides keep rows on the 16-byte grid; K, V
  * and Q take any strides and alignment (rows on the 16-byte grid with rotary_dim a multiple of 16 are
- * the fast ones). Q and Q_out may be the same tensor (of one type, with the same strides). Pointers are device pointers;
- * conventions as in tqt_rope_gfx950.h.
+ * the fast ones). Q and Q_out may be the same tensor (of one type, with the same strides). Pointers are
+ * device pointers; conventions as in tqt_rope_gfx950.h.
  */
 #ifndef TQT_KV_APPEND_ROPE_GFX950_H
 #define TQT_KV_APPEND_ROPE_GFX950_H

@@ -1,6 +1,6 @@
-// Joining the parts that several workgroups have of a row: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, with
-// the parts taken in the order of the keys. Bound by latency at few rows, by the parts' bytes (at most 3% of the
-// cache's at 256 keys a split) at many.
+// Joining the parts that several workgroups have of a row: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s,
+// with the parts taken in the order of the keys. Bound by latency at few rows (the batch's lengths, then the
+// parts), by the parts' bytes at many.
 #pragma once
 
 #include "attn_common.hpp"
@@ -8,23 +8,26 @@
 namespace tqt {
 namespace {
 
-// kWaves waves per row, head_dim / 4 threads along it and as many such groups as fit over the splits: one wave
-// (four rows a workgroup) where the parts are few, four where they are many. The first `few` rows of a head are
-// those that the few-row kernel may have (`each` tokens of every sequence), the others are all rows of Q, for
-// the tile kernel's.
-template <typename T, int kWaves>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int each, int rows)
+// A row's parts: part0, then from part1 on every `step` rows of the workspace.
+struct JoinRow
 {
-    __shared__ f32x4 s_acc[kWaves > 1 ? 256 : 1];
-    __shared__ float s_sum[kWaves > 1 ? 256 : 1];
-    const int tid = threadIdx.x, lane = tid & 63;
+    int parts;
+    long long part0, part1, step;
+    int token;  // row of Q
+};
+
+__device__ __forceinline__ long long join_part(const JoinRow &j, int k)
+{
+    return k == 0 ? j.part0 : j.part1 + (k - 1) * j.step;
+}
+
+// The parts of row `at_row` (the same for the whole wave) and query head `head` (a lane's own). The first `few`
+// rows are those that the few-row kernel may have (`each` tokens of every sequence), the others are all rows
+// of Q, for the tile kernel's. parts <= 1: nothing to join.
+__device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each, int at_row, int head, int lane)
+{
+    JoinRow j = {0, 0, 0, 0, 0};
     const int heads = static_cast<int>(a.group.d);
-    const int item = __builtin_amdgcn_readfirstlane(
-        static_cast<int>(blockIdx.x) * (4 / kWaves) + (kWaves > 1 ? 0 : tid >> 6));
-    if (item >= rows * a.q_heads) {
-        return;
-    }
-    const int at_row = item / a.q_heads, head = item - at_row * a.q_heads;
     const bool tiles = at_row >= few;
     AttnSeq s;
     int token, units = 0, run = 1, before = 0;
@@ -38,7 +41,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int
             b = here != 0 ? x0 + __builtin_ctzll(here) : -1;
         }
         if (b < 0) {
-            return;
+            return j;
         }
         s = attn_seq(a, b);
         token -= s.first;
@@ -58,41 +61,87 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int
         before = __builtin_amdgcn_readlane(batch.upto, b & 63) - units * a.kv_heads;
     }
     if (token >= s.nq || (s.nq * heads > a.few_rows) != tiles) {
-        return;
+        return j;
     }
-    // the row's parts: part0, then from part1 on every `step` rows of the workspace
+    j.token = s.first + token;
     uint32_t in_group;
     const int kvh = static_cast<int>(fast_div(head, a.group, in_group));
-    int parts;
-    long long part0, part1, step;
+    const int r = token * heads + static_cast<int>(in_group);
     if (tiles) {
         int first, last;
-        attn_tile_span(a, s, (token * heads + static_cast<int>(in_group)) / a.tile_rows, a.tile_rows, first,
-                       last);
-        parts = attn_splits(first, last, a.tile_chunk);
-        step = static_cast<long long>(a.q_tokens) * a.q_heads;
-        part0 = 2ll * a.few_workgroups * kAttnFewRows +
-                static_cast<long long>(s.first + token) * a.q_heads + head;
-        part1 = part0 + step;
+        attn_tile_span(a, s, r / a.tile_rows, a.tile_rows, first, last);
+        j.parts = attn_splits(first, last, a.tile_chunk);
+        j.step = static_cast<long long>(a.q_tokens) * a.q_heads;
+        j.part0 = 2ll * a.few_workgroups * kAttnFewRows + static_cast<long long>(j.token) * a.q_heads + head;
+        j.part1 = j.part0 + j.step;
     } else {
         before += kvh * units;
         const int w0 = before / run, w1 = (before + units - 1) / run;
-        parts = w1 - w0 + 1;
-        const int r = token * heads + static_cast<int>(in_group);
-        part0 = (2ll * w0 + 1) * kAttnFewRows + r;
-        part1 = 2ll * (w0 + 1) * kAttnFewRows + r;
-        step = 2 * kAttnFewRows;
+        j.parts = w1 - w0 + 1;
+        j.part0 = (2ll * w0 + 1) * kAttnFewRows + r;
+        j.part1 = 2ll * (w0 + 1) * kAttnFewRows + r;
+        j.step = 2 * kAttnFewRows;
     }
-    if (parts == 1) {
+    return j;
+}
+
+// Few parts: a wave takes as many heads of a row as fit at 4 elements a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few, int each, int rows)
+{
+    const int lane = threadIdx.x & 63;
+    const int across = a.head_dim / 4, per_wave = 64 / across;
+    const int blocks = (a.q_heads + per_wave - 1) / per_wave;
+    const int item =
+        __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
+    if (item >= rows * blocks) {
         return;
     }
-    token += s.first;
-    const int across = a.head_dim / 4, groups = 64 * kWaves / across;
-    const int me = kWaves > 1 ? tid : lane;
-    const int group = me / across, at = me - group * across;
+    const int at_row = item / blocks, group = lane / across, at = lane - group * across;
+    const int head = (item - at_row * blocks) * per_wave + group;
+    const bool mine = group < per_wave && head < a.q_heads;
+    const JoinRow j = join_row(a, few, each, at_row, mine ? head : 0, lane);
+    if (!mine || j.parts <= 1) {
+        return;
+    }
     float m = -INFINITY;
-    for (int k = lane; k < parts; k += 64) {
-        m = fmaxf(m, a.part_ml[2 * (k == 0 ? part0 : part1 + (k - 1) * step)]);
+#pragma unroll 4
+    for (int k = 0; k < j.parts; ++k) {
+        m = fmaxf(m, a.part_ml[2 * join_part(j, k)]);
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    f32x4 acc = 0.0f;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < j.parts; ++k) {
+        const long long r = join_part(j, k);
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
+        sum += a.part_ml[2 * r + 1] * f;
+        acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
+    }
+    const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
+    attn_put<T, 4>(a, -1, j.token, head, 4 * at, out, m, sum);
+}
+
+// Many parts: a workgroup takes one row, head_dim / 4 threads along it and as many such groups as fit over the
+// parts.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_many_kernel(AttnArgs a, int few, int each)
+{
+    __shared__ f32x4 s_acc[256];
+    __shared__ float s_sum[256];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int at_row = static_cast<int>(blockIdx.x) / a.q_heads;
+    const int head = static_cast<int>(blockIdx.x) - at_row * a.q_heads;
+    const JoinRow j = join_row(a, few, each, at_row, head, lane);
+    if (j.parts <= 1) {
+        return;
+    }
+    const int across = a.head_dim / 4, groups = 256 / across;
+    const int group = tid / across, at = tid - group * across;
+    float m = -INFINITY;
+    for (int k = lane; k < j.parts; k += 64) {
+        m = fmaxf(m, a.part_ml[2 * join_part(j, k)]);
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
@@ -103,44 +152,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int few, int
     float sum = 0.0f;
     if (group < groups) {
         // consecutive parts to one group: the sums' order is that of the keys
-        const int per = (parts + groups - 1) / groups;
-        const int k1 = min(parts, (group + 1) * per);
+        const int per = (j.parts + groups - 1) / groups;
+        const int k1 = min(j.parts, (group + 1) * per);
 #pragma unroll 8
         for (int k = group * per; k < k1; ++k) {
-            const long long r = k == 0 ? part0 : part1 + (k - 1) * step;
+            const long long r = join_part(j, k);
             const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
             sum += a.part_ml[2 * r + 1] * f;
             acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
         }
     }
-    if constexpr (kWaves > 1) {
-        s_acc[tid] = acc;
-        s_sum[tid] = sum;
-        __syncthreads();
-    }
-    const f32x4 own = acc;
-    const float own_sum = sum;
-    for (int k = 1; k < groups; ++k) {
-        if constexpr (kWaves > 1) {
-            if (tid < across) {
-                acc += s_acc[k * across + tid];
-                sum += s_sum[k * across + tid];
-            }
-        } else {
-            // every group's sums in turn, to the first
-            const int from = k * across + at;
-            sum += __shfl(own_sum, from);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[e] += __shfl(own[e], from);
-            }
-        }
-    }
-    if (me >= across) {
+    s_acc[tid] = acc;
+    s_sum[tid] = sum;
+    __syncthreads();
+    if (tid >= across) {
         return;
     }
+    for (int k = 1; k < groups; ++k) {
+        acc += s_acc[k * across + tid];
+        sum += s_sum[k * across + tid];
+    }
     const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
-    attn_put<T, 4>(a, -1, token, head, 4 * at, out, m, sum);
+    attn_put<T, 4>(a, -1, j.token, head, 4 * at, out, m, sum);
 }
 
 }  // namespace
