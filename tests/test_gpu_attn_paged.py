@@ -228,6 +228,29 @@ def test_not_finite_reaches_only_who_sees_it(gpu, name, which, bad, window):
         assert torch.isnan(b.out[seen][:, 2:]).all()
 
 
+@pytest.mark.parametrize("name", ["f16_qsi8dx", "bf16_qsi8dx"])
+@pytest.mark.parametrize("which", ["dsk", "dsv"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("lengths,at", [((90, 150), 101), ((4, 150), 147)])
+def test_scale_not_finite_reaches_only_who_sees_it(gpu, name, which, bad, lengths, at):
+    """The scale of one key is no number: rows that see the key are none either, the others as ever."""
+    c = Case(name, [lengths], 4, 2, 64, window=30)
+    getattr(c, which)[c.table[0, at // 16], 1, at % 16] = bad
+    c.run()
+    see = R.visible(*lengths, True, 30)[:, at]
+    k, v, kept = c.keys(0)
+    want = R.attention(c.q, k, v, R.visible(*lengths, True, 30), c.scale)
+    tol, tol_lse = R.attention_bound(c.kind, c.d, *want)
+    out, lse = R.host(c.out), R.host(c.lse)
+    fine = np.ones(out.shape[:2], bool)
+    fine[see, 2:] = False  # the heads that read key head 1
+    assert (np.abs(out - want[0]) <= tol)[fine].all()
+    assert (np.abs(lse - want[1]) <= tol_lse)[fine].all()
+    # an infinite key makes a score of either sign: a row that has -infinity there is as without the key
+    if which == "dsv" or np.isnan(bad):
+        assert not np.isfinite(out[~fine]).all(axis=-1).any()
+
+
 @pytest.mark.parametrize("name", ["f16_f16", "bf16_bf16"])
 @pytest.mark.parametrize("q_len", [1, 40])
 def test_scores_at_the_type_limits(gpu, name, q_len):
@@ -268,6 +291,19 @@ def test_mixed_batch_and_strides(gpu, name):
     Case(name, lengths, 8, 2, 80, pad=16).run().check()
     Case(name, lengths, 3, 3, 128, pad=8).run().check()
     Case(name, lengths, 48, 1, 64).run().check()
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("decode", [True, False])
+def test_many_sequences(gpu, name, decode):
+    """More sequences than a wave has lanes, of all kinds, empty ones among them."""
+    rng = np.random.default_rng(9)
+    lengths = []
+    for b in range(203):
+        kv = int(rng.choice([0, 1, 7, 40, 129, 300]))
+        q = 1 if decode or b % 5 else int(rng.integers(0, 60))
+        lengths.append((q, kv))
+    Case(name, lengths, 4, 2, 64).run().check()
 
 
 @pytest.mark.parametrize("name", NAMES)
