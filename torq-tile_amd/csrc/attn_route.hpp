@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cstddef>
 #include <cstdint>
 
 namespace tqt {
@@ -37,6 +38,10 @@ constexpr int kAttnJoinManyParts = 16;
 // are fewer, their keys are split, in spans of at least 256 (512 tokens of 32 / 8 heads over 8000 keys: 128
 // tiles in four parts, 88 us and 10 of join).
 constexpr int kAttnTileRows = 128;
+constexpr int attn_tile_per_cu(size_t cache_element, int head_dim)
+{
+    return head_dim > 128 ? 1 : head_dim > 64 || cache_element == 1 ? 2 : 3;
+}
 constexpr long long kAttnTileWorkgroups = 512;
 constexpr int kAttnTileLeast = 256;
 

@@ -57,7 +57,7 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
 }
 
 template <typename T, typename C, int DP, int NW, bool kFull>
-__global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(AttnArgs a)
+__global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn_tile_kernel(AttnArgs a)
 {
     constexpr bool kQuant = std::is_same<C, int8_t>::value;
     // The second product's type: int8 values are whole numbers in f16, which costs less than bf16 and rounds
@@ -313,8 +313,9 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(At
             return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
         u32x4 x[2][4];
+        constexpr int kKeys = attn_tile_per_cu(sizeof(C), DP) > 2 ? 2 : 4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kKeys; ++e) {
             x[0][e] = key(e >> 1, e & 1);
         }
 
@@ -360,24 +361,30 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void attn_tile_kernel(At
                 // 0 times a scale that is no number is 0: the row does not see the key
                 e = mul_zero_wins(e, s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)], sum[t]);
             }
-            p[2 * t + (r >> 3)][r & 7] = static_cast<P>(e);
+            prob8 &to = p[2 * t + (r >> 3)];
+            to[r & 7] = static_cast<P>(e);
+            if ((r & 7) == 7) {
+                asm volatile("" : "+v"(to));
+            }
         };
 #pragma unroll
         for (int k = 0; k < kProducts; ++k) {
-            if (k % 4 == 0 && k + 4 < kProducts) {
+            if (k % kKeys == 0 && k + kKeys < kProducts) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[((k >> 2) + 1) & 1][e] = key((k >> 1) + 2 + (e >> 1), e & 1);
+                for (int e = 0; e < kKeys; ++e) {
+                    x[(k / kKeys + 1) & 1][e] = key((k + kKeys + e) >> 1, e & 1);
                 }
             }
             after[k & 1] =
-                mfma32(__builtin_bit_cast(half8, x[(k >> 2) & 1][k & 3]), q[k >> 1], after[k & 1]);
+                mfma32(__builtin_bit_cast(half8, x[k / kKeys & 1][k % kKeys]), q[k >> 1], after[k & 1]);
             // exponentials of this step's scores, and what the last step's are for
             each(k, [&](int t, int r) {
                 st[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
             });
             if (k > 0) {
                 each(k - 1, use);
+                // holds them here: the compiler would sink all of it below the products
+                asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));
             }
             __builtin_amdgcn_sched_barrier(0);
         }
