@@ -220,6 +220,14 @@ struct PageAsked
     int page, offset;
 };
 
+// For a key below the sequence's length.
+__device__ __forceinline__ PageAsked attn_page_of(const AttnArgs &a, const int32_t *table, int j)
+{
+    uint32_t offset;
+    const int page = table[fast_div(static_cast<uint32_t>(j), a.page, offset)];
+    return {page, static_cast<int>(offset)};
+}
+
 __device__ __forceinline__ PageAsked attn_ask_page(const AttnArgs &a, const int32_t *table, int j, int hi)
 {
     PageAsked r;

@@ -145,14 +145,15 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     auto ask = [&](int j0) {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
-            asked[i] = attn_ask_page(a, table, j0 + 16 * (wave * kBlocks + i) + (lane >> 2), hi);
+            asked[i] = attn_page_of(a, table, min(j0 + 16 * (wave * kBlocks + i) + (lane >> 2), hi - 1));
         }
     };
-    auto resolve = [&]() {
+    auto resolve = [&](int j0) {
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
             v_next[i] = k_next[i];
             k_next[i] = attn_key(a, asked[i], kvh);
+            k_next[i].kept &= j0 + 16 * (wave * kBlocks + i) + (lane >> 2) < hi;
         }
     };
     auto note_kept = [&](int tile) {
@@ -262,33 +263,42 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             }
         }
     };
+    auto max_of = [&](const f32x16 (&st)[2]) {
+        float x = st[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x = fmaxf(x, st[t][r]);
+            }
+        }
+        return max_across_halves(x);
+    };
+    float top = 0.0f;   // of a tile's scores, masks left out
+    bool kept = false;  // whether all of its keys are on pages that are kept
     // One tile: its scores are in `st`; the next one's go to `after`, their products between the exponentials
     // of this one's (a wave issues in order, so that the two kinds have to alternate). `odd`: the tile's
     // number's lowest bit.
     auto step = [&](f32x16 (&st)[2], f32x16 (&after)[2], int j0, int n, auto odd) {
         constexpr int kOdd = decltype(odd)::value;
         const bool more = j0 + 64 < hi, more2 = j0 + 128 < hi;
-        if constexpr (kQuant) {
-            if (more2) {
+        if (more2) {
+            if constexpr (kQuant) {
                 load_raw(k_next, kbase, a.scale_k, 0);
-                note_kept(n + 2);
-            }
-            if (more) {
-                load_raw(v_next, vbase, a.scale_v, 1);
-            }
-        } else {
-            if (more2) {
+            } else {
                 load(k_next, kbase, 0, kOdd);
-                note_kept(n + 2);
             }
-            if (more) {
+            note_kept(n + 2);
+        }
+        if (more) {
+            if constexpr (kQuant) {
+                load_raw(v_next, vbase, a.scale_v, 1);
+            } else {
                 load(v_next, vbase, 1, kOdd ^ 1);
             }
         }
         ask(j0 + 192);
-        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[n & 3]);
-        const bool mixed = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) == 0 ||
-                           j0 < all_lo || j0 + 64 > all_hi;
+        const bool mixed = !kept || j0 < all_lo || j0 + 64 > all_hi;
         if (mixed) {
             uint32_t seen[2];
             see(j0, seen);
@@ -299,6 +309,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                     st[t][r] = (seen[t] >> r) & 1 ? st[t][r] : -INFINITY;
                 }
             }
+            top = max_of(st);
         }
 
         // operands are read from LDS a group of four ahead of their products
@@ -319,15 +330,8 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             x[0][e] = key(e >> 1, e & 1);
         }
 
-        float top = st[0][0];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                top = fmaxf(top, st[t][r]);
-            }
-        }
-        float want = max_across_halves(top) * a.scale;
+        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[(n + 1) & 3]);
+        float want = top * a.scale;
         if constexpr (kQuant) {
             const float mine = s_scale[1][kOdd][lane];
             want += __builtin_amdgcn_logf(wave_max(fmaxf(__builtin_isfinite(mine) ? mine : 0.0f, 0x1p-100f)));
@@ -418,6 +422,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         for (int e = 0; e < kAhead; ++e) {
             x[0][e] = value(e % kGroups, e / kGroups);
         }
+        top = after[0][0];
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
             if (k + 1 < kParts) {
@@ -433,20 +438,33 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                 const int at = k * kAhead + e;
                 o[at % kGroups] =
                     mfma32(__builtin_bit_cast(prob8, x[k & 1][e]), p[at / kGroups], o[at % kGroups]);
+                if constexpr (!kQuant) {
+                    // the next tile's maximum, held between the products as the exponentials are
+#pragma unroll
+                    for (int c = 8 * at / kGroups; c < 8 * (at + 1) / kGroups; ++c) {
+                        top = fmaxf(top, after[c >> 4][c & 15]);
+                    }
+                    asm volatile("" : "+v"(top));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        kept = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) != 0;
         if constexpr (kQuant) {
             scale_scores(after, kOdd ^ 1);
+            top = max_of(after);
             if (more2) {
                 store_raw(half8(), 0, kOdd);
             }
             if (more) {
                 store_raw(prob8(), 1, kOdd ^ 1);
             }
+        } else {
+            top = max_across_halves(top);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        resolve();
+        resolve(j0 + 192);
         __syncthreads();
     };
 
@@ -454,9 +472,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         f32x16 even[2], odd[2];
         // K of tiles 0 and 1, V of tile 0
         ask(lo);
-        resolve();
+        resolve(lo);
         ask(lo + 64);
-        resolve();
+        resolve(lo + 64);
         note_kept(1);
         if constexpr (kQuant) {
             load_raw(k_next, kbase, a.scale_k, 0);
@@ -479,8 +497,10 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        resolve();
+        resolve(lo + 128);
         __syncthreads();
+        const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[0]);
+        kept = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) != 0;
         even[0] = 0.0f;
         even[1] = 0.0f;
 #pragma unroll
@@ -495,6 +515,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         if constexpr (kQuant) {
             scale_scores(even, 0);
         }
+        top = max_of(even);
         __syncthreads();
         for (int j0 = lo, n = 0;;) {
             step(even, odd, j0, n, std::integral_constant<int, 0>());
@@ -517,7 +538,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             // that do see them.
             for (int j0 = lo; j0 < hi; j0 += 64) {
                 ask(j0);
-                resolve();
+                resolve(j0);
                 load(k_next, vbase, 1, 0);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 bool all_kept = true;
