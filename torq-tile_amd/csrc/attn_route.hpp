@@ -34,16 +34,22 @@ inline int attn_few_row_workgroups(long long units, int per_cu)
 // than so many.
 constexpr int kAttnJoinManyParts = 16;
 
-// The tile kernel is bound by instructions. Its workgroups (two fit a CU) should fill the chip: where the tiles
-// are fewer, their keys are split, in spans of at least 256 (512 tokens of 32 / 8 heads over 8000 keys: 128
-// tiles in four parts, 88 us and 10 of join).
+// The tile kernel is bound by instructions. Workgroups that a CU's registers hold:
 constexpr int kAttnTileRows = 128;
 constexpr int attn_tile_per_cu(size_t cache_element, int head_dim)
 {
     return head_dim > 128 ? 1 : head_dim > 64 || cache_element == 1 ? 2 : 3;
 }
-constexpr long long kAttnTileWorkgroups = 512;
+
+// Where the tiles are fewer than fill the chip, their keys are split, in spans of at least 256, for so many
+// workgroups: 512, or 256 where a CU holds one (512 tokens of 32 / 8 heads over 8000 keys: d 128 in four parts
+// 83 us and 10 of join; d 256 173 us with 256 workgroups, 189 with 512; 1000 tokens from an empty cache 50 and
+// 67). Heads of 64 are not faster with 768 (256 tokens over 16384 keys 60 us, 58 with 512).
 constexpr int kAttnTileLeast = 256;
+constexpr long long attn_tile_workgroups(long long head_dim)
+{
+    return head_dim > 128 ? 256 : 512;
+}
 
 // Tiles of all sequences at most, from the host's bounds.
 inline long long attn_tiles(long long batch, long long q_tokens, long long max_q_len, long long group)
@@ -57,9 +63,10 @@ struct AttnSplit
     int chunk, splits;
 };
 
-inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long span)
+inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long span,
+                                 long long head_dim = 128)
 {
-    const long long want = std::max(1ll, kAttnTileWorkgroups / std::max(1ll, tiles * kv_heads));
+    const long long want = std::max(1ll, attn_tile_workgroups(head_dim) / std::max(1ll, tiles * kv_heads));
     long long chunk = (span + want - 1) / want;
     chunk = std::max<long long>(kAttnTileLeast, (chunk + 63) / 64 * 64);
     AttnSplit s;
