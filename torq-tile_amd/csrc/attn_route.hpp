@@ -43,8 +43,8 @@ constexpr int attn_tile_per_cu(size_t cache_element, int head_dim)
 
 // Where the tiles are fewer than fill the chip, their keys are split, in spans of at least 256, for so many
 // workgroups: 512, or 256 where a CU holds one (512 tokens of 32 / 8 heads over 8000 keys: d 128 in four parts
-// 83 us and 10 of join; d 256 173 us with 256 workgroups, 189 with 512; 1000 tokens from an empty cache 50 and
-// 67). Heads of 64 are not faster with 768 (256 tokens over 16384 keys 60 us, 58 with 512).
+// 83 us and 10 of join; d 256 173 us with 256 workgroups, 189 with 512). Heads of 64 are not faster with 768
+// (256 tokens over 16384 keys 60 us, 58 with 512).
 constexpr int kAttnTileLeast = 256;
 constexpr long long attn_tile_workgroups(long long head_dim)
 {
@@ -63,21 +63,27 @@ struct AttnSplit
     int chunk, splits;
 };
 
+// What the parts and their join cost, in keys that a workgroup has meanwhile; a split that takes less from the
+// longest workgroup is not made. 32 / 8 heads of 128 (256), us with and without a split: 300 tokens from an
+// empty cache 18.3, 13.6 (29.3, 24.6), 512: 22.5, 17.4 (34.5, 31.5), 1000: 39, 27; 512 tokens over 1024
+// keys 33, 26 (46.6, 48.1), 256 over 1024 24.9, 25.8; 64 over 512 17.4, 16.9 (26.8, 30.9).
+constexpr long long attn_split_cost(long long workgroups, long long head_dim)
+{
+    return head_dim > 128 ? 128 + 200 * workgroups / 256 : 256 + 800 * workgroups / 512;
+}
+
 inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long span,
                                  long long head_dim = 128)
 {
-    const long long want = std::max(1ll, attn_tile_workgroups(head_dim) / std::max(1ll, tiles * kv_heads));
-    long long chunk = (span + want - 1) / want;
-    chunk = std::max<long long>(kAttnTileLeast, (chunk + 63) / 64 * 64);
-    AttnSplit s;
-    s.chunk = static_cast<int>(chunk);
+    const long long whole = std::max(1ll, tiles * kv_heads);
+    const long long want = std::max(1ll, attn_tile_workgroups(head_dim) / whole);
+    const long long chunk = std::max<long long>(kAttnTileLeast, ((span + want - 1) / want + 63) / 64 * 64);
     // a tile's span begins at a multiple of 64: up to 63 keys more
-    s.splits = static_cast<int>(std::max(1ll, (span + 63 + chunk - 1) / chunk));
-    if (want == 1) {
-        s.chunk = static_cast<int>((span + 127) / 64 * 64);
-        s.splits = 1;
+    const long long splits = (span + 63 + chunk - 1) / chunk;
+    if (want == 1 || span - chunk < attn_split_cost(whole * splits, head_dim)) {
+        return {static_cast<int>((span + 127) / 64 * 64), 1};
     }
-    return s;
+    return {static_cast<int>(chunk), static_cast<int>(splits)};
 }
 
 }  // namespace tqt
