@@ -94,6 +94,14 @@ def test_splits_cover_every_tile(rules):
             assert n <= splits, (group, nq, kv, window, tile, chunk, splits)
 
 
+def test_split_of_few_tiles_alone(rules):
+    """Many keys of few tiles are split; few keys, or tiles that fill the chip, are not."""
+    assert rules.r_splits(6, 2, 3001) == 12 and rules.r_chunk(6, 2, 3001) == 256
+    assert rules.r_splits(16, 8, 512) == 1 and rules.r_splits(64, 8, 10 ** 6) == 1
+    for span in (1, 63, 64, 65, 300):
+        assert rules.r_splits(1, 1, span) == 1 and rules.r_chunk(1, 1, span) >= span + 63
+
+
 def test_few_row_workgroups(rules):
     assert rules.r_few(1, 2) == 1 and rules.r_few(100, 2) == 100
     assert rules.r_few(10 ** 9, 2) == 512 and rules.r_few(10 ** 9, 1) == 256

@@ -148,6 +148,17 @@ def test_chunks(gpu, name, nq, nk, causal):
     Case(name, [(nq, nk)], 6, 2, 128, causal=causal).run().check()
 
 
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("window", [0, 1700])
+def test_few_tiles_over_many_keys(gpu, name, d, window):
+    """The keys of a tile are split and the parts joined, beside sequences that are not split; the second's
+    last pages are not kept, so that whole parts of it have no key."""
+    c = Case(name, [(40, 3001), (17, 1500), (1, 2000), (70, 30)], 4, 2, d, window=window)
+    c.table[1, 40:] = -1
+    c.run().check()
+
+
 @pytest.mark.parametrize("name", ["f16_f16", "bf16_qsi8dx"])
 @pytest.mark.parametrize("window", [1, 2, 15, 64, 100, 1000])
 @pytest.mark.parametrize("lengths", [[(1, 300), (1, 40)], [(90, 300), (1, 129), (33, 33)]])
