@@ -274,7 +274,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         }
         return max_across_halves(x);
     };
-    float top = 0.0f;   // of a tile's scores, masks left out
+    float top = 0.0f;   // of a tile's scores, masks left out (int8: found in the tile's own step)
     bool kept = false;  // whether all of its keys are on pages that are kept
     // One tile: its scores are in `st`; the next one's go to `after`, their products between the exponentials
     // of this one's (a wave issues in order, so that the two kinds have to alternate). `odd`: the tile's
@@ -309,6 +309,8 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                     st[t][r] = (seen[t] >> r) & 1 ? st[t][r] : -INFINITY;
                 }
             }
+        }
+        if (kQuant || mixed) {
             top = max_of(st);
         }
 
@@ -453,7 +455,6 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         kept = __builtin_amdgcn_readfirstlane(kept4[0] & kept4[1] & kept4[2] & kept4[3]) != 0;
         if constexpr (kQuant) {
             scale_scores(after, kOdd ^ 1);
-            top = max_of(after);
             if (more2) {
                 store_raw(half8(), 0, kOdd);
             }
