@@ -360,12 +360,18 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                 f(c >> 4, c & 15);
             }
         };
+        // int8: the values' scales, read a step ahead of their use
+        constexpr int kScales = 2 * ((32 + kProducts - 1) / kProducts);
+        float scales[kScales];
+        auto read_scale = [&](int t, int r) {
+            scales[(16 * t + r) % kScales] = s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)];
+        };
         auto use = [&](int t, int r) {
             float e = st[t][r];
             sum[t] += e;
             if constexpr (kQuant) {
                 // 0 times a scale that is no number is 0: the row does not see the key
-                e = mul_zero_wins(e, s_scale[1][kOdd][32 * t + 8 * (r >> 2) + 4 * h + (r & 3)], sum[t]);
+                e = mul_zero_wins(e, scales[(16 * t + r) % kScales], sum[t]);
             }
             prob8 &to = p[2 * t + (r >> 3)];
             to[r & 7] = static_cast<P>(e);
@@ -383,6 +389,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             }
             after[k & 1] =
                 mfma32(__builtin_bit_cast(half8, x[k / kKeys & 1][k % kKeys]), q[k >> 1], after[k & 1]);
+            if constexpr (kQuant) {
+                each(k, read_scale);
+            }
             // exponentials of this step's scores, and what the last step's are for
             each(k, [&](int t, int r) {
                 st[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], a.scale, -base_s));
