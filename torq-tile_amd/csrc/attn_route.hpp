@@ -34,7 +34,8 @@ inline int attn_few_row_workgroups(long long units, int per_cu)
 // than so many.
 constexpr int kAttnJoinManyParts = 16;
 
-// The tile kernel is bound by instructions. Workgroups that a CU's registers hold:
+// The tile kernel is bound by instructions. Workgroups that a CU's registers hold (a prompt of 4096, 32 / 8
+// heads of 64, bf16: three 105 us, two 117):
 constexpr int kAttnTileRows = 128;
 constexpr int attn_tile_per_cu(size_t cache_element, int head_dim)
 {

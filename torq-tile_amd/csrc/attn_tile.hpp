@@ -2,14 +2,17 @@
 // (token, query head) pair of one key head, so the heads of a group share the keys that a tile reads.
 //
 // Bound by the matrix cores and the vector instructions together: 4 d flops per row and key, and an exponential
-// with five operations around it. At d 128 a wave's tile takes 1024 cycles of the one and about 1000 of the
-// other; two waves a SIMD overlap them to 2060 (a prompt of 8192, bf16, 32 / 8 heads: 583-613 us, 900-940
-// TFLOP/s, where the library's 8192^3 product has 1155). As in the few-row kernel the first product is S^T = K
-// Q^T, so a lane holds 32 of a tile's 64 scores of one row (its neighbour 32 lanes on holds the others), the
-// statistics are one value a lane, and P^T is the second operand of O^T = V^T P^T without leaving the
-// registers. K and V go from memory to LDS directly (16 bytes a lane, a tile ahead of their use, two stages; K
-// one tile further), keys past the end and pages that are not kept from a block of zeros; int8 rows through
-// registers, where they become 16-bit whole numbers.
+// with five operations around it. A wave's tile takes about 1000 cycles of vector instructions, and 1024 (d 128)
+// or 512 (d 64) of the matrix cores. A wave issues in order, so the exponentials stand between the products with
+// the keys, and the next tile's maximum between those with the values. Two waves a SIMD at d 128 overlap
+// them to 1860 cycles a tile, at the clock that the power limit leaves (a prompt of 8192, bf16, 32 / 8 heads:
+// 559-585 us, 940-980 TFLOP/s, where the library's 8192^3 product has 1155), three at d 64 to 1050.
+//
+// As in the few-row kernel the first product is S^T = K Q^T, so a lane holds 32 of a tile's 64 scores of one row
+// (its neighbour 32 lanes on holds the others), the statistics are one value a lane, and P^T is the second
+// operand of O^T = V^T P^T without leaving the registers. K and V go from memory to LDS directly (16 bytes a
+// lane, a tile ahead of their use, two stages; K one tile further), keys past the end and pages that are not
+// kept from a block of zeros; int8 rows through registers, where they become 16-bit whole numbers.
 //
 // LDS layout of a tile: [key / 16][piece / 4][key % 16][4 pieces of 16 bytes], so that each lane of the 1 KB load
 // that fills one [16][4] block has the same key in all of its loads, and looks up one page per tile. A key's
