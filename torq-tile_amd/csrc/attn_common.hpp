@@ -81,7 +81,7 @@ __device__ __forceinline__ AttnSeq attn_pick(const AttnSeq &x, int at)
 __device__ __forceinline__ void attn_bounds(const AttnArgs &a, const AttnSeq &s, int pos, int &lo, int &hi)
 {
     hi = a.causal ? min(max(pos + 1, 0), s.kv_len) : s.kv_len;
-    lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    lo = attn_first_key(pos, a.window);
 }
 
 // Workgroups that share the keys [first, last) of some rows.

@@ -18,6 +18,14 @@ constexpr long long attn_span(long long max_q_len, long long max_kv_len, long lo
     return window > 0 ? std::min(max_kv_len, window + max_q_len - 1) : max_kv_len;
 }
 
+// The first key that a query at position `pos` sees through a window of `window` keys (0: none). Queries that
+// stand before every key have negative positions, down to 1 - 2^31, and a window may be 2^31 - 1: only the
+// difference of two positions that are not negative is formed.
+constexpr int attn_first_key(int pos, int window)
+{
+    return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
+
 // The few-row kernel reads each key once, so it is bound by the cache's bytes: every CU should have them in
 // flight all the time, whatever the lengths are. Its keys are cut into units of so many for each key head, and
 // the workgroups that fit the chip at once take equal runs of units, across sequences.
