@@ -317,6 +317,44 @@ __device__ __forceinline__ float mul_zero_wins(float x, float y, float &sum)
     return z;
 }
 
+// Int8 values: the probability e = 2^(s - ref) of a key goes to the second product times the value's scale, in f16.
+// `ref` is relative to what a row's largest such term is, not to its largest score: the maximum of
+// s + log2 |scale| over the keys that the row sees, less kValueLogUp. So no key that a row does not see changes
+// its bits, and weights 2^20 below the largest term keep all of theirs: the terms go up to
+// 2^(kValueLogUp - kValueDown), and 2^8 more where ref follows by steps of 8, below f16's 65504. What e (at most
+// 2^(kValueLogUp + 8 - kValueLogFloor) = 2^96, of up to 2^30 keys) and the sums of e need of f32's range is what
+// the three constants leave: scales from 2^-60 up, those below losing bits as f16's subnormals do.
+constexpr float kValueLogUp = 28.0f, kValueLogFloor = -60.0f;
+constexpr float kValueLogLeast = kValueLogFloor - kValueLogUp;
+constexpr float kValueDown = 0x1p-21f, kValueUp = 0x1p21f;
+
+// What is kept of a value's scale: the factor of its key's e, and the summand of its score in the maximum. A row of
+// zeros has a scale that says nothing (the append gives it 1): it counts as the smallest one. A scale that is no
+// number makes the maximum infinite, which makes the rows that see the key NaN; its
+// factor is 0, so that rows that do not see it take nothing from it.
+struct ValueScale
+{
+    float factor, log;
+};
+
+__device__ __forceinline__ ValueScale value_scale(float scale, bool zeros)
+{
+    const float size = __builtin_fabsf(scale);
+    const bool finite = size < INFINITY;  // false for a NaN
+    ValueScale v;
+    v.factor = finite && !zeros ? scale * kValueDown : 0.0f;
+    v.log = fmaxf(__builtin_amdgcn_logf(zeros ? 0.0f : size), kValueLogFloor) - kValueLogUp;
+    v.log = finite ? v.log : INFINITY;
+    return v;
+}
+
+// What the sums so far are multiplied by when `ref` becomes `base`: `half` twice. In one factor it could
+// leave f32's range where the sum does not (scales more than 2^126 apart). ref == base: 1.
+__device__ __forceinline__ float value_half_step(float ref, float base)
+{
+    return __builtin_amdgcn_exp2f(0.5f * (ref - base));
+}
+
 // The largest of a wave's values (none of them NaN): rotations within rows of 16, then across the rows.
 __device__ __forceinline__ float wave_max(float x)
 {

@@ -85,8 +85,24 @@ __device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each
     return j;
 }
 
+// A part's sums times 2^(m - base): over int8 caches the sum of probabilities in two steps, as its reference may
+// be further off than f32's range (value_half_step).
+template <bool kQuant>
+__device__ __forceinline__ float join_part_factor(float m, float base, float &sum)
+{
+    if constexpr (kQuant) {
+        const float half = value_half_step(m, base);
+        sum = sum * half * half;
+        return half * half;
+    } else {
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        sum *= f;
+        return f;
+    }
+}
+
 // Few parts: a wave takes as many heads of a row as fit at 4 elements a lane.
-template <typename T>
+template <typename T, bool kQuant>
 __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few, int each, int rows)
 {
     const int lane = threadIdx.x & 63;
@@ -115,8 +131,9 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few,
 #pragma unroll 4
     for (int k = 0; k < j.parts; ++k) {
         const long long r = join_part(j, k);
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
-        sum += a.part_ml[2 * r + 1] * f;
+        float part = a.part_ml[2 * r + 1];
+        const float f = join_part_factor<kQuant>(a.part_ml[2 * r], base, part);
+        sum += part;
         acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
     }
     const float out[4] = {acc[0], acc[1], acc[2], acc[3]};
@@ -125,7 +142,7 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few,
 
 // Many parts: a workgroup takes one row, head_dim / 4 threads along it and as many such groups as fit over the
 // parts.
-template <typename T>
+template <typename T, bool kQuant>
 __global__ __launch_bounds__(256) void attn_join_many_kernel(AttnArgs a, int few, int each)
 {
     __shared__ f32x4 s_acc[256];
@@ -157,8 +174,9 @@ __global__ __launch_bounds__(256) void attn_join_many_kernel(AttnArgs a, int few
 #pragma unroll 8
         for (int k = group * per; k < k1; ++k) {
             const long long r = join_part(j, k);
-            const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * r] - base);
-            sum += a.part_ml[2 * r + 1] * f;
+            float part = a.part_ml[2 * r + 1];
+            const float f = join_part_factor<kQuant>(a.part_ml[2 * r], base, part);
+            sum += part;
             acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
         }
     }

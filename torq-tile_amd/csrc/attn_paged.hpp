@@ -219,17 +219,18 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         });
         check_launch(where);
     }
+    constexpr bool kQuant = std::is_same<C, int8_t>::value;
     const bool join_tile = plan.run_tile && plan.tile.splits > 1;
     if (plan.few_workgroups > 1 || join_tile) {
         const int each = static_cast<int>(plan.few_tokens), few = plan.run_few ? a.batch * each : 0;
         const int rows = few + (join_tile ? a.q_tokens : 0);
         if (plan.few_many || plan.tile.splits > kAttnJoinManyParts) {
-            hipLaunchKernelGGL((attn_join_many_kernel<T>), dim3(static_cast<unsigned>(rows) * a.q_heads),
+            hipLaunchKernelGGL((attn_join_many_kernel<T, kQuant>), dim3(static_cast<unsigned>(rows) * a.q_heads),
                                dim3(256), 0, stream, a, few, each);
         } else {
             const int per_wave = 256 / a.head_dim;
             const long long items = static_cast<long long>(rows) * ((a.q_heads + per_wave - 1) / per_wave);
-            hipLaunchKernelGGL((attn_join_few_kernel<T>), dim3(static_cast<unsigned>((items + 3) / 4)),
+            hipLaunchKernelGGL((attn_join_few_kernel<T, kQuant>), dim3(static_cast<unsigned>((items + 3) / 4)),
                                dim3(256), 0, stream, a, few, each, rows);
         }
     }

@@ -73,7 +73,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     constexpr int kM = 32 * NW;
     __shared__ __attribute__((aligned(1024))) int8_t lds[4 * kTileBytes];  // K of even and odd tiles, V of both
     __shared__ __attribute__((aligned(16))) int s_kept[4][4];              // [tile % 4][16-key block]
-    __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];  // int8: [K, V][tile % 2]
+    // int8: the keys' scales and the values' factors, [K, V][tile % 2], and the values' logarithms
+    __shared__ __attribute__((aligned(16))) float s_scale[2][2][kQuant ? 64 : 4];
+    __shared__ __attribute__((aligned(16))) float s_log[2][kQuant ? 64 : 4];
 
     // the key heads of a tile side by side: with 8 (or a multiple), a head's tiles are all on one XCD, whose L2
     // its keys then pass once for them
@@ -134,9 +136,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     for (int i = 0; i < DP / 32; ++i) {
         o[i] = 0.0f;
     }
-    // Sums of 2^(s - ref) and 2^(s - ref) v. `ref`, in log2, follows the maximum of s (int8: of s and log2 of the
-    // tile's largest value scale, so that probability times scale stays as small) only when that has grown
-    // by more than 8: until then the probabilities stay below 256 and the sums as they are.
+    // Sums of 2^(s - ref) and 2^(s - ref) v. `ref`, in log2, follows the maximum of s (int8: of s and the logarithm
+    // of the value's scale, value_scale) over the keys that the row sees only when that has grown by more
+    // than 8: until then the probabilities stay below 256 and the sums as they are.
     float ref = -INFINITY, l = 0.0f;
     bool repair = false;  // values that are no numbers were taken out of tiles that not every row sees
 
@@ -223,8 +225,23 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                     *reinterpret_cast<H *>(at + ((2 * (lane & 1) + e) ^ f) * 16) = x[e];
                 }
             }
+            const int key = 16 * block + (lane >> 2);
+            if (which == 0) {
+                if ((lane & 3) == 0) {
+                    s_scale[0][tile & 1][key] = raw_scale[0][i];
+                }
+                continue;
+            }
+            uint32_t any = 0;
+#pragma unroll
+            for (int c = 0; c < kRaw; ++c) {
+                any |= raw[1][i][c][0] | raw[1][i][c][1] | raw[1][i][c][2] | raw[1][i][c][3];
+            }
+            const unsigned long long rows = __ballot(any != 0);
+            const ValueScale v = value_scale(raw_scale[1][i], ((rows >> (lane & ~3)) & 15) == 0);
             if ((lane & 3) == 0) {
-                s_scale[which][tile & 1][16 * block + (lane >> 2)] = raw_scale[which][i];
+                s_scale[1][tile & 1][key] = v.factor;
+                s_log[tile & 1][key] = v.log;
             }
         }
     };
@@ -277,7 +294,33 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         }
         return max_across_halves(x);
     };
-    float top = 0.0f;   // of a tile's scores, masks left out (int8: found in the tile's own step)
+    // int8: the largest of s + logarithm that this lane's row sees in a tile. Where every row sees all of the keys
+    // and their scales lie within 2^4 of the first one's, the largest score and 2^4 times that scale bound it
+    // from above by 8 at most, for which the terms have room below: prompts of 4096 at heads of 64 / 128 / 256
+    // take 177 / 231 / 503 us so and, of one run, 184 / 232 / 541 with every key's own summand.
+    auto value_top = [&](const f32x16 (&st)[2], int parity, bool mixed) {
+        const float mine = s_log[parity][lane];
+        const float most = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(
+                                                         __builtin_bit_cast(int, mine))) + 4.0f;
+        if (!mixed && __all(mine <= most && (mine >= most - 8.0f || mine == kValueLogLeast))) {
+            return __builtin_fmaf(max_of(st), a.scale, most);
+        }
+        float x = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(&s_log[parity][32 * t + 2 * r + 4 * h]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    // a score of -infinity beside an infinite logarithm is a NaN, which the maximum passes over
+                    x = fmaxf(x, __builtin_fmaf(st[t][r + c], a.scale, y[c]));
+                }
+            }
+        }
+        return max_across_halves(x);
+    };
+    float top = 0.0f;   // of a tile's scores, masks left out (int8: value_top of the tile's own step)
     bool kept = false;  // whether all of its keys are on pages that are kept
     // One tile: its scores are in `st`; the next one's go to `after`, their products between the exponentials
     // of this one's (a wave issues in order, so that the two kinds have to alternate). `odd`: the tile's
@@ -313,7 +356,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
                 }
             }
         }
-        if (kQuant || mixed) {
+        if constexpr (kQuant) {
+            top = value_top(st, kOdd, mixed);
+        } else if (mixed) {
             top = max_of(st);
         }
 
@@ -336,16 +381,21 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         }
 
         const i32x4 kept4 = *reinterpret_cast<const i32x4 *>(s_kept[(n + 1) & 3]);
-        float want = top * a.scale;
-        if constexpr (kQuant) {
-            const float mine = s_scale[1][kOdd][lane];
-            want += __builtin_amdgcn_logf(wave_max(fmaxf(__builtin_isfinite(mine) ? mine : 0.0f, 0x1p-100f)));
-        }
+        float want = kQuant ? top : top * a.scale;
         want = want - ref > 8.0f ? want : ref;
         const float base_s = want == -INFINITY ? 0.0f : want;
-        const float alpha = __builtin_amdgcn_exp2f(ref - base_s);
+        float alpha;
+        if constexpr (kQuant) {
+            alpha = value_half_step(ref, base_s);
+            l = l * alpha * alpha;
+            alpha *= alpha;
+            // infinite: a score, or the scale of a value that the row sees
+            l = want == INFINITY ? __builtin_nanf("") : l;
+        } else {
+            alpha = __builtin_amdgcn_exp2f(ref - base_s);
+            l *= alpha;
+        }
         ref = want;
-        l *= alpha;
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
@@ -373,8 +423,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             float e = st[t][r];
             sum[t] += e;
             if constexpr (kQuant) {
-                // 0 times a scale that is no number is 0: the row does not see the key
-                e = mul_zero_wins(e, scales[(16 * t + r) % kScales], sum[t]);
+                e *= scales[(16 * t + r) % kScales];
             }
             prob8 &to = p[2 * t + (r >> 3)];
             to[r & 7] = static_cast<P>(e);
@@ -602,7 +651,11 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     for (int i = 0; i < DP / 32; ++i) {
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const float out[4] = {o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            float out[4] = {o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+#pragma unroll
+            for (int c = 0; kQuant && c < 4; ++c) {
+                out[c] *= kValueUp;
+            }
             attn_put<T, 4>(a, part, s.first + token, head, 32 * i + 2 * r + 4 * h, out, ref, l);
         }
     }
