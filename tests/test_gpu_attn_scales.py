@@ -10,8 +10,10 @@ from test_gpu_attn_paged import Case
 pytestmark = pytest.mark.gpu
 
 INT8 = ["f16_qsi8dx", "bf16_qsi8dx"]
-# new tokens and keys: tiles, with the keys of one workgroup and split over several
+# new tokens and keys: tiles, with the keys of one workgroup and split over several; few rows, in one and in
+# several workgroups
 TILES = [(90, 150), (40, 3001)]
+FEW = [(8, 100), (5, 3001)]
 
 
 def values(c):
@@ -140,4 +142,48 @@ def test_tiles_negative(gpu, name, lengths):
 @pytest.mark.parametrize("lengths", TILES)
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_tiles_not_finite_underflow(gpu, name, lengths, bad):
+    check_not_finite_underflow(name, lengths, 64, bad)
+
+
+@pytest.mark.parametrize("name", INT8)
+@pytest.mark.parametrize("lengths", FEW)
+@pytest.mark.parametrize("d", [64, 96, 256])
+@pytest.mark.parametrize("factor,window", [(2.0 ** 20, 0), (2.0 ** 30, 40), (3e38, 0)])
+def test_few_rows_unseen(gpu, name, lengths, d, factor, window):
+    check_unseen(name, lengths, d, factor, window)
+
+
+@pytest.mark.parametrize("name", INT8)
+@pytest.mark.parametrize("lengths", FEW + [(1, 700)])
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** 20, 2.0 ** 100])
+def test_few_rows_zero_row(gpu, name, lengths, factor):
+    check_zero_row(name, lengths, 64, factor)
+    check_zero_row(name, lengths, 192, factor)
+
+
+@pytest.mark.parametrize("name", INT8)
+@pytest.mark.parametrize("lengths", FEW + [(1, 700)])
+@pytest.mark.parametrize("factor", [2.0 ** 8, 2.0 ** 14])
+def test_few_rows_low_score(gpu, name, lengths, factor):
+    check_low_score(name, lengths, 64, factor)
+    check_low_score(name, lengths, 128, factor)
+
+
+@pytest.mark.parametrize("lengths", FEW + [(1, 700)])
+@pytest.mark.parametrize("low,high", [(-7, 20), (-50, 100), (-30, 110)])
+@pytest.mark.parametrize("period", [75, 1])
+def test_few_rows_far_apart(gpu, lengths, low, high, period):
+    check_far_apart(lengths, 64, low, high, period)
+
+
+@pytest.mark.parametrize("name", INT8)
+@pytest.mark.parametrize("lengths", FEW)
+def test_few_rows_negative(gpu, name, lengths):
+    check_negative(name, lengths, 64)
+
+
+@pytest.mark.parametrize("name", INT8)
+@pytest.mark.parametrize("lengths", FEW)
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_few_rows_not_finite_underflow(gpu, name, lengths, bad):
     check_not_finite_underflow(name, lengths, 64, bad)

@@ -305,33 +305,21 @@ __device__ __forceinline__ float max_across_halves(float x)
     return fmaxf(x, y);
 }
 
-// x * y, and 0 where x or y is 0, whatever the other is. `sum` holds a sum that x has gone into: it keeps the
-// instruction behind that addition, since the compiler does not insert the wait state that a result of exp2
-// needs before an instruction in inline asm.
-__device__ __forceinline__ float mul_zero_wins(float x, float y, float &sum)
-{
-    float z = 0.0f;
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm("v_mul_legacy_f32 %0, %2, %3" : "=v"(z), "+v"(sum) : "v"(x), "v"(y));
-#endif
-    return z;
-}
-
-// Int8 values: the probability e = 2^(s - ref) of a key goes to the second product times the value's scale, in f16.
-// `ref` is relative to what a row's largest such term is, not to its largest score: the maximum of
-// s + log2 |scale| over the keys that the row sees, less kValueLogUp. So no key that a row does not see changes
-// its bits, and weights 2^20 below the largest term keep all of theirs: the terms go up to
-// 2^(kValueLogUp - kValueDown), and 2^8 more where ref follows by steps of 8, below f16's 65504. What e (at most
-// 2^(kValueLogUp + 8 - kValueLogFloor) = 2^96, of up to 2^30 keys) and the sums of e need of f32's range is what
-// the three constants leave: scales from 2^-60 up, those below losing bits as f16's subnormals do.
+// Int8 values: the probability e = 2^(s - ref) of a key goes to the second product times its value's scale, in f16.
+// `ref` follows a row's largest such term, not its largest score: it is the maximum of s + log2 |scale| over the
+// keys that the row sees, less kValueLogUp. So no key that a row does not see changes its bits, and the largest
+// term is 2^7 (2^28 down by 2^21): 2^-1 where the maximum is bounded from above by 2^8 (attn_tile.hpp), 2^15
+// where ref follows it by steps of 2^8, below f16's 65504. Terms 2^13 times smaller than the largest, or more,
+// keep all of f16's bits. What e (2^96 at most, of up to 2^30 keys) and its sums need of f32's range is what the
+// constants leave: scales from 2^-60 up, those below losing bits as f16's subnormals do.
 constexpr float kValueLogUp = 28.0f, kValueLogFloor = -60.0f;
 constexpr float kValueLogLeast = kValueLogFloor - kValueLogUp;
 constexpr float kValueDown = 0x1p-21f, kValueUp = 0x1p21f;
 
 // What is kept of a value's scale: the factor of its key's e, and the summand of its score in the maximum. A row of
 // zeros has a scale that says nothing (the append gives it 1): it counts as the smallest one. A scale that is no
-// number makes the maximum infinite, which makes the rows that see the key NaN; its
-// factor is 0, so that rows that do not see it take nothing from it.
+// number makes the maximum infinite, which makes the rows that see the key NaN; its factor is 0, so that rows
+// that do not see it take nothing from it.
 struct ValueScale
 {
     float factor, log;
@@ -355,23 +343,20 @@ __device__ __forceinline__ float value_half_step(float ref, float base)
     return __builtin_amdgcn_exp2f(0.5f * (ref - base));
 }
 
-// The largest of a wave's values (none of them NaN): rotations within rows of 16, then across the rows.
-__device__ __forceinline__ float wave_max(float x)
+// A part's sums times 2^(m - base): over int8 caches the sum of probabilities in two steps, as its reference may
+// be further off than f32's range (value_half_step).
+template <bool kQuant>
+__device__ __forceinline__ float part_factor(float m, float base, float &sum)
 {
-    auto rotated = [](float y, auto by) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y),
-                                                                     0x120 + decltype(by)::value, 0xf, 0xf,
-                                                                     false));
-    };
-    x = fmaxf(x, rotated(x, std::integral_constant<int, 1>()));
-    x = fmaxf(x, rotated(x, std::integral_constant<int, 2>()));
-    x = fmaxf(x, rotated(x, std::integral_constant<int, 4>()));
-    x = fmaxf(x, rotated(x, std::integral_constant<int, 8>()));
-    const int y = __builtin_bit_cast(int, x);
-    return fmaxf(fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 0)),
-                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 16))),
-                 fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 32)),
-                       __builtin_bit_cast(float, __builtin_amdgcn_readlane(y, 48))));
+    if constexpr (kQuant) {
+        const float half = value_half_step(m, base);
+        sum = sum * half * half;
+        return half * half;
+    } else {
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        sum *= f;
+        return f;
+    }
 }
 
 // 16 int8 as 16-bit floats, exactly: [0] the first 8, [1] the others.

@@ -32,7 +32,7 @@ struct FewRowTile
     static constexpr bool kQuant = std::is_same<C, int8_t>::value;
     static constexpr int kPieces = DP * static_cast<int>(sizeof(C)) / 64;  // 16-byte pieces of a row per lane
     static constexpr int kStride = DP * 2 + 16;                           // bytes of a value row in LDS
-    static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 256 : 0);
+    static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 384 : 0);
 };
 
 template <typename T, typename C, int DP, bool kFull>
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         for (int i = 0; i < DP / 16; ++i) {
             o[i] = 0.0f;
         }
-        // sums of 2^(s - ref) and 2^(s - ref) v; `ref` (log2) is the maximum of s so far, for int8 of s and log2 of
-        // the tile's largest value scale, so that probability times scale stays below 1
+        // sums of 2^(s - ref) and 2^(s - ref) v; `ref` (log2) is the maximum so far of s, for int8 of s and the
+        // logarithm of the value's scale (value_scale), over the keys that the row sees
         float ref = -INFINITY, l = 0.0f;
 
         // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
@@ -208,14 +208,26 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
                     }
                 }
             }
+            // int8: the keys' scales, the values' factors and logarithms
             float *scales = reinterpret_cast<float *>(mine + 32 * kStride);
-            float scale_log = 0.0f;
             if constexpr (kQuant) {
+                uint32_t any[2] = {0, 0};
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < kPieces; ++i) {
+                        any[t] |= vx[t][i][0] | vx[t][i][1] | vx[t][i][2] | vx[t][i][3];
+                    }
+                }
+                // this lane's scale is that of key lane % 32, whose row lanes col, col + 16, ... have
+                const unsigned long long rows0 = __ballot(any[0] != 0), rows1 = __ballot(any[1] != 0);
+                const unsigned long long rows = (lane & 16) != 0 ? rows1 : rows0;
+                const ValueScale v = value_scale(sv, ((rows >> col) & 0x0001000100010001ull) == 0);
                 if (lane < 32) {
                     scales[lane] = sk;
-                    scales[32 + lane] = sv;
+                    scales[32 + lane] = v.factor;
+                    scales[64 + lane] = v.log;
                 }
-                scale_log = __builtin_amdgcn_logf(wave_max(fmaxf(__builtin_isfinite(sv) ? sv : 0.0f, 0x1p-100f)));
             }
             const unsigned long long kept0 = __ballot(kept[0]), kept1 = __ballot(kept[1]);
             const uint32_t keptmask = static_cast<uint32_t>(kept0 & 0xffff) |
@@ -253,9 +265,10 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                f32x4 ks = 1.0f;
+                f32x4 ks = 1.0f, log = 0.0f;
                 if constexpr (kQuant) {
                     ks = *reinterpret_cast<f32x4 *>(scales + 16 * t + 4 * g);
+                    log = *reinterpret_cast<f32x4 *>(scales + 64 + 16 * t + 4 * g);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -267,17 +280,27 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
                         x *= ks[r];
                     }
                     st[t][r] = see ? x * a.scale : -INFINITY;
-                    // a NaN stays one: exp2 of it, below
-                    top = fmaxf(top, st[t][r]);
+                    // a NaN stays one: exp2 of it, below (that of a score of -infinity beside an infinite
+                    // logarithm is passed over)
+                    top = fmaxf(top, kQuant ? st[t][r] + log[r] : st[t][r]);
                 }
             }
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(ref, top + scale_log);
+            top = fmaxf(ref, top);
             const float base = top == -INFINITY ? 0.0f : top;
-            const float alpha = __builtin_amdgcn_exp2f(ref - base);
+            float alpha;
+            if constexpr (kQuant) {
+                alpha = value_half_step(ref, base);
+                l = l * alpha * alpha;
+                alpha *= alpha;
+                // infinite: a score, or the scale of a value that the row sees
+                l = top == INFINITY ? __builtin_nanf("") : l;
+            } else {
+                alpha = __builtin_amdgcn_exp2f(ref - base);
+                l *= alpha;
+            }
             ref = top;
-            l *= alpha;
             prob8 p;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -290,8 +313,7 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
                     float e = __builtin_amdgcn_exp2f(st[t][r] - base);
                     l += e;
                     if constexpr (kQuant) {
-                        // 0 times a scale that is no number is 0: the row does not see the key
-                        e = mul_zero_wins(e, vsc[r], l);
+                        e *= vsc[r];
                     }
                     p[4 * t + r] = static_cast<P>(e);
                 }
@@ -348,7 +370,7 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         float *mo = reinterpret_cast<float *>(mine);  // [16][DP]
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-            *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = o[i];
+            *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = kQuant ? o[i] * kValueUp : o[i];
         }
         if (lane < 16) {
             s_m[wave][lane] = ref;
@@ -367,8 +389,9 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
             float sum = 0.0f, acc[kOut] = {};
 #pragma unroll
             for (int w = 0; w < kAttnFewRowWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(s_m[w][r] - base);
-                sum += s_l[w][r] * f;
+                float part = s_l[w][r];
+                const float f = part_factor<kQuant>(s_m[w][r], base, part);
+                sum += part;
                 const float *from = reinterpret_cast<const float *>(lds + w * Tile::kWaveBytes) + r * DP + d0;
 #pragma unroll
                 for (int e = 0; e < kOut; ++e) {

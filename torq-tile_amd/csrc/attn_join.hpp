@@ -85,22 +85,6 @@ __device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each
     return j;
 }
 
-// A part's sums times 2^(m - base): over int8 caches the sum of probabilities in two steps, as its reference may
-// be further off than f32's range (value_half_step).
-template <bool kQuant>
-__device__ __forceinline__ float join_part_factor(float m, float base, float &sum)
-{
-    if constexpr (kQuant) {
-        const float half = value_half_step(m, base);
-        sum = sum * half * half;
-        return half * half;
-    } else {
-        const float f = __builtin_amdgcn_exp2f(m - base);
-        sum *= f;
-        return f;
-    }
-}
-
 // Few parts: a wave takes as many heads of a row as fit at 4 elements a lane.
 template <typename T, bool kQuant>
 __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few, int each, int rows)
@@ -132,7 +116,7 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few,
     for (int k = 0; k < j.parts; ++k) {
         const long long r = join_part(j, k);
         float part = a.part_ml[2 * r + 1];
-        const float f = join_part_factor<kQuant>(a.part_ml[2 * r], base, part);
+        const float f = part_factor<kQuant>(a.part_ml[2 * r], base, part);
         sum += part;
         acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
     }
@@ -175,7 +159,7 @@ __global__ __launch_bounds__(256) void attn_join_many_kernel(AttnArgs a, int few
         for (int k = group * per; k < k1; ++k) {
             const long long r = join_part(j, k);
             float part = a.part_ml[2 * r + 1];
-            const float f = join_part_factor<kQuant>(a.part_ml[2 * r], base, part);
+            const float f = part_factor<kQuant>(a.part_ml[2 * r], base, part);
             sum += part;
             acc += *reinterpret_cast<const f32x4 *>(a.part_o + r * a.head_dim + 4 * at) * f;
         }
