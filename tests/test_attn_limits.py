@@ -18,9 +18,17 @@ def rules(tmp_path_factory):
     d = tmp_path_factory.mktemp("limits")
     (d / "r.cpp").write_text('''
 #include "attn_route.hpp"
+#include "rope_route.hpp"
 using namespace tqt;
 extern "C" {
 int r_first_key(int pos, int window) { return attn_first_key(pos, window); }
+void r_rope(long long heads, long long d, int grid16, int pow2, long long *out)
+{
+    const RopeLaunch r = rope_launch(heads, d, grid16, pow2);
+    out[0] = r.rows;
+    out[1] = r.per_head;
+    out[2] = r.tokens;
+}
 }
 ''')
     subprocess.run([CLANG, "-O2", "-std=c++17", "-fwrapv", "-fPIC", "-shared", "-Wall", "-I" +
@@ -28,6 +36,7 @@ int r_first_key(int pos, int window) { return attn_first_key(pos, window); }
                    check=True)
     lib = ctypes.CDLL(str(d / "r.so"))
     lib.r_first_key.argtypes = [ctypes.c_int] * 2
+    lib.r_rope.argtypes = [ctypes.c_longlong] * 2 + [ctypes.c_int] * 2 + [ctypes.c_void_p]
     return lib
 
 
@@ -40,3 +49,29 @@ def test_first_key_of_a_window(rules, window):
     for pos in POSITIONS:
         want = max(pos - window + 1, 0) if window else 0
         assert rules.r_first_key(pos, window) == want, (pos, window)
+
+
+# rows of a token up to those of the widest calls: rope's 2^20 - 1 heads, the append's queries, keys and values
+@pytest.mark.parametrize("heads", [1, 33, 48, 1 << 16, (1 << 20) - 1, (1 << 20) - 1 + 2 * ((1 << 16) - 1)])
+@pytest.mark.parametrize("d", [1, 16, 20, 80, 128, 256, 1 << 15, (1 << 20) - 16])
+def test_rope_launches_fit(rules, heads, d):
+    """Every launch's work-items stay below 2^32 and its indexes below 2^31, and it has a token at least."""
+    for grid16 in (0, 1):
+        for pow2 in (0, 1):
+            if grid16 and d % 16 or pow2 and d > 256:
+                continue
+            out = (ctypes.c_longlong * 3)()
+            rules.r_rope(heads, d, grid16, pow2, out)
+            rows, per_head, tokens = out
+            assert tokens >= 1 and (grid16 or not rows)
+            threads = tokens * heads * per_head * (1 if rows else 64)
+            assert -(-threads // 256) * 256 < 2 ** 32 and tokens * heads * per_head < 2 ** 31
+            if rows:
+                assert per_head * 16 >= d and (not pow2 or per_head & (per_head - 1) == 0)
+
+
+def test_ordinary_rope_calls_take_one_launch(rules):
+    for heads, d, grid16 in ((32, 128, 1), (48, 128, 1), (32, 72, 0)):
+        out = (ctypes.c_longlong * 3)()
+        rules.r_rope(heads, d, grid16, 0, out)
+        assert out[0] == grid16 and out[2] >= 8192

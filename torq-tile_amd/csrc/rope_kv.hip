@@ -13,6 +13,7 @@
 // tokens of 96 int8 heads and 26.6 instead of 24.2 for 4096 of 48 from f32: fewer waves have loads in flight).
 #include "fast_div.hpp"
 #include "paged_kv.hpp"
+#include "rope_route.hpp"
 #include "tqt_hip_common.hpp"
 #include "tqt_kv_append_rope_gfx950.h"
 
@@ -411,28 +412,19 @@ void set_map(RopeArgs &a, const tqt_rope_map &m, const int32_t *positions)
     a.sign = m.inverse != 0 ? -1.0f : 1.0f;
 }
 
-// Launches the rows of all tokens, in pieces whose thread indexes stay below 2^30.
+// Launches the rows of all tokens. grid16: they suit rope_rows_kernel.
 template <typename SRC, typename DST, typename CACHE>
-void launch_rows(RopeArgs a, bool vec, hipStream_t stream, const char *where)
+void launch_rows(RopeArgs a, bool grid16, hipStream_t stream, const char *where)
 {
-    int per_head = a.head_dim / 16;
-    if (std::is_same<CACHE, int8_t>::value) {
-        int p = 1;
-        while (p < per_head) {
-            p *= 2;
-        }
-        per_head = p;  // a head's threads exchange their maxima in a butterfly
-    }
-    a.units = make_fast_div(vec ? per_head : 1);
+    const RopeLaunch r = rope_launch(a.rows, a.head_dim, grid16, std::is_same<CACHE, int8_t>::value);
+    a.units = make_fast_div(static_cast<uint32_t>(r.per_head));
     a.heads = make_fast_div(a.rows);
-    const long long per_token = static_cast<long long>(a.rows) * (vec ? per_head : 1);
-    const long long most = std::max(1ll, (1ll << 28) / per_token);
-    for (long long t0 = 0; t0 < a.tokens; t0 += most) {
-        const long long n = std::min(most, a.tokens - t0);
-        const uint32_t items = static_cast<uint32_t>(n * per_token);
-        const int per_block = vec ? kRopeThreads : kRopeThreads / 64;
+    for (long long t0 = 0; t0 < a.tokens; t0 += r.tokens) {
+        const long long n = std::min(r.tokens, a.tokens - t0);
+        const uint32_t items = static_cast<uint32_t>(n * a.rows * r.per_head);
+        const int per_block = r.rows ? kRopeThreads : kRopeThreads / 64;
         const dim3 grid((items + per_block - 1) / per_block);
-        if (vec) {
+        if (r.rows) {
             hipLaunchKernelGGL((rope_rows_kernel<SRC, DST, CACHE>), grid, dim3(kRopeThreads), 0, stream, a,
                                static_cast<int>(t0), items);
         } else {
