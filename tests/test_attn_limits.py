@@ -7,6 +7,9 @@ import subprocess
 
 import pytest
 
+import paged_ref as R
+import test_paged_host as H
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CLANG = "/opt/rocm/llvm/bin/clang++"
 
@@ -75,3 +78,22 @@ def test_ordinary_rope_calls_take_one_launch(rules):
         out = (ctypes.c_longlong * 3)()
         rules.r_rope(heads, d, grid16, 0, out)
         assert out[0] == grid16 and out[2] >= 8192
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_buffers_of_many_rows_are_not_split(d):
+    """q_tokens of a large buffer, of which a call's sequences use few rows: no parts, whose join would have a
+    workgroup for every row of the buffer."""
+    _, lib = R.binding()
+
+    def need(tokens):
+        p = H.changed(H.attn_params, batch=1, q_tokens=tokens, q_heads=16, kv__kv_heads=2, max_q_len=64,
+                      max_kv_len=100000, ld_table=6250, kv__num_pages=6250, kv__head_dim=d)
+        size = lib.op("attn_paged", "get_workspace_size")(ctypes.byref(p))
+        assert H.refusal("attn_paged_f16_f16", H.changed(lambda: p, workspace_size=size)) is None
+        return size
+
+    splits = need(64) // (64 * 16 * (d + 2) * 4)
+    assert splits > 16
+    assert need(2 ** 19 - 1) == splits * (2 ** 19 - 1) * 16 * (d + 2) * 4
+    assert need(2 ** 19) == need(2 ** 20) == 0

@@ -1,8 +1,10 @@
 """Attention over a paged cache at the ends of its arguments' ranges, on the GPU against the plain form in 64
 bits."""
 
+import numpy as np
 import pytest
 
+import paged_ref as R
 from test_gpu_attn_paged import NAMES, Case
 
 pytestmark = pytest.mark.gpu
@@ -14,3 +16,25 @@ def test_widest_windows(gpu, name, window):
     """Windows past every length, with queries that stand before every key beside others, for both kernels."""
     Case(name, [(4, 1), (3, 200), (7, 2)], 4, 2, 64, window=window).run().check()
     Case(name, [(9, 4), (40, 7), (70, 1), (33, 300)], 4, 2, 64, window=window).run().check()
+
+
+def test_few_rows_of_a_large_buffer(gpu):
+    """One sequence of 50 tokens over 20000 keys in a buffer of 2^20 rows: the others are not touched."""
+    import torch
+
+    mod, _ = R.binding()
+    heads, kv_heads, d, page, n, nk = 16, 2, 16, 64, 50, 20000
+    rng = np.random.default_rng(5)
+    q = torch.zeros((2 ** 20, heads, d), dtype=torch.float16, device="cuda:0")
+    q[:n] = R.dev(rng.standard_normal((n, heads, d)), "f16")
+    out, lse = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda:0")
+    k, v = (R.dev(rng.standard_normal((-(-nk // page), page, kv_heads, d)), "f16") for _ in range(2))
+    table = np.arange(k.shape[0], dtype=np.int32)[None]
+    R.run_attention("f16_f16", q, R.paged(mod, k, v), R.dev(np.array([0, n], np.int32)),
+                    R.dev(np.array([nk], np.int32)), R.dev(table), out, lse, 0.25)
+    assert (out[n:] == 9.0).all() and (lse[n:] == 9.0).all()
+    kk, vv = (R.host(t).reshape(-1, kv_heads, d)[:nk] for t in (k, v))
+    want = R.attention(R.host(q[:n]), kk, vv, R.visible(n, nk, True, 0), 0.25)
+    tol, tol_lse = R.attention_bound("f16", d, *want)
+    assert (np.abs(R.host(out[:n]) - want[0]) <= tol).all()
+    assert (np.abs(R.host(lse[:n]) - want[1]) <= tol_lse).all()

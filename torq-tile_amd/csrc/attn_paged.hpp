@@ -124,10 +124,11 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
         plan.few_many = plan.few_workgroups > heads * kAttnJoinManyParts;
     }
     plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
-    plan.tile = attn_tile_split(plan.tiles, p->kv.kv_heads,
+    plan.tile = attn_call_split(plan.tiles, p->kv.kv_heads,
                                 attn_span(std::min<long long>(p->max_q_len, kAttnTileRows / group + 2),
                                           p->max_kv_len, window),
-                                static_cast<long long>(p->kv.head_dim));
+                                static_cast<long long>(p->kv.head_dim),
+                                static_cast<long long>(p->q_tokens * p->q_heads));
     plan.parts = 2ll * plan.few_workgroups * kAttnFewRows;
     if (plan.run_tile && plan.tile.splits > 1) {
         plan.parts += plan.tile.splits * static_cast<long long>(p->q_tokens) * p->q_heads;

@@ -95,4 +95,16 @@ inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long 
     return {static_cast<int>(chunk), static_cast<int>(splits)};
 }
 
+// The parts and their join are laid out for every row of Q, `rows` (token, query head) pairs, whether a sequence has
+// it or not: q_tokens may be a buffer's. From so many rows on keys are not split, so that the join's grid stays
+// below 2^32 work-items (256 a row). A call of so few tiles that they are split has 2^15 rows of its own at most.
+constexpr long long kAttnJoinRows = 1 << 23;
+
+inline AttnSplit attn_call_split(long long tiles, long long kv_heads, long long span, long long head_dim,
+                                 long long rows)
+{
+    const AttnSplit s = attn_tile_split(tiles, kv_heads, span, head_dim);
+    return rows < kAttnJoinRows ? s : AttnSplit{static_cast<int>((span + 127) / 64 * 64), 1};
+}
+
 }  // namespace tqt
