@@ -17,7 +17,7 @@
  *                           scale_k, scale_v [num_pages][kv_heads][page_size]: amax = max |x| of the
  *                           (rotated, f32) row, scale = amax * f32(1 / 127) (1 for a row of zeros),
  *                           q = clamp(nearbyint(x / scale), -127, 127). A row with a NaN or an infinity
- *                           gets a scale that is one, so it reads back as NaN. Q_out has Q's type.
+ *                           gets a NaN for its scale, so it reads back as NaN. Q_out has Q's type.
  *
  * head_dim is a multiple of 16 up to 256; k, v and their strides keep rows on the 16-byte grid; K, V
  * and Q take any strides and alignment (rows on the 16-byte grid with rotary_dim a multiple of 16 are

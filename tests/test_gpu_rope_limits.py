@@ -1,10 +1,12 @@
-"""Rotary positions and their table at the ends of their arguments' ranges, on the GPU."""
+"""Rotary positions, their table and the append at the ends of their arguments' ranges, on the GPU."""
 
 import ctypes
 
+import numpy as np
 import pytest
 
 import paged_ref as R
+from test_gpu_rope_append import run_append
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +34,19 @@ def test_rows_past_one_grid(gpu):
     a, b, c, s = x[..., 0].float(), x[..., 1].float(), t[:, :1], t[:, 1:]
     assert torch.equal(y[..., 0], (a * c - b * s).half())
     assert torch.equal(y[..., 1], (b * c + a * s).half())
+
+
+@pytest.mark.parametrize("name", ["qsi8dx_f16", "qsi8dx_bf16"])
+@pytest.mark.parametrize("rot", [0, 64])
+@pytest.mark.parametrize("pads", [(0, 0, 0), (1, 0, 0)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_append_int8_not_finite_reads_back_as_nan(gpu, name, rot, bad, pads):
+    """Every element of a key's or value's row with a NaN or an infinity, that one's own among them."""
+    r = np.random.default_rng(1).standard_normal((4, 3, 64))
+    r[1, 1, 17] = r[2, 2, 40] = bad  # a key, a value
+    g = run_append(name, 4, 1, 1, 64, rot, rows=r, pads=pads)
+    for cache, scale, token in (("k", "sk", 1), ("v", "sv", 2)):
+        back = g[cache].double() * g[scale].double().transpose(1, 2)[..., None]
+        back = back.reshape(-1, 64)[R.dev(g["slots"])].cpu().numpy()
+        assert np.isnan(back[token]).all()
+        assert np.isfinite(np.delete(back, token, 0)).all()

@@ -76,7 +76,8 @@ __device__ __forceinline__ float nan_max(float m, float a)
     return a > m || a != a ? a : m;
 }
 
-// The scale of a row of an int8 cache; `zero`: every q is 0 (a scale that is 0 in f32 too).
+// The scale of a row of an int8 cache, NaN for a row with a NaN or an infinity; `zero`: every q is 0 (a scale that
+// is 0 in f32 too).
 struct QuantRow
 {
     float scale, inverse;
@@ -86,7 +87,7 @@ struct QuantRow
 __device__ __forceinline__ QuantRow quant_row(float amax)
 {
     QuantRow r;
-    r.scale = amax * (1.0f / 127.0f);
+    r.scale = amax < INFINITY ? amax * (1.0f / 127.0f) : __builtin_nanf("");
     r.zero = r.scale == 0.0f;
     if (r.zero) {
         r.scale = 1.0f;
