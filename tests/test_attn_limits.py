@@ -4,6 +4,7 @@ evaluated on the CPU."""
 import ctypes
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -97,3 +98,30 @@ def test_buffers_of_many_rows_are_not_split(d):
     assert splits > 16
     assert need(2 ** 19 - 1) == splits * (2 ** 19 - 1) * 16 * (d + 2) * 4
     assert need(2 ** 19) == need(2 ** 20) == 0
+
+
+def table_params():
+    mod, _ = R.binding()
+    return mod.RopeTableParams(table=4096, max_pos=10, rotary_dim=8, base=1e4)
+
+
+@pytest.mark.parametrize("max_pos,rot", [
+    (2 ** 31 - 1, 2), (2 ** 31 - 1, 4), (2 ** 31 - 1, 6), (2 ** 26 - 4, 128), (2 ** 26 - 3, 128), (2 ** 26, 128),
+    (2 ** 13, 2 ** 20 - 2), (2 ** 13 + 1, 2 ** 20 - 2)])
+def test_tables_past_one_launch_are_refused(max_pos, rot):
+    """Whether a run would take it is what get_error says: its workgroups of 256 threads, one per pair, are of fewer
+    than 2^32 threads."""
+    said = H.refusal("rope_table_f32", H.changed(table_params, max_pos=max_pos, rotary_dim=rot))
+    assert (said is None) == (-(-max_pos * (rot // 2) // 256) * 256 < 2 ** 32)
+
+
+def test_a_refused_table_aborts_in_both_forms():
+    """Also where there is nothing to write."""
+    for action in ("run", "run_async"):
+        code = ("import sys, ctypes; sys.path.insert(0, %r); import paged_ref as R\n"
+                "mod, lib = R.binding(); p = mod.RopeTableParams(table=4096, max_pos=0, rotary_dim=3, base=1e4)\n"
+                "lib.op('rope_table_f32', %r)(ctypes.byref(p)%s)\nprint('returned')"
+                % (os.path.join(ROOT, "tests"), action, ", None" if action == "run_async" else ""))
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+        assert r.returncode == -6 and "returned" not in r.stdout
+        assert H.refusal("rope_table_f32", H.changed(table_params, rotary_dim=3)).decode() in r.stderr

@@ -540,6 +540,13 @@ bool run_append(const tqt_kv_append_rope_params *p, hipStream_t stream, const ch
     return true;
 }
 
+// One thread per pair of a position.
+long long table_blocks(const tqt_rope_table_params *p)
+{
+    const long long pairs = static_cast<long long>(p->max_pos) * static_cast<long long>(p->rotary_dim / 2);
+    return (pairs + kRopeThreads - 1) / kRopeThreads;
+}
+
 const char *table_error(const tqt_rope_table_params *p)
 {
     if (p == nullptr) {
@@ -567,7 +574,32 @@ const char *table_error(const tqt_rope_table_params *p)
         (!(p->original_max_pos > 0.0) || !(p->low_turns > 0.0) || !(p->high_turns > p->low_turns))) {
         return "original_max_pos, low_turns and high_turns: 0 < low_turns < high_turns are needed";
     }
+    if (table_blocks(p) * kRopeThreads >= 0x100000000ll) {
+        return "max_pos * rotary_dim / 2 is too large for one launch";
+    }
     return nullptr;
+}
+
+bool run_table(const tqt_rope_table_params *p, hipStream_t stream)
+{
+    if (p == nullptr) {
+        return false;
+    }
+    const char *error = table_error(p);
+    TQT_REQUIRE(error == nullptr, error);
+    if (p->max_pos == 0 || p->rotary_dim == 0) {
+        return false;
+    }
+    double amplitude = p->amplitude;
+    if (amplitude == 0.0) {
+        amplitude = p->scaling == TQT_ROPE_RAMP ? 0.1 * std::log(p->factor) + 1.0 : 1.0;
+    }
+    const int half = static_cast<int>(p->rotary_dim / 2);
+    hipLaunchKernelGGL(rope_table_kernel, dim3(static_cast<unsigned>(table_blocks(p))), dim3(kRopeThreads), 0,
+                       stream, p->table, static_cast<long long>(p->max_pos) * half, half, p->base, p->factor,
+                       p->scaling, p->original_max_pos, p->low_turns, p->high_turns, amplitude);
+    check_launch("tqt_run_rope_table_f32_gfx950");
+    return true;
 }
 
 }  // namespace
@@ -630,36 +662,14 @@ const char *tqt_get_error_rope_table_f32_gfx950(const struct tqt_rope_table_para
 
 void tqt_run_rope_table_f32_gfx950_async(const struct tqt_rope_table_params *params, void *stream)
 {
-    if (params == nullptr) {
-        return;
-    }
-    const char *error = table_error(params);
-    TQT_REQUIRE(error == nullptr, error);
-    if (params->max_pos == 0 || params->rotary_dim == 0) {
-        return;
-    }
-    double amplitude = params->amplitude;
-    if (amplitude == 0.0) {
-        amplitude = params->scaling == TQT_ROPE_RAMP ? 0.1 * std::log(params->factor) + 1.0 : 1.0;
-    }
-    const int half = static_cast<int>(params->rotary_dim / 2);
-    const long long pairs = static_cast<long long>(params->max_pos) * half;
-    const long long blocks = (pairs + kRopeThreads - 1) / kRopeThreads;
-    TQT_REQUIRE(blocks * kRopeThreads < 0x100000000ll, "table too large for one launch");
-    hipLaunchKernelGGL(rope_table_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0,
-                       as_stream(stream), params->table, pairs, half, params->base, params->factor,
-                       params->scaling, params->original_max_pos, params->low_turns, params->high_turns,
-                       amplitude);
-    check_launch("tqt_run_rope_table_f32_gfx950");
+    run_table(params, as_stream(stream));
 }
 
 void tqt_run_rope_table_f32_gfx950(const struct tqt_rope_table_params *params)
 {
-    if (params == nullptr || params->max_pos == 0 || params->rotary_dim == 0) {
-        return;
+    if (run_table(params, nullptr)) {
+        finish_sync(nullptr, "tqt_run_rope_table_f32_gfx950");
     }
-    tqt_run_rope_table_f32_gfx950_async(params, nullptr);
-    finish_sync(nullptr, "tqt_run_rope_table_f32_gfx950");
 }
 
 }  // extern "C"
