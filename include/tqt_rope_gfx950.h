@@ -63,7 +63,8 @@ struct tqt_rope_params
  *   TQT_ROPE_RAMP    f_i where the pair makes more than high_turns turns over original_max_pos tokens,
  *                    f_i / factor where fewer than low_turns, and in between a blend linear in i (from
  *                    the floor of the one index to the ceiling of the other); the table's values are
- *                    times 0.1 ln(factor) + 1 unless amplitude says otherwise
+ *                    times 0.1 ln(factor) + 1 (times 1 for a factor up to 1) unless amplitude says
+ *                    otherwise
  *   TQT_ROPE_TURNS   the same two ends, with a blend linear in the number of turns
  * amplitude multiplies cosines and sines; 0 stands for the default (1, or TQT_ROPE_RAMP's). */
 #define TQT_ROPE_PLAIN 0

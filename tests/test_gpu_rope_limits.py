@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import paged_ref as R
-from test_gpu_rope_append import run_append
+from test_gpu_rope_append import run_append, table_freq
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,18 @@ def test_append_int8_not_finite_reads_back_as_nan(gpu, name, rot, bad, pads):
         back = back.reshape(-1, 64)[R.dev(g["slots"])].cpu().numpy()
         assert np.isnan(back[token]).all()
         assert np.isfinite(np.delete(back, token, 0)).all()
+
+
+@pytest.mark.parametrize("factor,amplitude", [(0.5, 1.0), (1e-5, 1.0), (1.0, 1.0), (4.0, 0.1 * np.log(4.0) + 1)])
+def test_ramp_amplitude(gpu, factor, amplitude):
+    """The ramp's amplitude grows with factors above 1 and is 1 for the others."""
+    import torch
+
+    mod, lib = R.binding()
+    t = torch.zeros((500, 32), device="cuda:0")
+    p = mod.RopeTableParams(table=R.ptr(t), max_pos=500, rotary_dim=32, scaling=mod.ROPE_RAMP, base=10000.0,
+                            factor=factor, original_max_pos=4096.0, low_turns=1, high_turns=32)
+    lib.op("rope_table_f32", "run")(ctypes.byref(p))
+    want = amplitude * R.rope_table(500, 32, freq=table_freq(32, 3, 10000.0, factor, 4096.0, 1, 32))
+    # one rounding to f32; the angles' own error in f64 is below 500 / 1e-5 * 2^-50
+    assert np.abs(R.host(t) - want).max() <= amplitude * 2.0 ** -24 + 5e7 * 2.0 ** -50

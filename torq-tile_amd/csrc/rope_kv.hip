@@ -592,7 +592,7 @@ bool run_table(const tqt_rope_table_params *p, hipStream_t stream)
     }
     double amplitude = p->amplitude;
     if (amplitude == 0.0) {
-        amplitude = p->scaling == TQT_ROPE_RAMP ? 0.1 * std::log(p->factor) + 1.0 : 1.0;
+        amplitude = p->scaling == TQT_ROPE_RAMP && p->factor > 1.0 ? 0.1 * std::log(p->factor) + 1.0 : 1.0;
     }
     const int half = static_cast<int>(p->rotary_dim / 2);
     hipLaunchKernelGGL(rope_table_kernel, dim3(static_cast<unsigned>(table_blocks(p))), dim3(kRopeThreads), 0,
