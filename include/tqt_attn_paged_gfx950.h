@@ -22,7 +22,7 @@
  * bf16_qsi8dx (int8 with a scale for each token and head).
  *
  * Preconditions: q_heads a multiple of kv_heads; head_dim a multiple of 16 up to 256; rows of Q, D, k and
- * v on the 16-byte grid; max_kv_len <= ld_table * page_size and below 2^30. max_q_len and max_kv_len bound
+ * v on the 16-byte grid; scale times log2(e) finite; max_kv_len <= ld_table * page_size and below 2^30. max_q_len and max_kv_len bound
  * q_len and kv_len of every sequence: the launch and its workspace are sized by them, so that lengths may
  * change on the device between replays of a captured call. (A kv_len past max_kv_len is taken as max_kv_len,
  * queries past max_q_len of a sequence are left out. Bounds near the lengths make a call faster.) q_start does

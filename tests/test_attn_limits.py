@@ -125,3 +125,10 @@ def test_a_refused_table_aborts_in_both_forms():
         r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
         assert r.returncode == -6 and "returned" not in r.stdout
         assert H.refusal("rope_table_f32", H.changed(table_params, rotary_dim=3)).decode() in r.stderr
+
+
+@pytest.mark.parametrize("scale,taken", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False),
+                                         (0.0, True), (1e-45, True)])
+def test_scales_whose_log2_form_overflows_are_refused(scale, taken):
+    for kind in H.ATTNS:
+        assert (H.refusal("attn_paged_" + kind, H.changed(H.attn_params, scale=scale)) is None) == taken

@@ -20,6 +20,12 @@ bool attn_empty(const tqt_attn_paged_params *p)
     return p->batch == 0 || p->q_tokens == 0 || p->q_heads == 0 || p->max_q_len == 0;
 }
 
+// What scores are multiplied by for powers of 2.
+float attn_log2_scale(float scale)
+{
+    return std::fabs(scale) * 1.4426950408889634f;
+}
+
 // The checks that the sizes alone decide.
 const char *attn_size_error(const tqt_attn_paged_params *p)
 {
@@ -72,8 +78,8 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
         p->d_token_stride % 8 != 0 || p->d_head_stride % 8 != 0) {
         return "rows of Q or D are off the 16-byte grid";
     }
-    if (!std::isfinite(p->scale)) {
-        return "scale is not finite";
+    if (!std::isfinite(attn_log2_scale(p->scale))) {
+        return "scale times log2(e) is not finite";
     }
     if (p->window > 0 && p->causal == 0) {
         return "a window needs causal";
@@ -194,7 +200,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.max_q_len = static_cast<int>(p->max_q_len);
     a.max_kv_len = static_cast<int>(p->max_kv_len);
     a.sign = p->scale > 0.0f ? 1.0f : p->scale < 0.0f ? -1.0f : 0.0f;
-    a.scale = p->scale == 0.0f ? 1.0f : std::fabs(p->scale) * 1.4426950408889634f;
+    a.scale = p->scale == 0.0f ? 1.0f : attn_log2_scale(p->scale);
     a.causal = p->causal != 0;
     // a window past every length is none
     a.window = p->window < (1u << 31) ? static_cast<int>(p->window) : 0;
