@@ -3,6 +3,7 @@ evaluated on the CPU."""
 
 import ctypes
 import os
+import random
 import subprocess
 import sys
 
@@ -26,6 +27,14 @@ def rules(tmp_path_factory):
 using namespace tqt;
 extern "C" {
 int r_first_key(int pos, int window) { return attn_first_key(pos, window); }
+long long r_span(long long q, long long kv, long long w) { return attn_span(q, kv, w); }
+int r_tile_rows() { return kAttnTileRows; }
+void r_split(long long tiles, long long kv_heads, long long span, long long d, int *out)
+{
+    const AttnSplit s = attn_call_split(tiles, kv_heads, span, d, 1000);
+    out[0] = s.chunk;
+    out[1] = s.splits;
+}
 void r_rope(long long heads, long long d, int grid16, int pow2, long long *out)
 {
     const RopeLaunch r = rope_launch(heads, d, grid16, pow2);
@@ -40,6 +49,8 @@ void r_rope(long long heads, long long d, int grid16, int pow2, long long *out)
                    check=True)
     lib = ctypes.CDLL(str(d / "r.so"))
     lib.r_first_key.argtypes = [ctypes.c_int] * 2
+    lib.r_span.argtypes, lib.r_span.restype = [ctypes.c_longlong] * 3, ctypes.c_longlong
+    lib.r_split.argtypes = [ctypes.c_longlong] * 4 + [ctypes.c_void_p]
     lib.r_rope.argtypes = [ctypes.c_longlong] * 2 + [ctypes.c_int] * 2 + [ctypes.c_void_p]
     return lib
 
@@ -132,3 +143,44 @@ def test_a_refused_table_aborts_in_both_forms():
 def test_scales_whose_log2_form_overflows_are_refused(scale, taken):
     for kind in H.ATTNS:
         assert (H.refusal("attn_paged_" + kind, H.changed(H.attn_params, scale=scale)) is None) == taken
+
+
+def split(rules, tiles, kv_heads, span, d):
+    out = (ctypes.c_int * 2)()
+    rules.r_split(tiles, kv_heads, span, d, out)
+    return tuple(out)
+
+
+@pytest.mark.parametrize("d", [16, 64, 128, 144, 192, 256])
+def test_splits_cover_every_tile_at_every_head_dim(rules, d):
+    """The spans of a tile's keys, from a multiple of 64 on, fit the splits that are launched."""
+    rng = random.Random(d)
+    m = rules.r_tile_rows()
+    several = 0
+    for _ in range(1500):
+        group = rng.choice([1, 3, 4, 8, 16, 50])
+        max_q, max_kv = rng.randint(1, 3000), rng.randint(1, 200000)
+        window = rng.choice([0, 0, rng.randint(1, 5000)])
+        tiles, heads = rng.randint(1, 60), rng.choice([1, 2, 8, 32])
+        span = rules.r_span(min(max_q, m // group + 2), max_kv, window)
+        chunk, splits = split(rules, tiles, heads, span, d)
+        assert chunk % 64 == 0 and splits >= 1
+        several += splits > 1
+        nq, kv = rng.randint(1, max_q), rng.randint(1, max_kv)
+        for tile in range(-(-nq * group // m)):
+            t0, t1 = tile * m // group, (min((tile + 1) * m, nq * group) - 1) // group
+            lo = max(kv - nq + t0 - window + 1, 0) if window else 0
+            hi = min(max(kv - nq + t1 + 1, 0), kv)
+            n = max(1, -(-(hi - lo // 64 * 64) // chunk))
+            assert n <= splits, (group, nq, kv, window, tile, chunk, splits)
+    assert several > 200
+
+
+@pytest.mark.parametrize("d,workgroups", [(64, 512), (128, 512), (192, 256), (256, 256)])
+def test_split_of_few_tiles_by_head_dim(rules, d, workgroups):
+    """As many workgroups as the chip holds of a head size; none where that many tiles are there already."""
+    assert split(rules, 4, 8, 2 ** 20, d)[1] in (workgroups // 32, workgroups // 32 + 1)
+    assert split(rules, workgroups // 8, 8, 2 ** 20, d)[1] == 1
+    for span in (1, 63, 64, 65, 300):
+        chunk, splits = split(rules, 1, 1, span, d)
+        assert splits == 1 and chunk >= span + 63

@@ -38,3 +38,22 @@ def test_few_rows_of_a_large_buffer(gpu):
     tol, tol_lse = R.attention_bound("f16", d, *want)
     assert (np.abs(R.host(out[:n]) - want[0]) <= tol).all()
     assert (np.abs(R.host(lse[:n]) - want[1]) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("max_q", [1, 2, 5, 20, 33])
+def test_queries_past_max_q_len_are_left_out(gpu, name, max_q):
+    """They keep what was there, and the others stand where they stood."""
+    lengths = [(50, 90), (3, 100), (1, 40), (34, 20)]
+    c = Case(name, lengths, 4, 2, 64).run(max_q=max_q)
+    for b, (nq, nk) in enumerate(lengths):
+        lo, n = int(c.starts[b]), min(nq, max_q)
+        assert (c.out[lo + n:lo + nq] == 9.0).all() and (c.lse[lo + n:lo + nq] == 9.0).all()
+        k, v, kept = c.keys(b)
+        see = (R.visible(nq, nk, True, 0) & kept[None])[:n]
+        want = R.attention(c.q[lo:lo + n], k, v, see, c.scale)
+        tol, tol_lse = R.attention_bound(c.kind, c.d, *want)
+        assert (np.abs(R.host(c.out[lo:lo + n]) - want[0]) <= tol).all()
+        seen = np.isfinite(want[1])
+        got = R.host(c.lse[lo:lo + n])
+        assert (np.abs(got[seen] - want[1][seen]) <= tol_lse[seen]).all() and np.isneginf(got[~seen]).all()
