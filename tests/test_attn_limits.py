@@ -184,3 +184,18 @@ def test_split_of_few_tiles_by_head_dim(rules, d, workgroups):
     for span in (1, 63, 64, 65, 300):
         chunk, splits = split(rules, 1, 1, span, d)
         assert splits == 1 and chunk >= span + 63
+
+
+def test_units_of_the_last_run_fit_32_bits():
+    """512 workgroups take equal runs of units, the last of which ends at or past the last unit: that end has to fit
+    32 bits too."""
+    def said(units):  # of 462 sequences with a key head each
+        assert units % 462 == 0
+        p = H.changed(H.attn_params, batch=462, q_tokens=462, q_heads=1, kv__kv_heads=1, ld_table=2 ** 23,
+                      kv__page_size=128, kv__num_pages=2 ** 20, max_kv_len=(units // 462 - 1) * 128)
+        return H.refusal("attn_paged_f16_f16", p)
+
+    top = 2 ** 31 - 2  # a multiple of 462
+    assert -(-(top - 2 * 462) // 512) * 512 < 2 ** 31 and said(top - 2 * 462) is None
+    for units in (top, top - 462):
+        assert -(-units // 512) * 512 >= 2 ** 31 and "too large" in said(units).decode()

@@ -41,8 +41,9 @@ const char *attn_size_error(const tqt_attn_paged_params *p)
     if (p->max_q_len * group >= top - 256) {
         return "max_q_len * (q_heads / kv_heads) too large";
     }
-    // units of the few-row kernel in 32 bits, and grids of fewer than 2^32 work-items
-    if (p->batch * p->kv.kv_heads * (p->max_kv_len / kAttnFewRowUnit + 1) >= top ||
+    // units of the few-row kernel in 32 bits, with the end of the last of up to 512 equal runs, which is up to 511
+    // past theirs, and grids of fewer than 2^32 work-items
+    if (p->batch * p->kv.kv_heads * (p->max_kv_len / kAttnFewRowUnit + 1) >= top - 512 ||
         p->batch * p->kv.kv_heads * kAttnFewRows >= (1u << 26)) {
         return "batch * kv_heads or batch * kv_heads * max_kv_len too large";
     }
