@@ -1,5 +1,6 @@
-"""One attention layer of a quantized transformer on the library alone: a prompt prefilled in chunks, then tokens
-decoded one by one, for a small batch of sequences.
+"""One attention layer of a quantized transformer on the library: a prompt prefilled in chunks, then tokens decoded one
+by one, for a small batch of sequences. (With --int8-cache torch casts the QKV product's f32 rows to the f16 that the
+append to an int8 cache takes.)
 
     python examples/attention_layer.py [--int8-cache] [--tokens N]
 

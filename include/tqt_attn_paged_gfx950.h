@@ -14,19 +14,21 @@
  * and a row that sees no key (or only keys with s_j = -infinity) gets D = 0 and lse = -infinity. What lies
  * in the cache at keys past kv_len, or in pages not named, is not used, whatever bits it holds, and an
  * infinity or NaN at a key reaches only the rows that see this key.
- * Scores, sums and the softmax are held in f32; the probabilities are rounded once, to Q's type (int8 caches:
- * times the value's scale, to f16), for the matrix product with the values. An int8 value's scale that is not
- * finite makes the rows that see its key not finite.
+ * Scores, sums and the softmax are held in f32; the probabilities are rounded once, to Q's type, for the matrix
+ * product with the values. Int8 caches: the probability times the value's scale is rounded, to f16, relative to
+ * the largest such term of the keys that the row sees (rows of zeros aside). Terms down to 2^-13 of it keep all
+ * bits, those below 2^-24 may be lost; value scales below 2^-60 lose bits in the same way. Scales may have either
+ * sign; one that is not finite makes the rows that see its key NaN.
  *
  * The function's name gives the type of Q and D, then the cache's: f16_f16, bf16_bf16, f16_qsi8dx,
  * bf16_qsi8dx (int8 with a scale for each token and head).
  *
  * Preconditions: q_heads a multiple of kv_heads; head_dim a multiple of 16 up to 256; rows of Q, D, k and
- * v on the 16-byte grid; scale times log2(e) finite; max_kv_len <= ld_table * page_size and below 2^30. max_q_len and max_kv_len bound
- * q_len and kv_len of every sequence: the launch and its workspace are sized by them, so that lengths may
- * change on the device between replays of a captured call. (A kv_len past max_kv_len is taken as max_kv_len,
- * queries past max_q_len of a sequence are left out. Bounds near the lengths make a call faster.) q_start does
- * not decrease, from 0 to at most q_tokens. workspace holds at least
+ * v on the 16-byte grid; scale times log2(e) finite; max_kv_len <= ld_table * page_size and below 2^30.
+ * max_q_len and max_kv_len bound q_len and kv_len of every sequence: the launch and its workspace are sized by
+ * them, so that lengths may change on the device between replays of a captured call. (A kv_len past max_kv_len
+ * is taken as max_kv_len, queries past max_q_len of a sequence are left out. Bounds near the lengths make a call
+ * faster.) q_start does not decrease, from 0 to at most q_tokens. workspace holds at least
  * tqt_get_workspace_size_attn_paged_gfx950 bytes on the 16-byte grid (it may be NULL for size 0), needs no
  * initial value, and is free again when the call has run. A row's sums do not depend on the order in which
  * workgroups run.

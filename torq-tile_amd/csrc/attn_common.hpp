@@ -203,10 +203,11 @@ __device__ __forceinline__ void few_row_pick(const FewRowBatch &x, int at, AttnS
     w.units = __builtin_amdgcn_readlane(x.work.units, at);
 }
 
-// Element offset of a key's row of one key head, or -1: past `hi`, or on no page of the cache.
 // 512 zero bytes: a row of keys that are not there.
 __device__ const u32x4 kAttnZeros[32] = {};
 
+// Where a key's row of one key head is: its element offset, its page and the offset in it. Not kept: past the keys
+// that are asked for, or on no page of the cache (then at is 0 and not read).
 struct KeyRow
 {
     long long at;

@@ -12,7 +12,9 @@
 // (its neighbour 32 lanes on holds the others), the statistics are one value a lane, and P^T is the second
 // operand of O^T = V^T P^T without leaving the registers. K and V go from memory to LDS directly (16 bytes a
 // lane, a tile ahead of their use, two stages; K one tile further), keys past the end and pages that are not
-// kept from a block of zeros; int8 rows through registers, where they become 16-bit whole numbers.
+// kept from a block of zeros; int8 rows through registers, where they become 16-bit whole numbers. Their decoding and
+// scales stand beside the exponentials (prompts of 4096 at d 64 / 128 / 256: 165 / 220 / 514 us, 106 / 168 / 360
+// over 16-bit caches).
 //
 // LDS layout of a tile: [key / 16][piece / 4][key % 16][4 pieces of 16 bytes], so that each lane of the 1 KB load
 // that fills one [16][4] block has the same key in all of its loads, and looks up one page per tile. A key's
