@@ -44,6 +44,13 @@ struct AttnArgs
     int few_workgroups, tile_chunk, tile_rows;
 };
 
+// With trees of new tokens: the mask's rows, of ld_mask words each, are Q's. causal is 0.
+struct AttnTreeArgs : AttnArgs
+{
+    const uint32_t *mask;
+    int ld_mask;
+};
+
 // A sequence of the batch, with every length brought inside what the host checked.
 struct AttnSeq
 {
@@ -84,6 +91,71 @@ __device__ __forceinline__ void attn_bounds(const AttnArgs &a, const AttnSeq &s,
     lo = attn_first_key(pos, a.window);
 }
 
+// The keys [lo, hi) that the rows of token `token` of a sequence may see.
+__device__ __forceinline__ void attn_row_keys(const AttnArgs &a, const AttnSeq &s, int token, int &lo, int &hi)
+{
+    attn_bounds(a, s, s.pos0 + token, lo, hi);
+}
+
+// Trees: new tokens are told apart by the mask, a window hides keys of the context alone.
+__device__ __forceinline__ void attn_row_keys(const AttnTreeArgs &a, const AttnSeq &s, int token, int &lo, int &hi)
+{
+    hi = s.kv_len;
+    lo = 0;
+    if (a.window > 0) {
+        const uint32_t *row = a.mask + static_cast<long long>(s.first + token) * a.ld_mask;
+        int n = 0;
+        for (int w = 0; w < a.ld_mask && 32 * w < s.q_len; ++w) {
+            const int bits = s.q_len - 32 * w;
+            n += __builtin_popcount(row[w] & (bits < 32 ? (1u << bits) - 1 : ~0u));
+        }
+        lo = min(attn_first_key(s.pos0 + n - 1, a.window), max(s.pos0, 0));
+    }
+}
+
+// The keys [first, last) that rows of the tokens t0 .. t1 may see, and [all_first, all_last) that each of them sees.
+struct AttnKeys
+{
+    int first, last, all_first, all_last;
+};
+
+__device__ __forceinline__ AttnKeys attn_keys(const AttnArgs &a, const AttnSeq &s, int t0, int t1)
+{
+    AttnKeys k;
+    attn_bounds(a, s, s.pos0 + t0, k.first, k.all_last);
+    attn_bounds(a, s, s.pos0 + t1, k.all_first, k.last);
+    return k;
+}
+
+// Trees: a mask names none to q_len of the new tokens, whichever it is.
+__device__ __forceinline__ AttnKeys attn_keys(const AttnTreeArgs &a, const AttnSeq &s, int, int)
+{
+    AttnKeys k;
+    const int context = max(s.pos0, 0);
+    k.first = min(attn_first_key(s.pos0 - 1, a.window), context);
+    k.last = static_cast<int>(min(static_cast<long long>(s.kv_len), s.pos0 + 32ll * a.ld_mask));
+    k.all_first = min(attn_first_key(s.kv_len - 1, a.window), context);
+    k.all_last = context;
+    return k;
+}
+
+// Bit i: whether key j0 + i is of the context or, by its mask, seen by the row of `token` (keys past kv_len are
+// told by attn_row_keys).
+__device__ __forceinline__ uint32_t attn_tree_bits(const AttnTreeArgs &a, const AttnSeq &s, int token, int j0)
+{
+    const uint32_t *row = a.mask + static_cast<long long>(s.first + token) * a.ld_mask;
+    auto word = [&](int w) { return w < a.ld_mask ? row[w] : 0u; };
+    const int t = j0 - s.pos0;
+    if (t <= -32) {
+        return ~0u;
+    }
+    if (t < 0) {
+        return word(0) << -t | ((1u << -t) - 1);
+    }
+    const int w = t >> 5, bit = t & 31;
+    return static_cast<uint32_t>((static_cast<uint64_t>(word(w + 1)) << 32 | word(w)) >> bit);
+}
+
 // Workgroups that share the keys [first, last) of some rows.
 __device__ __forceinline__ int attn_splits(int first, int last, int chunk)
 {
@@ -91,14 +163,14 @@ __device__ __forceinline__ int attn_splits(int first, int last, int chunk)
 }
 
 // The keys that a tile of `m` rows may see, from a multiple of 64 on.
-__device__ __forceinline__ void attn_tile_span(const AttnArgs &a, const AttnSeq &s, int tile, int m, int &first,
-                                               int &last)
+template <typename A>
+__device__ __forceinline__ AttnKeys attn_tile_keys(const A &a, const AttnSeq &s, int tile, int m)
 {
-    int unused;
     const int end = min((tile + 1) * m, s.nq * static_cast<int>(a.group.d)) - 1;
-    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(tile * m, a.group)), first, unused);
-    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(end, a.group)), unused, last);
-    first &= ~63;
+    AttnKeys k = attn_keys(a, s, static_cast<int>(fast_div(tile * m, a.group)),
+                           static_cast<int>(fast_div(end, a.group)));
+    k.first &= ~63;
+    return k;
 }
 
 // N elements of a row's sums from d0 on (d0 + N <= head_dim or d0 >= head_dim): the result where one
@@ -142,12 +214,13 @@ struct FewRowWork
     int first, last, units;  // units of one key head; 0: the sequence is not the few-row kernel's
 };
 
-__device__ __forceinline__ FewRowWork few_row_work(const AttnArgs &a, const AttnSeq &s)
+template <typename A>
+__device__ __forceinline__ FewRowWork few_row_work(const A &a, const AttnSeq &s)
 {
     FewRowWork w;
-    int unused;
-    attn_bounds(a, s, s.pos0, w.first, unused);
-    attn_bounds(a, s, s.pos0 + s.nq - 1, unused, w.last);
+    const AttnKeys k = attn_keys(a, s, 0, s.nq - 1);
+    w.first = k.first;
+    w.last = k.last;
     const int rows = s.nq * static_cast<int>(a.group.d);
     w.units = rows == 0 || rows > a.few_rows ? 0 : attn_splits(w.first, w.last, kAttnFewRowUnit);
     return w;
@@ -174,7 +247,8 @@ struct FewRowBatch
     int upto;        // units of sequences up to and with this lane's
 };
 
-__device__ __forceinline__ void few_row_batch(const AttnArgs &a, int b0, int before, int lane, FewRowBatch &x)
+template <typename A>
+__device__ __forceinline__ void few_row_batch(const A &a, int b0, int before, int lane, FewRowBatch &x)
 {
     const bool in = b0 + lane < a.batch;
     x.s = attn_seq(a, in ? b0 + lane : 0);
@@ -184,7 +258,8 @@ __device__ __forceinline__ void few_row_batch(const AttnArgs &a, int b0, int bef
 }
 
 // Units of a workgroup's run (all lanes of a wave call this); leaves the last 64 sequences in x.
-__device__ __forceinline__ int few_row_run(const AttnArgs &a, int lane, int &total, FewRowBatch &x)
+template <typename A>
+__device__ __forceinline__ int few_row_run(const A &a, int lane, int &total, FewRowBatch &x)
 {
     total = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {

@@ -36,9 +36,10 @@ struct FewRowTile
     static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 384 : 0);
 };
 
-template <typename T, typename C, int DP, bool kFull>
-__global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn_few_row_kernel(AttnArgs a)
+template <typename T, typename C, int DP, bool kFull, typename A>
+__global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn_few_row_kernel(A a)
 {
+    constexpr bool kTree = std::is_same<A, AttnTreeArgs>::value;
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
     constexpr bool kQuant = Tile::kQuant;
@@ -96,14 +97,13 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         const int token = static_cast<int>(fast_div(live ? col : 0, a.group, head_in_group));
         const int head = kvh * group + static_cast<int>(head_in_group);
         int row_lo, row_hi;
-        attn_bounds(a, s, s.pos0 + token, row_lo, row_hi);
+        attn_row_keys(a, s, token, row_lo, row_hi);
         if (!live) {
             row_hi = 0;
         }
         // keys outside [all_lo, all_hi) are not seen by every row
-        int all_lo, all_hi, unused;
-        attn_bounds(a, s, s.pos0, unused, all_hi);
-        attn_bounds(a, s, s.pos0 + s.nq - 1, all_lo, unused);
+        const AttnKeys keys = attn_keys(a, s, 0, s.nq - 1);
+        const int all_lo = keys.all_first, all_hi = keys.all_last;
 
         // Q^T: the elements that the pieces of K bring in the same steps
         half8 q[kSteps];
@@ -263,6 +263,11 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
             {
                 const int below = min(max(row_lo - jt, 0), 32), upto = min(max(row_hi - jt, 0), 32);
                 in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
+            }
+            if constexpr (kTree) {
+                if (jt + 32 > all_hi) {
+                    in &= attn_tree_bits(a, s, token, jt);
+                }
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {

@@ -24,7 +24,8 @@ __device__ __forceinline__ long long join_part(const JoinRow &j, int k)
 // The parts of row `at_row` (the same for the whole wave) and query head `head` (a lane's own). The first `few`
 // rows are those that the few-row kernel may have (`each` tokens of every sequence), the others are all rows
 // of Q, for the tile kernel's. parts <= 1: nothing to join.
-__device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each, int at_row, int head, int lane)
+template <typename A>
+__device__ __forceinline__ JoinRow join_row(const A &a, int few, int each, int at_row, int head, int lane)
 {
     JoinRow j = {0, 0, 0, 0, 0};
     const int heads = static_cast<int>(a.group.d);
@@ -68,9 +69,8 @@ __device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each
     const int kvh = static_cast<int>(fast_div(head, a.group, in_group));
     const int r = token * heads + static_cast<int>(in_group);
     if (tiles) {
-        int first, last;
-        attn_tile_span(a, s, r / a.tile_rows, a.tile_rows, first, last);
-        j.parts = attn_splits(first, last, a.tile_chunk);
+        const AttnKeys keys = attn_tile_keys(a, s, r / a.tile_rows, a.tile_rows);
+        j.parts = attn_splits(keys.first, keys.last, a.tile_chunk);
         j.step = static_cast<long long>(a.q_tokens) * a.q_heads;
         j.part0 = 2ll * a.few_workgroups * kAttnFewRows + static_cast<long long>(j.token) * a.q_heads + head;
         j.part1 = j.part0 + j.step;
@@ -86,8 +86,8 @@ __device__ __forceinline__ JoinRow join_row(const AttnArgs &a, int few, int each
 }
 
 // Few parts: a wave takes as many heads of a row as fit at 4 elements a lane.
-template <typename T, bool kQuant>
-__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few, int each, int rows)
+template <typename T, bool kQuant, typename A>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(A a, int few, int each, int rows)
 {
     const int lane = threadIdx.x & 63;
     const int across = a.head_dim / 4, per_wave = 64 / across;
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a, int few,
 
 // Many parts: a workgroup takes one row, head_dim / 4 threads along it and as many such groups as fit over the
 // parts.
-template <typename T, bool kQuant>
-__global__ __launch_bounds__(256) void attn_join_many_kernel(AttnArgs a, int few, int each)
+template <typename T, bool kQuant, typename A>
+__global__ __launch_bounds__(256) void attn_join_many_kernel(A a, int few, int each)
 {
     __shared__ f32x4 s_acc[256];
     __shared__ float s_sum[256];

@@ -6,7 +6,7 @@
 #include "attn_few_row.hpp"
 #include "attn_join.hpp"
 #include "attn_tile.hpp"
-#include "tqt_attn_paged_gfx950.h"
+#include "tqt_attn_tree_gfx950.h"
 
 #include <algorithm>
 #include <cmath>
@@ -54,7 +54,8 @@ const char *attn_size_error(const tqt_attn_paged_params *p)
     return nullptr;
 }
 
-const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool quant)
+// The checks of a call, `need` bytes of workspace apart.
+const char *attn_call_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool quant)
 {
     if (p == nullptr) {
         return "params == NULL";
@@ -85,11 +86,42 @@ const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool 
     if (p->window > 0 && p->causal == 0) {
         return "a window needs causal";
     }
-    const size_t need = tqt_get_workspace_size_attn_paged_gfx950(p);
+    return nullptr;
+}
+
+const char *attn_space_error(const tqt_attn_paged_params *p, size_t need)
+{
     if (p->workspace_size < need || (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace)))) {
         return "the workspace is too small or off the 16-byte grid";
     }
     return nullptr;
+}
+
+inline const char *attn_error(const tqt_attn_paged_params *p, size_t cache_bytes, bool quant)
+{
+    const char *e = attn_call_error(p, cache_bytes, quant);
+    return e != nullptr || attn_empty(p) ? e : attn_space_error(p, tqt_get_workspace_size_attn_paged_gfx950(p));
+}
+
+inline const char *attn_tree_error(const tqt_attn_tree_params *p, size_t cache_bytes, bool quant)
+{
+    if (p == nullptr) {
+        return "params == NULL";
+    }
+    const char *e = attn_call_error(&p->attn, cache_bytes, quant);
+    if (e != nullptr || attn_empty(&p->attn)) {
+        return e;
+    }
+    if (p->attn.causal != 1) {
+        return "trees need causal == 1";
+    }
+    if (p->mask == nullptr) {
+        return "mask == NULL";
+    }
+    if (p->ld_mask >= (1u << 25) || p->ld_mask * 32 < p->attn.max_q_len) {
+        return "ld_mask words hold fewer than max_q_len bits, or are too many";
+    }
+    return attn_space_error(&p->attn, tqt_get_workspace_size_attn_tree_gfx950(p));
 }
 
 // What a call launches, from its sizes (which have been checked).
@@ -110,7 +142,9 @@ int few_row_per_cu(size_t head_dim)
     return head_dim > 128 ? 1 : 2;
 }
 
-AttnPlan attn_plan(const tqt_attn_paged_params *p)
+// mask_bits: of a row, with trees, whose rows see the window before the context's end and all new tokens
+// that have a bit; else 0.
+AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
 {
     AttnPlan plan = {};
     const long long group = p->q_heads / p->kv.kv_heads;
@@ -124,7 +158,7 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     plan.few_tokens = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
     if (plan.run_few) {
         const long long heads = static_cast<long long>(p->batch) * p->kv.kv_heads;
-        const long long span = attn_span(plan.few_tokens, p->max_kv_len, window);
+        const long long span = attn_span(mask_bits > 0 ? mask_bits + 1 : plan.few_tokens, p->max_kv_len, window);
         plan.few_workgroups = attn_few_row_workgroups(
             heads * std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit),
             few_row_per_cu(p->kv.head_dim));
@@ -132,7 +166,9 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p)
     }
     plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
     plan.tile = attn_call_split(plan.tiles, p->kv.kv_heads,
-                                attn_span(std::min<long long>(p->max_q_len, kAttnTileRows / group + 2),
+                                attn_span(mask_bits > 0 ? mask_bits + 1
+                                                        : std::min<long long>(p->max_q_len,
+                                                                              kAttnTileRows / group + 2),
                                           p->max_kv_len, window),
                                 static_cast<long long>(p->kv.head_dim),
                                 static_cast<long long>(p->q_tokens * p->q_heads));
@@ -160,18 +196,9 @@ void by_head_dim(int head_dim, F f)
     }
 }
 
-template <typename T, typename C>
-bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *where)
+// Everything of a call but what its plan says.
+void set_attn(AttnArgs &a, const tqt_attn_paged_params *p)
 {
-    if (p == nullptr) {
-        return false;
-    }
-    const char *error = attn_error(p, sizeof(C), std::is_same<C, int8_t>::value);
-    TQT_REQUIRE(error == nullptr, error);
-    if (attn_empty(p)) {
-        return false;
-    }
-    AttnArgs a = {};
     a.q = p->Q;
     a.d = p->D;
     a.lse = p->lse;
@@ -205,7 +232,11 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.causal = p->causal != 0;
     // a window past every length is none
     a.window = p->window < (1u << 31) ? static_cast<int>(p->window) : 0;
-    const AttnPlan plan = attn_plan(p);
+}
+
+template <typename T, typename C, typename A>
+void launch_attn(A a, const AttnPlan &plan, const tqt_attn_paged_params *p, hipStream_t stream, const char *where)
+{
     a.few_workgroups = plan.few_workgroups;
     a.tile_chunk = plan.tile.chunk;
     a.tile_rows = kAttnTileRows;
@@ -214,7 +245,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     a.part_ml = a.part_o + plan.parts * a.head_dim;
     if (plan.run_few) {
         by_head_dim<64, 128, 256>(a.head_dim, [&](auto dp, auto full) {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value>), dim3(plan.few_workgroups),
+            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value, A>), dim3(plan.few_workgroups),
                                dim3(64 * kAttnFewRowWaves), 0, stream, a);
         });
         check_launch(where);
@@ -222,7 +253,7 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
     if (plan.run_tile) {
         const dim3 grid(static_cast<unsigned>(plan.tiles * a.kv_heads), plan.tile.splits);
         by_head_dim<64, 96, 128, 192, 256>(a.head_dim, [&](auto dp, auto full) {
-            hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value>), grid, dim3(256), 0, stream,
+            hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value, A>), grid, dim3(256), 0, stream,
                                a);
         });
         check_launch(where);
@@ -233,16 +264,53 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         const int each = static_cast<int>(plan.few_tokens), few = plan.run_few ? a.batch * each : 0;
         const int rows = few + (join_tile ? a.q_tokens : 0);
         if (plan.few_many || plan.tile.splits > kAttnJoinManyParts) {
-            hipLaunchKernelGGL((attn_join_many_kernel<T, kQuant>), dim3(static_cast<unsigned>(rows) * a.q_heads),
+            hipLaunchKernelGGL((attn_join_many_kernel<T, kQuant, A>), dim3(static_cast<unsigned>(rows) * a.q_heads),
                                dim3(256), 0, stream, a, few, each);
         } else {
             const int per_wave = 256 / a.head_dim;
             const long long items = static_cast<long long>(rows) * ((a.q_heads + per_wave - 1) / per_wave);
-            hipLaunchKernelGGL((attn_join_few_kernel<T, kQuant>), dim3(static_cast<unsigned>((items + 3) / 4)),
+            hipLaunchKernelGGL((attn_join_few_kernel<T, kQuant, A>), dim3(static_cast<unsigned>((items + 3) / 4)),
                                dim3(256), 0, stream, a, few, each, rows);
         }
     }
     check_launch(where);
+}
+
+
+template <typename T, typename C>
+bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *where)
+{
+    if (p == nullptr) {
+        return false;
+    }
+    const char *error = attn_error(p, sizeof(C), std::is_same<C, int8_t>::value);
+    TQT_REQUIRE(error == nullptr, error);
+    if (attn_empty(p)) {
+        return false;
+    }
+    AttnArgs a = {};
+    set_attn(a, p);
+    launch_attn<T, C>(a, attn_plan(p), p, stream, where);
+    return true;
+}
+
+template <typename T, typename C>
+bool run_attn_tree(const tqt_attn_tree_params *p, hipStream_t stream, const char *where)
+{
+    if (p == nullptr) {
+        return false;
+    }
+    const char *error = attn_tree_error(p, sizeof(C), std::is_same<C, int8_t>::value);
+    TQT_REQUIRE(error == nullptr, error);
+    if (attn_empty(&p->attn)) {
+        return false;
+    }
+    AttnTreeArgs a = {};
+    set_attn(a, &p->attn);
+    a.causal = 0;
+    a.mask = p->mask;
+    a.ld_mask = static_cast<int>(p->ld_mask);
+    launch_attn<T, C>(a, attn_plan(&p->attn, 32 * static_cast<long long>(p->ld_mask)), &p->attn, stream, where);
     return true;
 }
 
@@ -266,3 +334,20 @@ bool run_attn(const tqt_attn_paged_params *p, hipStream_t stream, const char *wh
         }                                                                                             \
     }
 
+
+#define TQT_ATTN_TREE_ENTRIES(NAME, T, C)                                                             \
+    const char *tqt_get_error_attn_tree_##NAME##_gfx950(const struct tqt_attn_tree_params *params)    \
+    {                                                                                                 \
+        return attn_tree_error(params, sizeof(C), std::is_same<C, int8_t>::value);                    \
+    }                                                                                                 \
+    void tqt_run_attn_tree_##NAME##_gfx950_async(const struct tqt_attn_tree_params *params,           \
+                                                 void *stream)                                        \
+    {                                                                                                 \
+        run_attn_tree<T, C>(params, as_stream(stream), "tqt_run_attn_tree_" #NAME "_gfx950");         \
+    }                                                                                                 \
+    void tqt_run_attn_tree_##NAME##_gfx950(const struct tqt_attn_tree_params *params)                 \
+    {                                                                                                 \
+        if (run_attn_tree<T, C>(params, nullptr, "tqt_run_attn_tree_" #NAME "_gfx950")) {             \
+            finish_sync(nullptr, "tqt_run_attn_tree_" #NAME "_gfx950");                               \
+        }                                                                                             \
+    }

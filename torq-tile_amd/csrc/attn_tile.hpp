@@ -61,9 +61,10 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
     return false;
 }
 
-template <typename T, typename C, int DP, int NW, bool kFull>
-__global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn_tile_kernel(AttnArgs a)
+template <typename T, typename C, int DP, int NW, bool kFull, typename A>
+__global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn_tile_kernel(A a)
 {
+    constexpr bool kTree = std::is_same<A, AttnTreeArgs>::value;
     constexpr bool kQuant = std::is_same<C, int8_t>::value;
     // The second product's type: int8 values are whole numbers in f16, which costs less than bf16 and rounds
     // the probabilities less.
@@ -89,13 +90,12 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
         return;
     }
     const int group = static_cast<int>(a.group.d);
-    int first, last;
-    attn_tile_span(a, s, tile, kM, first, last);
-    const int splits = attn_splits(first, last, a.tile_chunk);
+    const AttnKeys keys = attn_tile_keys(a, s, tile, kM);
+    const int splits = attn_splits(keys.first, keys.last, a.tile_chunk);
     if (split >= splits) {
         return;
     }
-    const int lo = first + split * a.tile_chunk, hi = min(last, lo + a.tile_chunk);
+    const int lo = keys.first + split * a.tile_chunk, hi = min(keys.last, lo + a.tile_chunk);
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -111,12 +111,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     const int token = static_cast<int>(fast_div(live ? row : rows - 1, a.group, head_in_group));
     const int head = kvh * group + static_cast<int>(head_in_group);
     int row_lo, row_hi;
-    attn_bounds(a, s, s.pos0 + token, row_lo, row_hi);
+    attn_row_keys(a, s, token, row_lo, row_hi);
     // the keys that every row of the workgroup sees
-    int all_lo, all_hi, unused;
-    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(tile * kM, a.group)), unused, all_hi);
-    attn_bounds(a, s, s.pos0 + static_cast<int>(fast_div(min((tile + 1) * kM, rows) - 1, a.group)), all_lo,
-                unused);
+    const int all_lo = keys.all_first, all_hi = keys.all_last;
 
     half8 q[DP / 16];
     const T *qp = static_cast<const T *>(a.q) + (s.first + token) * a.q_ts + head * a.q_hs;
@@ -268,6 +265,9 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             const int upto = min(max(row_hi - j0 - 32 * t, 0), 32);
             uint32_t in = static_cast<uint32_t>(kept >> (32 * t));
             in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
+            if constexpr (kTree) {
+                in &= attn_tree_bits(a, s, token, j0 + 32 * t);
+            }
             in >>= 4 * h;
             seen[t] = (in & 0xfu) | ((in >> 4) & 0xf0u) | ((in >> 8) & 0xf00u) | ((in >> 12) & 0xf000u);
         }

@@ -1,0 +1,390 @@
+// The bookkeeping of a step over a paged cache on gfx950: pages, block tables, lengths, slots, positions, tree masks.
+//
+// Bound by latency: some 30 bytes a token. What a sequence gets depends on all before it (rows, returned pages,
+// needs are running sums over the batch), so one workgroup goes over the batch, a thread a sequence; the rows
+// follow, a thread each, which finds its sequence by bisection: in the same workgroup where they are few (one launch
+// instead of two), by a grid of their own else. A row's page comes from the block table or, for pages taken in this
+// step, from the stack, by an index that follows from the sums alone; the row at a taken page's start writes the
+// table's entry, so that no thread walks over a sequence's pages.
+#include "fast_div.hpp"
+#include "paged_route.hpp"
+#include "tqt_hip_common.hpp"
+#include "tqt_paged_plan_gfx950.h"
+
+#include <algorithm>
+
+namespace tqt {
+namespace {
+
+constexpr int kPlanMostLen = 1 << 30;
+
+// What the rows of a sequence need to know.
+struct PlanSeq
+{
+    int kv_len;
+    int held;        // entries of the block table that it had; -1: refused
+    uint32_t fresh;  // entry j >= held comes from place fresh - j of the stack
+    int unused;
+};
+
+struct PlanArgs
+{
+    const int32_t *new_len, *kv_len, *held, *free_count;
+    int32_t *kv_len_out, *held_out, *free_count_out, *refused;
+    int32_t *table, *free_pages, *q_start, *positions;
+    int64_t *slots;
+    const int32_t *parent;
+    uint32_t *mask;
+    PlanSeq *seqs;  // [batch], or nullptr: in LDS
+    long long ld_table;
+    int batch, tokens, num_pages, free_capacity, ld_mask;
+    FastDiv page;
+};
+
+// A row: where its sequence and its token are known from q_start and seqs.
+__device__ __forceinline__ void plan_row(const PlanArgs &a, int row, int total, const int32_t *q_start,
+                                         const PlanSeq *seqs)
+{
+    if (row >= total) {
+        a.slots[row] = -1;
+        a.positions[row] = 0;
+        for (int w = 0; w < a.ld_mask; ++w) {
+            a.mask[static_cast<long long>(row) * a.ld_mask + w] = 0;
+        }
+        return;
+    }
+    // the last sequence that begins at or before the row
+    int b = 0;
+    for (int end = a.batch; end - b > 1;) {
+        const int mid = (b + end) >> 1;
+        if (q_start[mid] <= row) {
+            b = mid;
+        } else {
+            end = mid;
+        }
+    }
+    const int first = q_start[b], i = row - first;
+    const PlanSeq s = seqs[b];
+    uint32_t offset;
+    const uint32_t col = fast_div(static_cast<uint32_t>(s.kv_len + i), a.page, offset);
+    long long slot = -1;
+    if (s.held >= 0) {
+        int32_t *entry = a.table + b * a.ld_table + col;
+        int page;
+        if (static_cast<int>(col) < s.held) {
+            page = *entry;
+        } else {
+            page = a.free_pages[s.fresh - col];
+            if (offset == 0) {
+                *entry = page;
+            }
+        }
+        if (page >= 0 && page < a.num_pages) {
+            slot = static_cast<long long>(page) * a.page.d + offset;
+        }
+    }
+    a.slots[row] = slot;
+    if (a.parent == nullptr) {
+        a.positions[row] = s.kv_len + i;
+        return;
+    }
+    // up the tree: numbers fall, so the mask's words are done from the last to the first
+    auto above = [&](int t) {
+        const int p = a.parent[first + t];
+        return p < t ? max(p, -1) : -1;
+    };
+    int t = i, depth = -1;
+    for (; (t >> 5) >= a.ld_mask; t = above(t)) {
+        ++depth;
+    }
+    for (int w = a.ld_mask - 1; w >= 0; --w) {
+        uint32_t word = 0;
+        for (; t >= 0 && (t >> 5) == w; t = above(t)) {
+            word |= 1u << (t & 31);
+            ++depth;
+        }
+        a.mask[static_cast<long long>(row) * a.ld_mask + w] = word;
+    }
+    a.positions[row] = s.kv_len + depth;
+}
+
+__device__ __forceinline__ long long plan_wave_sum(long long x, int lane)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const long long y = __shfl_up(x, off);
+        x += lane >= off ? y : 0;
+    }
+    return x;
+}
+
+// The sum of the workgroup's threads up to and with this one, and of all of them. Every thread calls it.
+__device__ __forceinline__ long long plan_sum(long long x, long long (&s_wave)[kPlanThreads / 64], long long &all)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long upto = plan_wave_sum(x, lane);
+    __syncthreads();
+    if (lane == 63) {
+        s_wave[wave] = upto;
+    }
+    __syncthreads();
+    const long long other = plan_wave_sum(lane < kPlanThreads / 64 ? s_wave[lane] : 0, lane);
+    all = __shfl(other, 63);
+    return upto + (wave > 0 ? __shfl(other, wave - 1) : 0);
+}
+
+// Sequences, a thread each, kPlanThreads at a time; with kRows also the rows (then batch <= kPlanThreads).
+template <bool kRows>
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
+{
+    __shared__ long long s_wave[kPlanThreads / 64];
+    __shared__ int s_list[kPlanThreads], s_held[kPlanThreads];
+    __shared__ long long s_upto[kPlanThreads];
+    __shared__ int32_t s_start[kRows ? kPlanThreads + 1 : 1];
+    __shared__ PlanSeq s_seqs[kRows ? kPlanThreads : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int count = min(max(a.free_count[0], 0), a.free_capacity);
+
+    // 1. pages of ended sequences
+    long long top = count;
+    for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+        const bool ended = b0 + tid < a.batch && a.new_len[b0 + tid] < 0;
+        const int held =
+            ended ? static_cast<int>(min(max(static_cast<long long>(a.held[b0 + tid]), 0ll), a.ld_table)) : 0;
+        if (!__syncthreads_or(held > 0)) {
+            continue;
+        }
+        long long n;
+        const int at = static_cast<int>(plan_sum(held > 0, s_wave, n)) - 1;
+        if (held > 0) {
+            s_list[at] = b0 + tid;
+            s_held[at] = held;
+        }
+        __syncthreads();
+        // a wave counts the kept pages of every so many-th of them
+        for (int k = wave; k < n; k += kPlanThreads / 64) {
+            const int32_t *table = a.table + s_list[k] * a.ld_table;
+            int kept = 0;
+#pragma unroll 8
+            for (int j = lane; j < s_held[k]; j += 64) {
+                const int page = table[j];
+                kept += page >= 0 && page < a.num_pages;
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                kept += __shfl_xor(kept, off);
+            }
+            if (lane == 0) {
+                s_upto[k] = kept;
+            }
+        }
+        __syncthreads();
+        long long returned;
+        const long long upto = plan_sum(tid < n ? s_upto[tid] : 0, s_wave, returned);
+        if (tid < n) {
+            s_upto[tid] = upto - s_upto[tid];
+        }
+        __syncthreads();
+        for (int k = wave; k < n; k += kPlanThreads / 64) {
+            const int32_t *table = a.table + s_list[k] * a.ld_table;
+            long long to = top + s_upto[k];
+            for (int j0 = 0; j0 < s_held[k]; j0 += 64) {
+                const int page = j0 + lane < s_held[k] ? table[j0 + lane] : -1;
+                const bool kept = page >= 0 && page < a.num_pages;
+                const unsigned long long all = __ballot(kept);
+                const long long here = to + __builtin_popcountll(all & ((1ull << lane) - 1));
+                if (kept && here < a.free_capacity) {
+                    a.free_pages[here] = page;
+                }
+                to += __builtin_popcountll(all);
+            }
+        }
+        top += returned;
+        __syncthreads();
+    }
+    top = min(top, static_cast<long long>(a.free_capacity));
+
+    // 2., 3. what the others need and get
+    long long rows = 0, needed = 0, taken = 0;
+    int refused = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+        const int b = b0 + tid;
+        const bool in = b < a.batch;
+        const int given = in ? a.new_len[b] : 0;
+        const bool ended = given < 0;
+        const int n = min(max(given, 0), kPlanMostLen);
+        const int kv_len = in ? min(max(a.kv_len[b], 0), kPlanMostLen) : 0;
+        uint32_t rest;
+        const long long own = fast_div(static_cast<uint32_t>(kv_len), a.page, rest) + (rest > 0);
+        const long long held =
+            in ? max(min(max(static_cast<long long>(a.held[b]), 0ll), a.ld_table), own) : 0;
+        long long all;
+        const long long rows_upto = rows + plan_sum(n, s_wave, all);
+        const long long before = rows_upto - n;
+        rows += all;
+        long long need = 0;
+        bool fits = in && !ended && rows_upto <= a.tokens && kv_len + static_cast<long long>(n) <= kPlanMostLen;
+        if (fits) {
+            const long long want = fast_div(static_cast<uint32_t>(kv_len + n), a.page, rest) + (rest > 0);
+            need = max(want - held, 0ll);
+            fits = held + need <= a.ld_table;
+            need = fits ? need : 0;
+        }
+        const long long upto = needed + plan_sum(need, s_wave, all);
+        needed += all;
+        const bool served = fits && (need == 0 || upto <= top);
+        plan_sum(served ? need : 0, s_wave, all);
+        taken += all;
+        plan_sum(in && !ended && !served, s_wave, all);
+        refused += static_cast<int>(all);
+        if (in) {
+            a.kv_len_out[b] = ended ? 0 : served ? kv_len + n : kv_len;
+            a.held_out[b] = static_cast<int32_t>(ended ? 0 : served ? held + need : held);
+            const int32_t start = static_cast<int32_t>(min(before, static_cast<long long>(a.tokens)));
+            const PlanSeq s = {kv_len, served ? static_cast<int>(held) : -1,
+                               static_cast<uint32_t>(top - 1 - (upto - need) + held), 0};
+            a.q_start[b] = start;
+            if constexpr (kRows) {
+                s_start[tid] = start;
+                s_seqs[tid] = s;
+            } else {
+                a.seqs[b] = s;
+            }
+        }
+    }
+    const int total = static_cast<int>(min(rows, static_cast<long long>(a.tokens)));
+    if (tid == 0) {
+        a.q_start[a.batch] = total;
+        a.free_count_out[0] = static_cast<int32_t>(top - taken);
+        a.refused[0] = refused;
+    }
+    if constexpr (kRows) {
+        __syncthreads();
+        for (int row = tid; row < a.tokens; row += kPlanThreads) {
+            plan_row(a, row, total, s_start, s_seqs);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a)
+{
+    const int row = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+    if (row < a.tokens) {
+        plan_row(a, row, a.q_start[a.batch], a.q_start, a.seqs);
+    }
+}
+
+const char *plan_error(const tqt_paged_plan_params *p)
+{
+    if (p == nullptr) {
+        return "params == NULL";
+    }
+    if (p->batch >= (1u << 16) || p->tokens >= (1u << 30) || p->ld_table >= (1u << 31) ||
+        p->free_capacity >= (1u << 31) || p->ld_mask >= (1u << 25)) {
+        return "batch, tokens, ld_table, free_capacity or ld_mask too large";
+    }
+    if (p->page_size == 0 || p->page_size >= (1u << 31) || p->num_pages >= (1u << 31) ||
+        p->num_pages * p->page_size >= (1u << 31)) {
+        return "page_size is 0, or the cache holds 2^31 tokens or more";
+    }
+    if (p->free_count == nullptr || p->free_count_out == nullptr || p->refused == nullptr ||
+        p->q_start == nullptr || (p->free_pages == nullptr && p->free_capacity > 0)) {
+        return "free_count / free_count_out / refused / q_start / free_pages == NULL";
+    }
+    if (p->batch > 0 && (p->new_len == nullptr || p->kv_len == nullptr || p->kv_len_out == nullptr ||
+                         p->held == nullptr || p->held_out == nullptr ||
+                         (p->block_table == nullptr && p->ld_table > 0))) {
+        return "new_len / kv_len / kv_len_out / held / held_out / block_table == NULL";
+    }
+    if (p->tokens > 0 && (p->positions == nullptr || p->slots == nullptr)) {
+        return "positions / slots == NULL";
+    }
+    if (p->parent == nullptr ? p->mask != nullptr || p->ld_mask > 0
+                             : p->mask == nullptr || p->ld_mask == 0) {
+        return "trees need parent, mask and ld_mask together";
+    }
+    const size_t need = tqt_get_workspace_size_paged_plan_gfx950(p);
+    if (p->workspace_size < need || (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace)))) {
+        return "the workspace is too small or off the 16-byte grid";
+    }
+    return nullptr;
+}
+
+bool run_plan(const tqt_paged_plan_params *p, hipStream_t stream, const char *where)
+{
+    if (p == nullptr) {
+        return false;
+    }
+    const char *error = plan_error(p);
+    TQT_REQUIRE(error == nullptr, error);
+    PlanArgs a = {};
+    a.new_len = p->new_len;
+    a.kv_len = p->kv_len;
+    a.held = p->held;
+    a.free_count = p->free_count;
+    a.kv_len_out = p->kv_len_out;
+    a.held_out = p->held_out;
+    a.free_count_out = p->free_count_out;
+    a.refused = p->refused;
+    a.table = p->block_table;
+    a.free_pages = p->free_pages;
+    a.q_start = p->q_start;
+    a.positions = p->positions;
+    a.slots = p->slots;
+    a.parent = p->parent;
+    a.mask = p->mask;
+    a.seqs = static_cast<PlanSeq *>(p->workspace);
+    a.ld_table = static_cast<long long>(p->ld_table);
+    a.batch = static_cast<int>(p->batch);
+    a.tokens = static_cast<int>(p->tokens);
+    a.num_pages = static_cast<int>(p->num_pages);
+    a.free_capacity = static_cast<int>(p->free_capacity);
+    a.ld_mask = static_cast<int>(p->ld_mask);
+    a.page = make_fast_div(static_cast<uint32_t>(p->page_size));
+    if (plan_one_launch(a.batch, a.tokens)) {
+        hipLaunchKernelGGL((plan_kernel<true>), dim3(1), dim3(kPlanThreads), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((plan_kernel<false>), dim3(1), dim3(kPlanThreads), 0, stream, a);
+        check_launch(where);
+        if (a.tokens > 0) {
+            hipLaunchKernelGGL(plan_rows_kernel, dim3((a.tokens + 255) / 256), dim3(256), 0, stream, a);
+        }
+    }
+    check_launch(where);
+    return true;
+}
+
+}  // namespace
+}  // namespace tqt
+
+using namespace tqt;
+
+extern "C" {
+
+size_t tqt_get_workspace_size_paged_plan_gfx950(const struct tqt_paged_plan_params *params)
+{
+    if (params == nullptr || params->batch >= (1u << 16) || params->tokens >= (1u << 30) ||
+        plan_one_launch(static_cast<long long>(params->batch), static_cast<long long>(params->tokens))) {
+        return 0;
+    }
+    return params->batch * sizeof(PlanSeq);
+}
+
+const char *tqt_get_error_paged_plan_gfx950(const struct tqt_paged_plan_params *params)
+{
+    return plan_error(params);
+}
+
+void tqt_run_paged_plan_gfx950_async(const struct tqt_paged_plan_params *params, void *stream)
+{
+    run_plan(params, as_stream(stream), "tqt_run_paged_plan_gfx950");
+}
+
+void tqt_run_paged_plan_gfx950(const struct tqt_paged_plan_params *params)
+{
+    if (run_plan(params, nullptr, "tqt_run_paged_plan_gfx950")) {
+        finish_sync(nullptr, "tqt_run_paged_plan_gfx950");
+    }
+}
+
+}  // extern "C"

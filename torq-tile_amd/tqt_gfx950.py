@@ -270,6 +270,114 @@ class AttnPagedParams(ctypes.Structure):
     ]
 
 
+class HeadNorm(ctypes.Structure):
+    """struct tqt_head_norm (include/tqt_norm_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("weight", c_vp),
+        ("shift", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class NormRopeParams(ctypes.Structure):
+    """struct tqt_norm_rope_params (include/tqt_norm_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("rope", RopeParams),
+        ("norm", HeadNorm),
+    ]
+
+
+class NormRopeGradParams(ctypes.Structure):
+    """struct tqt_norm_rope_grad_params (include/tqt_norm_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("forward", NormRopeParams),
+        ("dY", c_vp),
+        ("dy_token_stride", c_size),
+        ("dy_head_stride", c_size),
+        ("dX", c_vp),
+        ("dx_token_stride", c_size),
+        ("dx_head_stride", c_size),
+        ("dweight", c_vp),
+        ("workspace", c_vp),
+        ("workspace_size", c_size),
+    ]
+
+
+class KVAppendNormRopeParams(ctypes.Structure):
+    """struct tqt_kv_append_norm_rope_params (include/tqt_kv_append_norm_rope_gfx950.h)."""
+
+    _fields_ = [
+        ("append", KVAppendRopeParams),
+        ("q_norm", HeadNorm),
+        ("k_norm", HeadNorm),
+    ]
+
+
+class PagedPlanParams(ctypes.Structure):
+    """struct tqt_paged_plan_params (include/tqt_paged_plan_gfx950.h)."""
+
+    _fields_ = [
+        ("batch", c_size),
+        ("tokens", c_size),
+        ("page_size", c_size),
+        ("num_pages", c_size),
+        ("new_len", c_vp),
+        ("kv_len", c_vp),
+        ("kv_len_out", c_vp),
+        ("held", c_vp),
+        ("held_out", c_vp),
+        ("block_table", c_vp),
+        ("ld_table", c_size),
+        ("free_pages", c_vp),
+        ("free_capacity", c_size),
+        ("free_count", c_vp),
+        ("free_count_out", c_vp),
+        ("refused", c_vp),
+        ("q_start", c_vp),
+        ("positions", c_vp),
+        ("slots", c_vp),
+        ("parent", c_vp),
+        ("mask", c_vp),
+        ("ld_mask", c_size),
+        ("workspace", c_vp),
+        ("workspace_size", c_size),
+    ]
+
+
+class KVKeepParams(ctypes.Structure):
+    """struct tqt_kv_keep_params (include/tqt_kv_keep_gfx950.h)."""
+
+    _fields_ = [
+        ("batch", c_size),
+        ("max_keep", c_size),
+        ("q_start", c_vp),
+        ("kv_len", c_vp),
+        ("kv_len_out", c_vp),
+        ("keep", c_vp),
+        ("ld_keep", c_size),
+        ("keep_len", c_vp),
+        ("block_table", c_vp),
+        ("ld_table", c_size),
+        ("layers", c_size),
+        ("layer_stride", c_size),
+        ("scale_layer_stride", c_size),
+        ("kv", PagedKV),
+    ]
+
+
+class AttnTreeParams(ctypes.Structure):
+    """struct tqt_attn_tree_params (include/tqt_attn_tree_gfx950.h)."""
+
+    _fields_ = [
+        ("attn", AttnPagedParams),
+        ("mask", c_vp),
+        ("ld_mask", c_size),
+    ]
+
+
 # C type (as written in include/*.h, parameter name dropped) -> ctypes type.
 _CTYPES = {
     "size_t": c_size,
@@ -293,6 +401,12 @@ _CTYPES = {
     "const struct tqt_rope_table_params *": ctypes.POINTER(RopeTableParams),
     "const struct tqt_kv_append_rope_params *": ctypes.POINTER(KVAppendRopeParams),
     "const struct tqt_attn_paged_params *": ctypes.POINTER(AttnPagedParams),
+    "const struct tqt_norm_rope_params *": ctypes.POINTER(NormRopeParams),
+    "const struct tqt_norm_rope_grad_params *": ctypes.POINTER(NormRopeGradParams),
+    "const struct tqt_kv_append_norm_rope_params *": ctypes.POINTER(KVAppendNormRopeParams),
+    "const struct tqt_paged_plan_params *": ctypes.POINTER(PagedPlanParams),
+    "const struct tqt_kv_keep_params *": ctypes.POINTER(KVKeepParams),
+    "const struct tqt_attn_tree_params *": ctypes.POINTER(AttnTreeParams),
 }
 # f16 / bf16 values are passed in SSE registers on x86-64, which ctypes cannot fill: functions
 # taking them are checked for export but not bound (the test shim in tests/abi_shim calls them).
