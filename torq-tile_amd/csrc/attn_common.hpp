@@ -37,7 +37,7 @@ struct AttnArgs
     int few_rows;  // sequences of at most so many rows to a key head are the few-row kernel's
     // Parts of rows whose keys several workgroups have, in the workspace: f32 sums not divided by the sum of
     // probabilities, and (maximum in log2, sum). The few-row kernel's come first: workgroup w's are 2 w (of a
-    // sequence that began before its run) and 2 w + 1 (of one that ends after it), kAttnFewRows rows each;
+    // sequence that began before its run) and 2 w + 1 (of one that ends after it), attn_few_rows rows each;
     // then the tile kernel's, [split][row of Q][query head], each of tile_chunk keys.
     float *part_o;   // [][head_dim]
     float *part_ml;  // [][2]
@@ -50,6 +50,20 @@ struct AttnTreeArgs : AttnArgs
     const uint32_t *mask;
     int ld_mask;
 };
+
+// Rows of one key head that the few-row kernel takes at most, which is what a part of its rows has.
+template <typename A>
+constexpr int attn_few_rows(int head_dim)
+{
+    return std::is_same<A, AttnTreeArgs>::value ? attn_tree_few_rows(head_dim) : kAttnFewRows;
+}
+
+// Workgroups of the few-row kernel that a CU holds, by their registers.
+template <typename A>
+constexpr int attn_few_row_per_cu(int head_dim)
+{
+    return head_dim > (std::is_same<A, AttnTreeArgs>::value ? 64 : 128) ? 1 : 2;
+}
 
 // A sequence of the batch, with every length brought inside what the host checked.
 struct AttnSeq

@@ -37,9 +37,10 @@ struct FewRowTile
 };
 
 template <typename T, typename C, int DP, bool kFull, typename A>
-__global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn_few_row_kernel(A a)
+__global__ __launch_bounds__(64 * kAttnFewRowWaves, attn_few_row_per_cu<A>(DP)) void attn_few_row_kernel(A a)
 {
     constexpr bool kTree = std::is_same<A, AttnTreeArgs>::value;
+    constexpr int kRows = attn_few_rows<A>(DP), kCols = kRows / 16;  // columns of 16 rows
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
     constexpr bool kQuant = Tile::kQuant;
@@ -88,48 +89,59 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         const int lo = work.first + unit0 * kAttnFewRowUnit;
         const int hi = unit1 == work.units ? work.last : lo + (unit1 - unit0) * kAttnFewRowUnit;
         const bool whole = unit1 - unit0 == work.units;
-        const long long part = whole ? -1 : (2ll * wg + (unit0 == 0)) * kAttnFewRows;
+        const long long part = whole ? -1 : (2ll * wg + (unit0 == 0)) * kRows;
         const int32_t *table = a.table + b * a.ld_table;
         const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
-        // this lane's row, and the keys that it sees
-        const bool live = col < rows;
+        // this lane's rows, 16 c + col, and the keys that they see
         uint32_t head_in_group;
-        const int token = static_cast<int>(fast_div(live ? col : 0, a.group, head_in_group));
-        const int head = kvh * group + static_cast<int>(head_in_group);
-        int row_lo, row_hi;
-        attn_row_keys(a, s, token, row_lo, row_hi);
-        if (!live) {
-            row_hi = 0;
+        int token[kCols], row_lo[kCols], row_hi[kCols];
+        half8 q[kCols][kSteps];
+        const auto used = [&](int c) { return c == 0 || 16 * c < rows; };  // whether a column has rows
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            const bool live = 16 * c + col < rows;
+            token[c] = static_cast<int>(fast_div(live ? 16 * c + col : 0, a.group, head_in_group));
+            const int head = kvh * group + static_cast<int>(head_in_group);
+            attn_row_keys(a, s, token[c], row_lo[c], row_hi[c]);
+            if (!live) {
+                row_hi[c] = 0;
+            }
+            // Q^T: the elements that the pieces of K bring in the same steps
+            const T *qp = static_cast<const T *>(a.q) + (s.first + token[c]) * a.q_ts + head * a.q_hs;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int d0 = kQuant ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+                half8 x = {};
+                if (live && d0 < a.head_dim) {
+                    x = *reinterpret_cast<const half8 *>(qp + d0);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = static_cast<T>(static_cast<float>(x[e]) * a.sign);
+                }
+                q[c][i] = x;
+            }
         }
         // keys outside [all_lo, all_hi) are not seen by every row
         const AttnKeys keys = attn_keys(a, s, 0, s.nq - 1);
         const int all_lo = keys.all_first, all_hi = keys.all_last;
 
-        // Q^T: the elements that the pieces of K bring in the same steps
-        half8 q[kSteps];
-        const T *qp = static_cast<const T *>(a.q) + (s.first + token) * a.q_ts + head * a.q_hs;
+        f32x4 o[kCols][DP / 16];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const int d0 = kQuant ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
-            half8 x = {};
-            if (live && d0 < a.head_dim) {
-                x = *reinterpret_cast<const half8 *>(qp + d0);
+        for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                o[c][i] = 0.0f;
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = static_cast<T>(static_cast<float>(x[e]) * a.sign);
-            }
-            q[i] = x;
-        }
-
-        f32x4 o[DP / 16];
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            o[i] = 0.0f;
         }
         // sums of 2^(s - ref) and 2^(s - ref) v; `ref` (log2) is the maximum so far of s, for int8 of s and the
         // logarithm of the value's scale (value_scale), over the keys that the row sees
-        float ref = -INFINITY, l = 0.0f;
+        float ref[kCols], l[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            ref[c] = -INFINITY;
+            l[c] = 0.0f;
+        }
 
         // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
         u32x4 kx[2][kPieces], vx[2][kPieces];
@@ -176,19 +188,29 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
         }
         for (; j0 < hi; j0 += kAttnFewRowUnit) {
             // S^T
-            f32x4 st[2];
+            f32x4 st[kCols][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                st[t] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    st[c][t] = 0.0f;
+                }
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
+                    half8 h[2];
                     if constexpr (kQuant) {
-                        half8 h[2];
                         int8_to_half(kx[t][i], h);
-                        st[t] = mfma16(h[0], q[2 * i], st[t]);
-                        st[t] = mfma16(h[1], q[2 * i + 1], st[t]);
                     } else {
-                        st[t] = mfma16(__builtin_bit_cast(half8, kx[t][i]), q[i], st[t]);
+                        h[0] = __builtin_bit_cast(half8, kx[t][i]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        if constexpr (kQuant) {
+                            st[c][t] = mfma16(h[0], q[c][2 * i], st[c][t]);
+                            st[c][t] = mfma16(h[1], q[c][2 * i + 1], st[c][t]);
+                        } else {
+                            st[c][t] = mfma16(h[0], q[c][i], st[c][t]);
+                        }
                     }
                 }
             }
@@ -258,70 +280,75 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
             }
 
             // softmax of this lane's 8 keys: 16 t + 4 g + r
-            float top = -INFINITY;
-            uint32_t seen = 0, in = keptmask;
-            {
-                const int below = min(max(row_lo - jt, 0), 32), upto = min(max(row_hi - jt, 0), 32);
-                in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
-            }
-            if constexpr (kTree) {
-                if (jt + 32 > all_hi) {
-                    in &= attn_tree_bits(a, s, token, jt);
-                }
-            }
+            prob8 p[kCols];
+            uint32_t seen[kCols];
+            float alpha[kCols];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 ks = 1.0f, log = 0.0f;
-                if constexpr (kQuant) {
-                    ks = *reinterpret_cast<f32x4 *>(scales + 16 * t + 4 * g);
-                    log = *reinterpret_cast<f32x4 *>(scales + 64 + 16 * t + 4 * g);
+            for (int c = 0; c < kCols; ++c) {
+                float top = -INFINITY;
+                uint32_t in = keptmask;
+                seen[c] = 0;
+                {
+                    const int below = min(max(row_lo[c] - jt, 0), 32), upto = min(max(row_hi[c] - jt, 0), 32);
+                    in &= static_cast<uint32_t>((1ull << upto) - 1) & ~static_cast<uint32_t>((1ull << below) - 1);
                 }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int key = 16 * t + 4 * g + r;
-                    const bool see = (in >> key) & 1;
-                    seen |= static_cast<uint32_t>(see) << (4 * t + r);
-                    float x = st[t][r];
-                    if constexpr (kQuant) {
-                        x *= ks[r];
+                if constexpr (kTree) {
+                    if (jt + 32 > all_hi) {
+                        in &= attn_tree_bits(a, s, token[c], jt);
                     }
-                    st[t][r] = see ? x * a.scale : -INFINITY;
-                    // a NaN stays one: exp2 of it, below (that of a score of -infinity beside an infinite
-                    // logarithm is passed over)
-                    top = fmaxf(top, kQuant ? st[t][r] + log[r] : st[t][r]);
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(ref, top);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float alpha;
-            if constexpr (kQuant) {
-                alpha = value_half_step(ref, base);
-                l = l * alpha * alpha;
-                alpha *= alpha;
-                // infinite: a score, or the scale of a value that the row sees
-                l = top == INFINITY ? __builtin_nanf("") : l;
-            } else {
-                alpha = __builtin_amdgcn_exp2f(ref - base);
-                l *= alpha;
-            }
-            ref = top;
-            prob8 p;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 vsc = 1.0f;
-                if constexpr (kQuant) {
-                    vsc = *reinterpret_cast<f32x4 *>(scales + 32 + 16 * t + 4 * g);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float e = __builtin_amdgcn_exp2f(st[t][r] - base);
-                    l += e;
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 ks = 1.0f, log = 0.0f;
                     if constexpr (kQuant) {
-                        e *= vsc[r];
+                        ks = *reinterpret_cast<f32x4 *>(scales + 16 * t + 4 * g);
+                        log = *reinterpret_cast<f32x4 *>(scales + 64 + 16 * t + 4 * g);
                     }
-                    p[4 * t + r] = static_cast<P>(e);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int key = 16 * t + 4 * g + r;
+                        const bool see = (in >> key) & 1;
+                        seen[c] |= static_cast<uint32_t>(see) << (4 * t + r);
+                        float x = st[c][t][r];
+                        if constexpr (kQuant) {
+                            x *= ks[r];
+                        }
+                        st[c][t][r] = see ? x * a.scale : -INFINITY;
+                        // a NaN stays one: exp2 of it, below (that of a score of -infinity beside an infinite
+                        // logarithm is passed over)
+                        top = fmaxf(top, kQuant ? st[c][t][r] + log[r] : st[c][t][r]);
+                    }
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(ref[c], top);
+                const float base = top == -INFINITY ? 0.0f : top;
+                if constexpr (kQuant) {
+                    alpha[c] = value_half_step(ref[c], base);
+                    l[c] = l[c] * alpha[c] * alpha[c];
+                    alpha[c] *= alpha[c];
+                    // infinite: a score, or the scale of a value that the row sees
+                    l[c] = top == INFINITY ? __builtin_nanf("") : l[c];
+                } else {
+                    alpha[c] = __builtin_amdgcn_exp2f(ref[c] - base);
+                    l[c] *= alpha[c];
+                }
+                ref[c] = top;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 vsc = 1.0f;
+                    if constexpr (kQuant) {
+                        vsc = *reinterpret_cast<f32x4 *>(scales + 32 + 16 * t + 4 * g);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float e = __builtin_amdgcn_exp2f(st[c][t][r] - base);
+                        l[c] += e;
+                        if constexpr (kQuant) {
+                            e *= vsc[r];
+                        }
+                        p[c][4 * t + r] = static_cast<P>(e);
+                    }
                 }
             }
             const char *columns = mine + (4 * g + (col >> 2)) * kStride + 8 * (lane & 3);
@@ -331,25 +358,31 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
                 return u32x4{x0[0], x0[1], x1[0], x1[1]};
             };
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                o[i] = o[i] * alpha;
+            for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) {
+                    o[c][i] = o[c][i] * alpha[c];
+                }
             }
             if constexpr (!kQuant) {
                 if (bad) {
-                    half8 see1;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        see1[e] = static_cast<T>((seen >> e) & 1 ? 1.0f : 0.0f);
-                    }
+                    for (int c = 0; c < kCols; ++c) {
+                        half8 see1;
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) {
-                        u32x4 clean, code;
-                        split_not_finite<T>(value(i), clean, code);
-                        const f32x4 count =
-                            mfma16(__builtin_bit_cast(half8, code), see1, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        for (int e = 0; e < 8; ++e) {
+                            see1[e] = static_cast<T>((seen[c] >> e) & 1 ? 1.0f : 0.0f);
+                        }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            o[i][r] += not_finite_term(count[r]);
+                        for (int i = 0; i < DP / 16; ++i) {
+                            u32x4 clean, code;
+                            split_not_finite<T>(value(i), clean, code);
+                            const f32x4 count =
+                                mfma16(__builtin_bit_cast(half8, code), see1, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                o[c][i][r] += not_finite_term(count[r]);
+                            }
                         }
                     }
                     wave_lds_fence();
@@ -365,50 +398,60 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, DP == 256 ? 1 : 2) void attn
             // O^T
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                o[i] = mfma16(__builtin_bit_cast(prob8, value(i)), p, o[i]);
+                const prob8 v = __builtin_bit_cast(prob8, value(i));
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    o[c][i] = mfma16(v, p[c], o[c][i]);
+                }
             }
         }
 
-        // the four waves meet: sums of the lanes of a row, then of the waves
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        wave_lds_fence();
-        float *mo = reinterpret_cast<float *>(mine);  // [16][DP]
+        // the four waves meet, 16 rows at a time: sums of the lanes of a row, then of the waves
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = kQuant ? o[i] * kValueUp : o[i];
-        }
-        if (lane < 16) {
-            s_m[wave][lane] = ref;
-            s_l[wave][lane] = l;
-        }
-        __syncthreads();
-        constexpr int kThreads = 4 * kAttnFewRowWaves, kOut = DP / kThreads;  // threads along a row, elements of each
-        const int r = tid / kThreads, d0 = (tid % kThreads) * kOut;
-        if (r < rows) {
-            float mm = s_m[0][r];
-#pragma unroll
-            for (int w = 1; w < kAttnFewRowWaves; ++w) {
-                mm = fmaxf(mm, s_m[w][r]);
+        for (int c = 0; c < kCols; ++c) {
+            if (!used(c)) {
+                break;
             }
-            const float base = mm == -INFINITY ? 0.0f : mm;
-            float sum = 0.0f, acc[kOut] = {};
+            l[c] += __shfl_xor(l[c], 16);
+            l[c] += __shfl_xor(l[c], 32);
+            wave_lds_fence();
+            float *mo = reinterpret_cast<float *>(mine);  // [16][DP]
 #pragma unroll
-            for (int w = 0; w < kAttnFewRowWaves; ++w) {
-                float part = s_l[w][r];
-                const float f = part_factor<kQuant>(s_m[w][r], base, part);
-                sum += part;
-                const float *from = reinterpret_cast<const float *>(lds + w * Tile::kWaveBytes) + r * DP + d0;
+            for (int i = 0; i < DP / 16; ++i) {
+                *reinterpret_cast<f32x4 *>(mo + col * DP + 16 * i + 4 * g) = kQuant ? o[c][i] * kValueUp : o[c][i];
+            }
+            if (lane < 16) {
+                s_m[wave][lane] = ref[c];
+                s_l[wave][lane] = l[c];
+            }
+            __syncthreads();
+            constexpr int kThreads = 4 * kAttnFewRowWaves, kOut = DP / kThreads;  // threads of a row, elements of each
+            const int r = tid / kThreads, d0 = (tid % kThreads) * kOut;
+            if (16 * c + r < rows) {
+                float mm = s_m[0][r];
 #pragma unroll
-                for (int e = 0; e < kOut; ++e) {
-                    acc[e] += from[e] * f;
+                for (int w = 1; w < kAttnFewRowWaves; ++w) {
+                    mm = fmaxf(mm, s_m[w][r]);
                 }
+                const float base = mm == -INFINITY ? 0.0f : mm;
+                float sum = 0.0f, acc[kOut] = {};
+#pragma unroll
+                for (int w = 0; w < kAttnFewRowWaves; ++w) {
+                    float part_sum = s_l[w][r];
+                    const float f = part_factor<kQuant>(s_m[w][r], base, part_sum);
+                    sum += part_sum;
+                    const float *from = reinterpret_cast<const float *>(lds + w * Tile::kWaveBytes) + r * DP + d0;
+#pragma unroll
+                    for (int e = 0; e < kOut; ++e) {
+                        acc[e] += from[e] * f;
+                    }
+                }
+                const int out_token = static_cast<int>(fast_div(16 * c + r, a.group, head_in_group));
+                attn_put<T, kOut>(a, part < 0 ? -1 : part + 16 * c + r, s.first + out_token,
+                                  kvh * group + static_cast<int>(head_in_group), d0, acc, mm, sum);
             }
-            const int out_token = static_cast<int>(fast_div(r, a.group, head_in_group));
-            attn_put<T, kOut>(a, part < 0 ? -1 : part + r, s.first + out_token,
-                              kvh * group + static_cast<int>(head_in_group), d0, acc, mm, sum);
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 

@@ -121,6 +121,10 @@ inline const char *attn_tree_error(const tqt_attn_tree_params *p, size_t cache_b
     if (p->ld_mask >= (1u << 25) || p->ld_mask * 32 < p->attn.max_q_len) {
         return "ld_mask words hold fewer than max_q_len bits, or are too many";
     }
+    // the join's grid, as in attn_size_error
+    if (p->attn.batch * p->attn.kv.kv_heads * 32 >= (1u << 26)) {
+        return "batch * kv_heads too large";
+    }
     return attn_space_error(&p->attn, tqt_get_workspace_size_attn_tree_gfx950(p));
 }
 
@@ -136,32 +140,27 @@ struct AttnPlan
     long long parts;  // rows of the workspace
 };
 
-// Workgroups of the few-row kernel that a CU holds, by their registers.
-int few_row_per_cu(size_t head_dim)
-{
-    return head_dim > 128 ? 1 : 2;
-}
-
 // mask_bits: of a row, with trees, whose rows see the window before the context's end and all new tokens
 // that have a bit; else 0.
 AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
 {
+    const int head_dim = static_cast<int>(p->kv.head_dim);
+    const int few_rows = mask_bits > 0 ? attn_few_rows<AttnTreeArgs>(head_dim) : kAttnFewRows;
     AttnPlan plan = {};
     const long long group = p->q_heads / p->kv.kv_heads;
     const long long window = static_cast<long long>(std::min<size_t>(p->window, 1u << 31));
     // where the bounds say that every sequence has max_q_len tokens, or there is one, its length decides;
     // a shorter one after all is the tile kernel's
     const bool alike = p->batch == 1 || p->q_tokens == p->batch * p->max_q_len;
-    plan.run_few = group <= kAttnFewRows &&
-                   (!alike || static_cast<long long>(p->max_q_len) * group <= kAttnFewRows);
-    plan.run_tile = static_cast<long long>(p->max_q_len) * group > kAttnFewRows;
-    plan.few_tokens = std::min<long long>(p->max_q_len, std::max(1ll, kAttnFewRows / group));
+    plan.run_few = group <= few_rows && (!alike || static_cast<long long>(p->max_q_len) * group <= few_rows);
+    plan.run_tile = static_cast<long long>(p->max_q_len) * group > few_rows;
+    plan.few_tokens = std::min<long long>(p->max_q_len, std::max(1ll, few_rows / group));
     if (plan.run_few) {
         const long long heads = static_cast<long long>(p->batch) * p->kv.kv_heads;
         const long long span = attn_span(mask_bits > 0 ? mask_bits + 1 : plan.few_tokens, p->max_kv_len, window);
         plan.few_workgroups = attn_few_row_workgroups(
             heads * std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit),
-            few_row_per_cu(p->kv.head_dim));
+            mask_bits > 0 ? attn_few_row_per_cu<AttnTreeArgs>(head_dim) : attn_few_row_per_cu<AttnArgs>(head_dim));
         plan.few_many = plan.few_workgroups > heads * kAttnJoinManyParts;
     }
     plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
@@ -172,7 +171,7 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
                                           p->max_kv_len, window),
                                 static_cast<long long>(p->kv.head_dim),
                                 static_cast<long long>(p->q_tokens * p->q_heads));
-    plan.parts = 2ll * plan.few_workgroups * kAttnFewRows;
+    plan.parts = 2ll * plan.few_workgroups * few_rows;
     if (plan.run_tile && plan.tile.splits > 1) {
         plan.parts += plan.tile.splits * static_cast<long long>(p->q_tokens) * p->q_heads;
     }
@@ -240,7 +239,7 @@ void launch_attn(A a, const AttnPlan &plan, const tqt_attn_paged_params *p, hipS
     a.few_workgroups = plan.few_workgroups;
     a.tile_chunk = plan.tile.chunk;
     a.tile_rows = kAttnTileRows;
-    a.few_rows = plan.run_few ? kAttnFewRows : 0;
+    a.few_rows = plan.run_few ? attn_few_rows<A>(a.head_dim) : 0;
     a.part_o = static_cast<float *>(p->workspace);
     a.part_ml = a.part_o + plan.parts * a.head_dim;
     if (plan.run_few) {

@@ -11,6 +11,11 @@ namespace tqt {
 // Rows of one key head that the few-row kernel takes: (new tokens) x (query heads per key head), as many
 // as its matrix instruction has columns.
 constexpr int kAttnFewRows = 16;
+// With trees, two columns of that instruction; one at heads over 128, whose two do not fit the registers.
+constexpr int attn_tree_few_rows(int head_dim)
+{
+    return head_dim > 128 ? 16 : 32;
+}
 
 // Keys that the queries of one sequence may see at most.
 constexpr long long attn_span(long long max_q_len, long long max_kv_len, long long window)
