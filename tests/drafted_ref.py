@@ -125,7 +125,7 @@ def plan(new_len, kv_len, held, table, free, count, tokens, page, num_pages, par
         served = False
         if new_len[b] >= 0:
             need = max(pages_of(int(kv_len[b]) + n) - h, 0)
-            fits = total <= tokens and h + need <= ld and kv_len[b] + n <= 2 ** 30
+            fits = (n == 0 or total <= tokens) and h + need <= ld and kv_len[b] + n <= 2 ** 30
             need = need if fits else 0
             served = fits and (need == 0 or needed + need <= top)
             needed += need

@@ -12,11 +12,13 @@
 #include "tqt_paged_plan_gfx950.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tqt {
 namespace {
 
 constexpr int kPlanMostLen = 1 << 30;
+constexpr int kPlanStarts = 2048;  // sequences whose first rows the rows' workgroups hold in LDS
 
 // What the rows of a sequence need to know.
 struct PlanSeq
@@ -41,9 +43,9 @@ struct PlanArgs
     FastDiv page;
 };
 
-// A row: where its sequence and its token are known from q_start and seqs.
+// A row: its sequence follows from q_start and seqs (these and parent are the call's or copies of them in LDS).
 __device__ __forceinline__ void plan_row(const PlanArgs &a, int row, int total, const int32_t *q_start,
-                                         const PlanSeq *seqs)
+                                         const PlanSeq *seqs, const int32_t *parent)
 {
     if (row >= total) {
         a.slots[row] = -1;
@@ -90,7 +92,7 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int row, int total, 
     }
     // up the tree: numbers fall, so the mask's words are done from the last to the first
     auto above = [&](int t) {
-        const int p = a.parent[first + t];
+        const int p = parent[first + t];
         return p < t ? max(p, -1) : -1;
     };
     int t = i, depth = -1;
@@ -108,88 +110,145 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int row, int total, 
     a.positions[row] = s.kv_len + depth;
 }
 
-__device__ __forceinline__ long long plan_wave_sum(long long x, int lane)
+// Sum of the lanes up to and with this one, by moves between lanes (row_shr and row_bcast: shuffles go through LDS, and
+// each of their six steps waits some hundred cycles).
+__device__ __forceinline__ long long plan_wave_sum(long long x)
 {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const long long y = __shfl_up(x, off);
-        x += lane >= off ? y : 0;
-    }
+    auto add = [&](auto ctrl, auto rows) {
+        const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), ctrl.value, rows.value, 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), ctrl.value, rows.value, 0xf, false);
+        x += static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 |
+                                    static_cast<uint32_t>(lo));
+    };
+    typedef std::integral_constant<int, 0xf> All;
+    add(std::integral_constant<int, 0x111>(), All());
+    add(std::integral_constant<int, 0x112>(), All());
+    add(std::integral_constant<int, 0x114>(), All());
+    add(std::integral_constant<int, 0x118>(), All());
+    add(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+    add(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
     return x;
 }
 
-// The sum of the workgroup's threads up to and with this one, and of all of them. Every thread calls it.
-__device__ __forceinline__ long long plan_sum(long long x, long long (&s_wave)[kPlanThreads / 64], long long &all)
+__device__ __forceinline__ long long plan_lane(long long x, int lane)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long upto = plan_wave_sum(x, lane);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), lane);
+    return static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(
+                                      __builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane)))
+                                      << 32 |
+                                  lo);
+}
+
+// The sum of the workgroup's threads up to and with this one, and of all of them. Every thread calls it.
+// `on`: whether the wave has sequences, the same for all of its lanes; others only meet the barriers.
+__device__ __forceinline__ long long plan_sum(long long x, bool on, long long (&s_wave)[kPlanThreads / 64],
+                                              long long &all)
+{
+    constexpr int kWaves = kPlanThreads / 64;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const long long upto = on ? plan_wave_sum(x) : 0;
     __syncthreads();
     if (lane == 63) {
         s_wave[wave] = upto;
     }
     __syncthreads();
-    const long long other = plan_wave_sum(lane < kPlanThreads / 64 ? s_wave[lane] : 0, lane);
-    all = __shfl(other, 63);
-    return upto + (wave > 0 ? __shfl(other, wave - 1) : 0);
+    const long long other = plan_wave_sum(lane < kWaves ? s_wave[lane] : 0);
+    all = plan_lane(other, kWaves - 1);
+    return upto + (wave > 0 ? plan_lane(other, wave - 1) : 0);
 }
 
-// Sequences, a thread each, kPlanThreads at a time; with kRows also the rows (then batch <= kPlanThreads).
+// Pages of an ended sequence that a lane keeps from counting them to putting them on the stack.
+constexpr int kPlanHeld = 8;
+
+// Sequences, a thread each, kPlanThreads at a time; with kRows also the rows (then batch <= kPlanThreads). Bound by
+// what its waves issue and by the rows' chains of reads: waves without sequences skip the sums, but take rows. 64
+// sequences, five of them ended, with 1014 rows in trees take 9.5 us so, 10.4 where all waves do all, 14.1 with 256
+// threads, and 14.8 with shuffles, two sums more and the parents read from global memory.
 template <bool kRows>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
 {
     __shared__ long long s_wave[kPlanThreads / 64];
     __shared__ int s_list[kPlanThreads], s_held[kPlanThreads];
     __shared__ long long s_upto[kPlanThreads];
+    __shared__ unsigned long long s_taken;
+    __shared__ int s_refused;
     __shared__ int32_t s_start[kRows ? kPlanThreads + 1 : 1];
     __shared__ PlanSeq s_seqs[kRows ? kPlanThreads : 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int count = min(max(a.free_count[0], 0), a.free_capacity);
+    __shared__ int32_t s_parent[kRows ? kPlanRowsOfOne : 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // what the first round of threads reads is asked for together: each wait for memory takes a microsecond
+    const int first_count = a.free_count[0];
+    const bool first_in = tid < a.batch;
+    const int first_new = first_in ? a.new_len[tid] : 0, first_held = first_in ? a.held[tid] : 0;
+    const int first_kv = first_in ? a.kv_len[tid] : 0;
+    auto new_len = [&](int b) { return b < kPlanThreads ? first_new : b < a.batch ? a.new_len[b] : 0; };
+    auto held_pages = [&](int b) { return b < kPlanThreads ? first_held : b < a.batch ? a.held[b] : 0; };
+    if constexpr (kRows) {
+        // the way up a tree is a chain of reads
+        if (a.parent != nullptr) {
+            for (int row = tid; row < a.tokens; row += kPlanThreads) {
+                s_parent[row] = a.parent[row];
+            }
+        }
+    }
+    if (tid == 0) {
+        s_taken = 0;
+        s_refused = 0;
+    }
+    const int count = min(max(first_count, 0), a.free_capacity);
 
     // 1. pages of ended sequences
     long long top = count;
     for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
-        const bool ended = b0 + tid < a.batch && a.new_len[b0 + tid] < 0;
-        const int held =
-            ended ? static_cast<int>(min(max(static_cast<long long>(a.held[b0 + tid]), 0ll), a.ld_table)) : 0;
+        const bool on = b0 + 64 * wave < a.batch;
+        int held = 0;
+        if (on && new_len(b0 + tid) < 0) {
+            held = static_cast<int>(min(max(static_cast<long long>(held_pages(b0 + tid)), 0ll), a.ld_table));
+        }
         if (!__syncthreads_or(held > 0)) {
             continue;
         }
         long long n;
-        const int at = static_cast<int>(plan_sum(held > 0, s_wave, n)) - 1;
+        const int at = static_cast<int>(plan_sum(held > 0, on, s_wave, n)) - 1;
         if (held > 0) {
             s_list[at] = b0 + tid;
             s_held[at] = held;
         }
         __syncthreads();
-        // a wave counts the kept pages of every so many-th of them
+        // a wave counts the kept pages of every so many-th of them; those of its first are at hand afterwards
+        int pages[kPlanHeld];
         for (int k = wave; k < n; k += kPlanThreads / 64) {
             const int32_t *table = a.table + s_list[k] * a.ld_table;
             int kept = 0;
-#pragma unroll 8
-            for (int j = lane; j < s_held[k]; j += 64) {
+            if (k == wave) {
+#pragma unroll
+                for (int i = 0; i < kPlanHeld; ++i) {
+                    pages[i] = 64 * i + lane < s_held[k] ? table[64 * i + lane] : -1;
+                    kept += pages[i] >= 0 && pages[i] < a.num_pages;
+                }
+            }
+            for (int j = (k == wave ? 64 * kPlanHeld : 0) + lane; j < s_held[k]; j += 64) {
                 const int page = table[j];
                 kept += page >= 0 && page < a.num_pages;
             }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                kept += __shfl_xor(kept, off);
-            }
+            const long long all = plan_lane(plan_wave_sum(kept), 63);
             if (lane == 0) {
-                s_upto[k] = kept;
+                s_upto[k] = all;
             }
         }
         __syncthreads();
         long long returned;
-        const long long upto = plan_sum(tid < n ? s_upto[tid] : 0, s_wave, returned);
+        const long long mine = tid < n ? s_upto[tid] : 0;
+        const long long upto = plan_sum(mine, 64 * wave < n, s_wave, returned);
         if (tid < n) {
-            s_upto[tid] = upto - s_upto[tid];
+            s_upto[tid] = upto - mine;
         }
         __syncthreads();
         for (int k = wave; k < n; k += kPlanThreads / 64) {
             const int32_t *table = a.table + s_list[k] * a.ld_table;
             long long to = top + s_upto[k];
-            for (int j0 = 0; j0 < s_held[k]; j0 += 64) {
-                const int page = j0 + lane < s_held[k] ? table[j0 + lane] : -1;
+            auto put = [&](int page) {
                 const bool kept = page >= 0 && page < a.num_pages;
                 const unsigned long long all = __ballot(kept);
                 const long long here = to + __builtin_popcountll(all & ((1ull << lane) - 1));
@@ -197,6 +256,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
                     a.free_pages[here] = page;
                 }
                 to += __builtin_popcountll(all);
+            };
+            if (k == wave) {
+#pragma unroll
+                for (int i = 0; i < kPlanHeld; ++i) {
+                    put(pages[i]);
+                }
+            }
+            for (int j0 = k == wave ? 64 * kPlanHeld : 0; j0 < s_held[k]; j0 += 64) {
+                put(j0 + lane < s_held[k] ? table[j0 + lane] : -1);
             }
         }
         top += returned;
@@ -204,43 +272,52 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
     }
     top = min(top, static_cast<long long>(a.free_capacity));
 
-    // 2., 3. what the others need and get
-    long long rows = 0, needed = 0, taken = 0;
-    int refused = 0;
+    // 2., 3. what the others need and get. Sequences whose rows do not fit come after all whose rows do, so that the
+    // sums may count their pages. Those that get pages come before all that get none: the last one's sum is what
+    // is taken.
+    long long rows = 0, needed = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
         const int b = b0 + tid;
         const bool in = b < a.batch;
-        const int given = in ? a.new_len[b] : 0;
+        if (b0 + 64 * wave >= a.batch) {
+            long long all;
+            plan_sum(0, false, s_wave, all);
+            rows += all;
+            plan_sum(0, false, s_wave, all);
+            continue;
+        }
+        const int given = new_len(b), has = held_pages(b);
+        const int kv_len = min(max(b < kPlanThreads ? first_kv : in ? a.kv_len[b] : 0, 0), kPlanMostLen);
         const bool ended = given < 0;
         const int n = min(max(given, 0), kPlanMostLen);
-        const int kv_len = in ? min(max(a.kv_len[b], 0), kPlanMostLen) : 0;
         uint32_t rest;
         const long long own = fast_div(static_cast<uint32_t>(kv_len), a.page, rest) + (rest > 0);
-        const long long held =
-            in ? max(min(max(static_cast<long long>(a.held[b]), 0ll), a.ld_table), own) : 0;
-        long long all;
-        const long long rows_upto = rows + plan_sum(n, s_wave, all);
-        const long long before = rows_upto - n;
-        rows += all;
+        const long long held = max(min(max(static_cast<long long>(has), 0ll), a.ld_table), own);
         long long need = 0;
-        bool fits = in && !ended && rows_upto <= a.tokens && kv_len + static_cast<long long>(n) <= kPlanMostLen;
+        bool fits = in && !ended && kv_len + static_cast<long long>(n) <= kPlanMostLen;
         if (fits) {
             const long long want = fast_div(static_cast<uint32_t>(kv_len + n), a.page, rest) + (rest > 0);
             need = max(want - held, 0ll);
             fits = held + need <= a.ld_table;
             need = fits ? need : 0;
         }
-        const long long upto = needed + plan_sum(need, s_wave, all);
+        long long all;
+        const long long rows_upto = rows + plan_sum(n, true, s_wave, all);
+        rows += all;
+        const long long upto = needed + plan_sum(need, true, s_wave, all);
         needed += all;
-        const bool served = fits && (need == 0 || upto <= top);
-        plan_sum(served ? need : 0, s_wave, all);
-        taken += all;
-        plan_sum(in && !ended && !served, s_wave, all);
-        refused += static_cast<int>(all);
+        const bool served = fits && (n == 0 || rows_upto <= a.tokens) && (need == 0 || upto <= top);
+        if (served && need > 0) {
+            atomicMax(&s_taken, static_cast<unsigned long long>(upto));
+        }
+        const unsigned long long refused = __ballot(in && !ended && !served);
+        if (lane == 0 && refused != 0) {
+            atomicAdd(&s_refused, static_cast<int>(__builtin_popcountll(refused)));
+        }
         if (in) {
             a.kv_len_out[b] = ended ? 0 : served ? kv_len + n : kv_len;
             a.held_out[b] = static_cast<int32_t>(ended ? 0 : served ? held + need : held);
-            const int32_t start = static_cast<int32_t>(min(before, static_cast<long long>(a.tokens)));
+            const int32_t start = static_cast<int32_t>(min(rows_upto - n, static_cast<long long>(a.tokens)));
             const PlanSeq s = {kv_len, served ? static_cast<int>(held) : -1,
                                static_cast<uint32_t>(top - 1 - (upto - need) + held), 0};
             a.q_start[b] = start;
@@ -253,24 +330,34 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
         }
     }
     const int total = static_cast<int>(min(rows, static_cast<long long>(a.tokens)));
+    __syncthreads();
     if (tid == 0) {
         a.q_start[a.batch] = total;
-        a.free_count_out[0] = static_cast<int32_t>(top - taken);
-        a.refused[0] = refused;
+        a.free_count_out[0] = static_cast<int32_t>(top - static_cast<long long>(s_taken));
+        a.refused[0] = s_refused;
     }
     if constexpr (kRows) {
-        __syncthreads();
         for (int row = tid; row < a.tokens; row += kPlanThreads) {
-            plan_row(a, row, total, s_start, s_seqs);
+            plan_row(a, row, total, s_start, s_seqs, s_parent);
         }
     }
 }
 
 __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a)
 {
+    __shared__ int32_t s_start[kPlanStarts];
     const int row = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+    const int total = a.q_start[a.batch];
+    const int32_t *q_start = a.q_start;
+    if (a.batch <= kPlanStarts) {
+        for (int b = threadIdx.x; b < a.batch; b += 256) {
+            s_start[b] = a.q_start[b];
+        }
+        __syncthreads();
+        q_start = s_start;
+    }
     if (row < a.tokens) {
-        plan_row(a, row, a.q_start[a.batch], a.q_start, a.seqs);
+        plan_row(a, row, total, q_start, a.seqs, a.parent);
     }
 }
 
