@@ -159,6 +159,17 @@ def test_few_trees_over_many_keys(gpu, name, d, window):
 
 
 @pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("short", [3, 9])
+def test_whole_sequences_beside_split_tiles(gpu, name, short):
+    """Many sequences of few rows, whose keys are not split, beside a tree of tiles whose keys are (short 9: rows of a
+    tile, of two columns at heads of 64)."""
+    rng = np.random.default_rng(short)
+    lengths = [(short, int(rng.integers(short, 500))) for _ in range(70)] + [(40, 1900), (1, 1), (70, 1300)]
+    Tree(name, lengths, 4, 2, 64).run().check()
+    Tree(name, lengths[40:], 8, 4, 128, window=900).run().check()
+
+
+@pytest.mark.parametrize("name", NAMES)
 def test_rows_that_see_nothing(gpu, name):
     """No keys, or more new tokens than keys, so that some of the new ones' own keys do not exist."""
     for chain in (0.0, 1.0):

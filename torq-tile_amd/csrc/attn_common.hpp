@@ -49,7 +49,28 @@ struct AttnTreeArgs : AttnArgs
 {
     const uint32_t *mask;
     int ld_mask;
+    int few_unit;  // keys of the few-row kernel's units: kAttnFewRowUnit, or all of a sequence's
 };
+
+// Keys of the few-row kernel's units.
+__device__ __forceinline__ int attn_few_unit(const AttnArgs &)
+{
+    return kAttnFewRowUnit;
+}
+__device__ __forceinline__ int attn_few_unit(const AttnTreeArgs &a)
+{
+    return a.few_unit;
+}
+
+// Rows of the few-row kernel's parts, which the tile kernel's follow.
+__device__ __forceinline__ long long attn_few_parts(const AttnArgs &a)
+{
+    return 2ll * a.few_workgroups * kAttnFewRows;
+}
+__device__ __forceinline__ long long attn_few_parts(const AttnTreeArgs &a)
+{
+    return a.few_unit == kAttnFewRowUnit ? 2ll * a.few_workgroups * attn_tree_few_rows(a.head_dim) : 0;
+}
 
 // Rows of one key head that the few-row kernel takes at most, which is what a part of its rows has.
 template <typename A>
@@ -236,7 +257,7 @@ __device__ __forceinline__ FewRowWork few_row_work(const A &a, const AttnSeq &s)
     w.first = k.first;
     w.last = k.last;
     const int rows = s.nq * static_cast<int>(a.group.d);
-    w.units = rows == 0 || rows > a.few_rows ? 0 : attn_splits(w.first, w.last, kAttnFewRowUnit);
+    w.units = rows == 0 || rows > a.few_rows ? 0 : attn_splits(w.first, w.last, attn_few_unit(a));
     return w;
 }
 

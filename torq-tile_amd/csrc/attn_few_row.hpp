@@ -1,5 +1,5 @@
 // Attention of few rows: sequences with at most 16 rows to a key head (one decoded token of up to 16 query
-// heads, or a few tokens of fewer).
+// heads, or a few tokens of fewer); with trees of new tokens 32, in two columns of the matrix instruction.
 //
 // Bound by the cache's bytes: per key 2 d elements are read once for 4 d 16 flops on the matrix cores. The
 // batch's keys are cut into units of 128 for each key head, and the workgroups that fit the chip at once take
@@ -19,6 +19,12 @@
 // own LDS, which is read down its columns. Int8 rows become 16-bit whole numbers on the way (exactly), their
 // scales go to the scores and the probabilities (32 sequences of 1024-4096 keys, 32 key heads of 128, f16: 150 us,
 // 4.7 TB/s).
+//
+// Trees: two columns share the keys' operands and the values' reads from LDS. At heads of 128 they take 408 registers,
+// so one wave a SIMD, which still keeps the memory busy: 64 trees of 3-8 tokens over 2048-8192 keys (bf16, 32 / 8
+// heads of 128) take 256-264 us (5.1-5.3 TB/s) and 9 of join; with two waves 91 registers spill, and as tiles (those
+// of more than 16 rows, the others here) they took 242 + 108. The first tile's loads go ahead of the queries', which
+// a short context notices (64 keys 10.0 -> 9.8 us).
 #pragma once
 
 #include "attn_common.hpp"
@@ -92,6 +98,54 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, attn_few_row_per_cu<A>(DP)) 
         const long long part = whole ? -1 : (2ll * wg + (unit0 == 0)) * kRows;
         const int32_t *table = a.table + b * a.ld_table;
         const C *kbase = static_cast<const C *>(a.k), *vbase = static_cast<const C *>(a.v);
+        // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
+        u32x4 kx[2][kPieces], vx[2][kPieces];
+        float sk = 0.0f, sv = 0.0f;  // int8: the scales of key lane % 32
+        PageAsked asked[2];
+        bool kept[2];
+        auto ask = [&](int j) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                asked[t] = attn_ask_page(a, table, j + 16 * t + col, hi);
+            }
+        };
+        auto fetch = [&]() {
+            const C *zeros = reinterpret_cast<const C *>(kAttnZeros);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const KeyRow r = attn_key(a, asked[t], kvh);
+                kept[t] = r.kept;
+                const C *kp = (r.kept ? kbase + r.at : zeros) + g * kElems;
+                const C *vp = (r.kept ? vbase + r.at : zeros) + g * kElems;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int d0 = 4 * i * kElems;
+                    const bool in = kFull || d0 + g * kElems < a.head_dim;
+                    kx[t][i] = *reinterpret_cast<const u32x4 *>(in ? kp + d0 : zeros);
+                    vx[t][i] = *reinterpret_cast<const u32x4 *>(in ? vp + d0 : zeros);
+                }
+                if constexpr (kQuant) {
+                    if (t == ((lane >> 4) & 1)) {
+                        const long long at =
+                            (static_cast<long long>(r.kept ? r.page : 0) * a.kv_heads + kvh) * a.page.d + r.offset;
+                        sk = r.kept ? a.scale_k[at] : 0.0f;
+                        sv = r.kept ? a.scale_v[at] : 0.0f;
+                    }
+                }
+            }
+        };
+
+        int j0 = lo + 32 * wave;
+        auto first_tile = [&]() {
+            if (j0 < hi) {
+                ask(j0);
+                fetch();
+                ask(j0 + kAttnFewRowUnit);
+            }
+        };
+        if constexpr (kTree) {
+            first_tile();
+        }
         // this lane's rows, 16 c + col, and the keys that they see
         uint32_t head_in_group;
         int token[kCols], row_lo[kCols], row_hi[kCols];
@@ -143,48 +197,8 @@ __global__ __launch_bounds__(64 * kAttnFewRowWaves, attn_few_row_per_cu<A>(DP)) 
             l[c] = 0.0f;
         }
 
-        // a tile's rows: this lane's are keys col and 16 + col; their pages are asked for a tile ahead
-        u32x4 kx[2][kPieces], vx[2][kPieces];
-        float sk = 0.0f, sv = 0.0f;  // int8: the scales of key lane % 32
-        PageAsked asked[2];
-        bool kept[2];
-        auto ask = [&](int j) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                asked[t] = attn_ask_page(a, table, j + 16 * t + col, hi);
-            }
-        };
-        auto fetch = [&]() {
-            const C *zeros = reinterpret_cast<const C *>(kAttnZeros);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const KeyRow r = attn_key(a, asked[t], kvh);
-                kept[t] = r.kept;
-                const C *kp = (r.kept ? kbase + r.at : zeros) + g * kElems;
-                const C *vp = (r.kept ? vbase + r.at : zeros) + g * kElems;
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int d0 = 4 * i * kElems;
-                    const bool in = kFull || d0 + g * kElems < a.head_dim;
-                    kx[t][i] = *reinterpret_cast<const u32x4 *>(in ? kp + d0 : zeros);
-                    vx[t][i] = *reinterpret_cast<const u32x4 *>(in ? vp + d0 : zeros);
-                }
-                if constexpr (kQuant) {
-                    if (t == ((lane >> 4) & 1)) {
-                        const long long at =
-                            (static_cast<long long>(r.kept ? r.page : 0) * a.kv_heads + kvh) * a.page.d + r.offset;
-                        sk = r.kept ? a.scale_k[at] : 0.0f;
-                        sv = r.kept ? a.scale_v[at] : 0.0f;
-                    }
-                }
-            }
-        };
-
-        int j0 = lo + 32 * wave;
-        if (j0 < hi) {
-            ask(j0);
-            fetch();
-            ask(j0 + kAttnFewRowUnit);
+        if constexpr (!kTree) {
+            first_tile();
         }
         for (; j0 < hi; j0 += kAttnFewRowUnit) {
             // S^T

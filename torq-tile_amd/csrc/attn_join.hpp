@@ -72,7 +72,7 @@ __device__ __forceinline__ JoinRow join_row(const A &a, int few, int each, int a
         const AttnKeys keys = attn_tile_keys(a, s, r / a.tile_rows, a.tile_rows);
         j.parts = attn_splits(keys.first, keys.last, a.tile_chunk);
         j.step = static_cast<long long>(a.q_tokens) * a.q_heads;
-        j.part0 = 2ll * a.few_workgroups * attn_few_rows<A>(a.head_dim) + static_cast<long long>(j.token) * a.q_heads + head;
+        j.part0 = attn_few_parts(a) + static_cast<long long>(j.token) * a.q_heads + head;
         j.part1 = j.part0 + j.step;
     } else {
         before += kvh * units;

@@ -133,6 +133,7 @@ struct AttnPlan
 {
     bool run_few, run_tile;
     int few_workgroups;    // 0: no few-row kernel
+    bool few_whole;        // keys of a sequence and key head are not split
     bool few_many;         // parts for a row of the few-row kernel
     long long few_tokens;  // of a sequence of the few-row kernel, at most
     long long tiles;
@@ -158,8 +159,9 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
     if (plan.run_few) {
         const long long heads = static_cast<long long>(p->batch) * p->kv.kv_heads;
         const long long span = attn_span(mask_bits > 0 ? mask_bits + 1 : plan.few_tokens, p->max_kv_len, window);
+        plan.few_whole = mask_bits > 0 && span <= attn_tree_whole(heads);
         plan.few_workgroups = attn_few_row_workgroups(
-            heads * std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit),
+            heads * (plan.few_whole ? 1 : std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit)),
             mask_bits > 0 ? attn_few_row_per_cu<AttnTreeArgs>(head_dim) : attn_few_row_per_cu<AttnArgs>(head_dim));
         plan.few_many = plan.few_workgroups > heads * kAttnJoinManyParts;
     }
@@ -171,7 +173,7 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
                                           p->max_kv_len, window),
                                 static_cast<long long>(p->kv.head_dim),
                                 static_cast<long long>(p->q_tokens * p->q_heads));
-    plan.parts = 2ll * plan.few_workgroups * few_rows;
+    plan.parts = plan.few_whole ? 0 : 2ll * plan.few_workgroups * few_rows;
     if (plan.run_tile && plan.tile.splits > 1) {
         plan.parts += plan.tile.splits * static_cast<long long>(p->q_tokens) * p->q_heads;
     }
@@ -259,8 +261,9 @@ void launch_attn(A a, const AttnPlan &plan, const tqt_attn_paged_params *p, hipS
     }
     constexpr bool kQuant = std::is_same<C, int8_t>::value;
     const bool join_tile = plan.run_tile && plan.tile.splits > 1;
-    if (plan.few_workgroups > 1 || join_tile) {
-        const int each = static_cast<int>(plan.few_tokens), few = plan.run_few ? a.batch * each : 0;
+    const bool join_few = plan.few_workgroups > 1 && !plan.few_whole;
+    if (join_few || join_tile) {
+        const int each = static_cast<int>(plan.few_tokens), few = join_few ? a.batch * each : 0;
         const int rows = few + (join_tile ? a.q_tokens : 0);
         if (plan.few_many || plan.tile.splits > kAttnJoinManyParts) {
             hipLaunchKernelGGL((attn_join_many_kernel<T, kQuant, A>), dim3(static_cast<unsigned>(rows) * a.q_heads),
@@ -309,7 +312,9 @@ bool run_attn_tree(const tqt_attn_tree_params *p, hipStream_t stream, const char
     a.causal = 0;
     a.mask = p->mask;
     a.ld_mask = static_cast<int>(p->ld_mask);
-    launch_attn<T, C>(a, attn_plan(&p->attn, 32 * static_cast<long long>(p->ld_mask)), &p->attn, stream, where);
+    const AttnPlan plan = attn_plan(&p->attn, 32 * static_cast<long long>(p->ld_mask));
+    a.few_unit = plan.few_whole ? 1 << 30 : kAttnFewRowUnit;
+    launch_attn<T, C>(a, plan, &p->attn, stream, where);
     return true;
 }
 

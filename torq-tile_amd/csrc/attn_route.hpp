@@ -43,6 +43,15 @@ inline int attn_few_row_workgroups(long long units, int per_cu)
     return static_cast<int>(std::max(1ll, std::min(units, 256ll * per_cu)));
 }
 
+// With trees, spans of so many keys at most are not split where a batch has so many (sequence, key head) pairs: a
+// workgroup takes all keys of one, and no join follows. (7 tokens of 32 / 8 heads of 128, us whole and split: one
+// sequence of 200 keys 13.1, 14.4, of 400 17.4, 14.6; 8 of 1000 23.9, 24.7, of 1500 31, 28; 32 of 2000 42, 55, of 4000
+// 87, 91; 128 of 2000 187, 205, of 4000 340, 329.)
+inline long long attn_tree_whole(long long pairs)
+{
+    return std::min(2048ll, std::max(256ll, 16 * pairs));
+}
+
 // Whether the join of the few-row kernel's parts takes four waves for a row instead of one: at more parts
 // than so many.
 constexpr int kAttnJoinManyParts = 16;

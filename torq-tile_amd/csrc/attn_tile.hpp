@@ -645,7 +645,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
     }
     l += __shfl_xor(l, 32);
     const long long part = splits == 1 ? -1
-                                       : 2ll * a.few_workgroups * attn_few_rows<A>(a.head_dim) +
+                                       : attn_few_parts(a) +
                                              (static_cast<long long>(split) * a.q_tokens + s.first + token) *
                                                  a.q_heads +
                                              head;
