@@ -180,7 +180,7 @@ KEEPS = ["kv_keep_" + k for k in ("f16", "bf16", "qsi8dx")]
     dict(q_start=None), dict(kv_len=None), dict(keep=None), dict(keep_len=None), dict(block_table=None),
     dict(batch=2 ** 16), dict(layers=2 ** 16), dict(max_keep=2 ** 31, ld_keep=2 ** 31), dict(ld_table=2 ** 31),
     dict(max_keep=5), dict(layer_stride=8193), dict(kv_len_out=8192), dict(kv_len_out=8200), dict(kv_len_out=8184),
-    dict(batch=2 ** 15, layers=2 ** 15)])
+    dict(batch=2 ** 15, layers=2 ** 15), dict(slots=4096, tokens=2 ** 31)])
 def test_keep_refusals(change):
     for name in KEEPS:
         assert H.refusal(name, keep_params()) is None
@@ -190,7 +190,8 @@ def test_keep_refusals(change):
 def test_keep_takes():
     for name in KEEPS:
         for change in (dict(batch=0, q_start=None), dict(layers=0, kv_len=None), dict(kv_len_out=None),
-                       dict(max_keep=0, keep=None), dict(layers=1, layer_stride=3), dict(kv_len_out=8204)):
+                       dict(max_keep=0, keep=None), dict(layers=1, layer_stride=3), dict(kv_len_out=8204),
+                       dict(slots=4096, tokens=7), dict(slots=None, tokens=2 ** 31)):
             assert H.refusal(name, H.changed(keep_params, **change)) is None, (name, change)
 
 
@@ -206,13 +207,28 @@ TREES = ["attn_tree_" + k for k in H.ATTNS]
     dict(Q=None), dict(D=None), dict(q_start=None), dict(kv_len=None), dict(block_table=None), dict(q_heads=5),
     dict(max_kv_len=65), dict(Q=4104), dict(D=4100), dict(q_token_stride=260), dict(d_head_stride=65),
     dict(scale=NAN), dict(scale=INF), dict(causal=0), dict(causal=2), dict(batch=2 ** 24),
-    dict(q_tokens=2 ** 31), dict(workspace=None), dict(workspace=4100), dict(workspace_size=0)]) + [
+    dict(q_tokens=2 ** 31)]) + [
     dict(mask=None), dict(ld_mask=0), dict(ld_mask=2 ** 25), dict(attn__max_q_len=33)])
 def test_tree_refusals(change):
     base = lambda: H.changed(tree_params, attn__max_kv_len=64, attn__batch=2)  # noqa: E731
     for name in TREES:
         assert H.refusal(name, base()) is None
         assert H.refusal(name, H.changed(base, **change)), name
+
+
+@pytest.mark.parametrize("change", inside("attn", [dict(workspace=None), dict(workspace=4100),
+                                                   dict(workspace_size=0)]))
+def test_tree_workspace(change):
+    """Keys that are split need a workspace; spans that one workgroup takes whole need none."""
+    long = lambda: H.changed(tree_params, attn__max_kv_len=2 ** 16, attn__ld_table=2 ** 12)  # noqa: E731
+    short = lambda: H.changed(tree_params, attn__max_kv_len=64)  # noqa: E731
+    _, lib = R.binding()
+    size = lib.op("attn_tree", "get_workspace_size")
+    assert size(ctypes.byref(long())) > 0 and size(ctypes.byref(short())) == 0
+    for name in TREES:
+        assert H.refusal(name, long()) is None
+        assert H.refusal(name, H.changed(long, **change)), name
+        assert H.refusal(name, H.changed(short, **change)) is None, name
 
 
 def test_tree_takes():

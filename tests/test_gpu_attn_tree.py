@@ -339,6 +339,23 @@ def test_graph_replay_with_changing_lengths_and_trees(gpu, lengths):
         c.check()
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_two_at_once(gpu, name):
+    """Calls on streams of their own, with parts in workspaces of their own."""
+    import torch
+
+    both = [Tree(name, [(5, 1500), (3, 700)], 4, 2, 64), Tree(name, [(40, 1200), (20, 900)], 4, 2, 64)]
+    params, streams = [c.params() for c in both], [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for p, s in zip(params, streams):
+            D.run("attn_tree_" + name, p, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c in both:
+        assert c.size > 0
+        c.check()
+
+
 def test_nothing_to_do(gpu):
     mod, lib = R.binding()
     run = lib.op("attn_tree_f16_f16", "run")

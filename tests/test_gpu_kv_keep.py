@@ -131,6 +131,34 @@ def test_pages_not_kept(gpu, kind):
     c.check()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_sequences_that_brought_nothing(gpu, kind):
+    """With slots: a first row without one leaves its sequence as it is, whatever its list names; rows past the slots
+    are none."""
+    lengths = [(7, 50), (5, 23), (0, 12), (6, 40), (4, 3), (9, 33), (3, 20)]
+    keep = [[0, 2, 5], [1, 3], [], [2, 4, 5], [0, 1], [8], [1, 2]]
+    c = Keep(kind, lengths, keep, layers=2)
+    starts = np.concatenate(([0], np.cumsum([q for q, _ in lengths])))
+    tokens = int(starts[6])  # the last sequence's rows are past the buffer
+    slots = np.arange(tokens, dtype=np.int64)
+    slots[starts[0] + 1] = slots[starts[0] + 3] = -1  # rows past the first do not matter
+    out = [1, 3, 4, 6]
+    for b in (1, 3, 4):
+        slots[starts[b]] = -1
+    c.lengths = [(0, n) if b in out else (q, n) for b, (q, n) in enumerate(lengths)]
+    want, kv_len = c.want()
+    assert [kv_len[b] for b in out] == [23, 40, 3, 20]
+    c.lengths = lengths
+    p = c.params()
+    dev = R.dev(slots)
+    p.slots, p.tokens = R.ptr(dev), tokens
+    D.run("kv_keep_" + kind, p)
+    for x, y in zip(c.c + c.s, want):
+        if x is not None:
+            np.testing.assert_array_equal(c.rows(x), y)
+    assert c.out.tolist() == kv_len + [77]
+
+
 def test_longer_than_the_table(gpu):
     """A kv_len past the block table counts as its end."""
     c = Keep("f16", [(6, 30)], [[1, 3, 5]])
@@ -182,6 +210,25 @@ def test_replayed_as_lists_change(gpu):
         torch.cuda.synchronize()
         np.testing.assert_array_equal(c.rows(c.c[0]), want[0])
         np.testing.assert_array_equal(c.rows(c.c[1]), want[1])
+        assert c.out.tolist() == kv_len + [77]
+
+
+def test_two_at_once(gpu):
+    """Calls of two caches on streams of their own."""
+    import torch
+
+    both = [Keep("f16", [(20, 60)] * 40, [[1, 4, 9, 15]] * 40), Keep("qsi8dx", [(30, 95)] * 30, [[0, 2, 29]] * 30)]
+    want = [c.want() for c in both]
+    params = [c.params() for c in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for c, p, s in zip(both, params, streams):
+        D.run("kv_keep_" + c.kind, p, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, (rows, kv_len) in zip(both, want):
+        for x, y in zip(c.c + c.s, rows):
+            if x is not None:
+                np.testing.assert_array_equal(c.rows(x), y)
         assert c.out.tolist() == kv_len + [77]
 
 

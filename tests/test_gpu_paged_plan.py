@@ -196,6 +196,22 @@ def test_parents_that_are_none(gpu):
     Plan([7, 3], [5, 9], 4, parent=np.append(parent, [7, 7, 7]), tokens=13).check()
 
 
+def test_two_at_once(gpu):
+    """Calls on streams of their own: one launch each, and two."""
+    import torch
+
+    rng = np.random.default_rng(8)
+    plans = [Plan(*random_step(rng, batch, new, 300), 16, spare=4000, seed=batch)
+             for batch, new in ((90, 20), (200, 40), (90, 20), (200, 40))]
+    params, streams = [c.params() for c in plans], [torch.cuda.Stream() for _ in plans]
+    torch.cuda.synchronize()
+    for p, s in zip(params, streams):
+        D.run("paged_plan", p, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, p in zip(plans, params):
+        c.check(p=p)
+
+
 def test_replayed_with_changing_lengths(gpu):
     """A captured step whose lengths, held pages and stack are its own outputs, over several replays."""
     import torch

@@ -365,6 +365,8 @@ class KVKeepParams(ctypes.Structure):
         ("layer_stride", c_size),
         ("scale_layer_stride", c_size),
         ("kv", PagedKV),
+        ("slots", c_vp),
+        ("tokens", c_size),
     ]
 
 
