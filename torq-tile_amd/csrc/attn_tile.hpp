@@ -16,6 +16,12 @@
 // scales stand beside the exponentials (prompts of 4096 at d 64 / 128 / 256: 165 / 220 / 514 us, 106 / 168 / 360
 // over 16-bit caches).
 //
+// Trees: tiles over the context see all of it and are as any other; those that the mask reaches read its words, a
+// row's 64 bits a tile. 16 trees of 26 to 62 tokens over 4096-16384 keys (int8, 32 / 8 heads of 128) take 390-414 us and
+// 10 of join, 0.17 of the matrix cores' cycles and 0.31 of the vector issue: lengths differ, so that half of the wave
+// slots stand empty (16 sequences of 8192 each 292 us, 32 of 4096, whose keys are not split, 251), and 2796 rows fill
+// 3712.
+//
 // LDS layout of a tile: [key / 16][piece / 4][key % 16][4 pieces of 16 bytes], so that each lane of the 1 KB load
 // that fills one [16][4] block has the same key in all of its loads, and looks up one page per tile. A key's
 // pieces are at piece ^ f(key), f = 2 bit1(key) + bit2(key): the 8 keys that a 16-byte read of K takes at a

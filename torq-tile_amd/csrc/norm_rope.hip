@@ -6,6 +6,9 @@
 // Bound by memory: x and dy are read once, dx is written once. The two sums of a head, x^2 and f u x, meet in one
 // butterfly over its threads. A workgroup goes over every so many-th head, so that a thread keeps its 16 elements
 // and their share of dweight stays in its registers; the workgroups' shares are joined in order by a second launch.
+// 4099 tokens of 32 bf16 heads of 128 (101 MB) take 22.9-23.9 us, 4.2-4.4 TB/s, and 1.8-3.6 of join. Heads off the
+// 16-element grid (a rotary_dim that is no multiple of 16 too) take a wave each, with loads of one element a lane: 2000
+// tokens of 32 f32 heads of 80, 40 turned, 110 us forward and back.
 #include "rope_rows.hpp"
 
 namespace tqt {
