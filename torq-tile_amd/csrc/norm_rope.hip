@@ -6,7 +6,8 @@
 // Bound by memory: x and dy are read once, dx is written once. The two sums of a head, x^2 and f u x, meet in one
 // butterfly over its threads. A workgroup goes over every so many-th head, so that a thread keeps its 16 elements
 // and their share of dweight stays in its registers; the workgroups' shares are joined in order by a second launch.
-// 4099 tokens of 32 bf16 heads of 128 (101 MB) take 22.9-23.9 us, 4.2-4.4 TB/s, and 1.8-3.6 of join. Heads off the
+// 4099 tokens of 32 bf16 heads of 128 (101 MB) take 22.8-23.9 us, 4.2-4.4 TB/s, and 3 of join; loads a step ahead of
+// their use gained 0.6 and cost 2.5 with f32 rows (registers), 512, 768 or 2048 workgroups took 1-4 more. Heads off the
 // 16-element grid (a rotary_dim that is no multiple of 16 too) take a wave each, with loads of one element a lane: 2000
 // tokens of 32 f32 heads of 80, 40 turned, 110 us forward and back.
 #include "rope_rows.hpp"
@@ -210,9 +211,18 @@ __global__ __launch_bounds__(256) void norm_grad_join_kernel(const float *part, 
     const int e = blockIdx.x * 4 + (threadIdx.x & 3), at = threadIdx.x >> 2;
     double sum = 0.0;
     if (e < head_dim) {
-#pragma unroll 16
-        for (int i = at; i < parts; i += 64) {
-            sum += part[static_cast<long long>(i) * head_dim + e];
+        // 16 loads in flight whatever `parts` is: past the end they are the last share's (with a remainder's one by
+        // one, the gradient of 500, 1000 tokens of 32 heads of 128 took 11.8, 17.2 us, now 10.0, 13.3)
+        for (int i = at; i < parts; i += 64 * 16) {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[j] = part[static_cast<long long>(min(i + 64 * j, parts - 1)) * head_dim + e];
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                sum += i + 64 * j < parts ? x[j] : 0.0f;
+            }
         }
     }
     s_sum[at][threadIdx.x & 3] = sum;
