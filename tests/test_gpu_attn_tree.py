@@ -339,6 +339,63 @@ def test_graph_replay_with_changing_lengths_and_trees(gpu, lengths):
         c.check()
 
 
+# 8 key heads with two query heads each: 17 to 64 tokens are a tile, so 8 to 16 sequences are 64 to 128 workgroups, whose
+# keys are cut into equal spans of each sequence's own
+EVEN = [[(40, 2000), (33, 500), (64, 1400), (20, 64), (17, 17), (50, 900), (5, 700), (0, 30), (30, 1100), (64, 64), (21, 0)],
+        [(30, 1500)] * 9, [(17 + 5 * i, 40 + 131 * i) for i in range(10)], [(65, 1800), (100, 130), (128, 1300), (70, 71)]]
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("lengths", EVEN)
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (144, 0), (64, 150)])
+def test_spans_of_each_sequence(gpu, name, lengths, d, window):
+    kv = {"max_kv": 6000} if window == 0 else {}
+    c = Tree(name, lengths, 16, 8, d, window=window)
+    per = -(-6000 // c.page)
+    if kv:  # the bound is far above the lengths; the table has to hold it
+        wide = np.zeros((len(lengths), per), np.int32)
+        wide[:, :c.table.shape[1]] = c.table
+        c.table = wide
+    c.run(**kv).check()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_spans_of_a_round(gpu, name):
+    """Half a round of workgroups and more (64 sequences of one tile, 8 key heads), and one length over all others."""
+    lengths = [(17 + b % 40, 17 + b % 40 + 5 * b) for b in range(62)] + [(40, 4100), (3, 900)]
+    c = Tree(name, lengths, 16, 8, 64)
+    wide = np.zeros((len(lengths), 8200 // c.page + 1), np.int32)
+    wide[:, :c.table.shape[1]] = c.table
+    c.table = wide
+    c.run(max_kv=8200).check()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_spans_replayed_as_lengths_change(gpu, name):
+    """One graph, eager calls between its replays: equal lengths, one long one, short ones, the bounds' own."""
+    import torch
+
+    longest = [(64, 3000)] * 10
+    c = Tree(name, longest, 16, 8, 64)
+    p = c.params(max_kv=3000)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        D.run("attn_tree_" + name, p, torch.cuda.current_stream().cuda_stream)
+    q_len = [q for q, _ in longest]
+    for lengths in (longest, [(64, 3000)] + [(64, 70)] * 9, [(64, 64 + 300 * b) for b in range(10)], [(64, 64)] * 10):
+        assert [q for q, _ in lengths] == q_len
+        c.lengths = lengths
+        c.args[1].copy_(R.dev(np.array([n for _, n in lengths], np.int32)))
+        for replay in range(2):
+            c.out.fill_(9.0)
+            if replay:
+                D.run("attn_tree_" + name, p)
+            graph.replay()
+            torch.cuda.synchronize()
+            c.check()
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_two_at_once(gpu, name):
     """Calls on streams of their own, with parts in workspaces of their own."""

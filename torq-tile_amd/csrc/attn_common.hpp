@@ -50,7 +50,21 @@ struct AttnTreeArgs : AttnArgs
     const uint32_t *mask;
     int ld_mask;
     int few_unit;  // keys of the few-row kernel's units: kAttnFewRowUnit, or all of a sequence's
+    // Tiles in equal spans (attn_even_parts; 0: none), of even_least keys to even_most, a multiple of 64, for even_round
+    // workgroups or twice as many; each sequence's span goes to even_chunk, where the join finds it.
+    int even_parts, even_least, even_most, even_round;
+    int *even_chunk;  // [64]
 };
+
+// Keys that a workgroup of the tile kernel takes of a sequence, for the join.
+__device__ __forceinline__ int attn_tile_span(const AttnArgs &a, int)
+{
+    return a.tile_chunk;
+}
+__device__ __forceinline__ int attn_tile_span(const AttnTreeArgs &a, int b)
+{
+    return a.even_parts > 0 ? a.even_chunk[b] : a.tile_chunk;
+}
 
 // Keys of the few-row kernel's units.
 __device__ __forceinline__ int attn_few_unit(const AttnArgs &)

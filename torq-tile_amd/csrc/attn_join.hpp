@@ -31,10 +31,9 @@ __device__ __forceinline__ JoinRow join_row(const A &a, int few, int each, int a
     const int heads = static_cast<int>(a.group.d);
     const bool tiles = at_row >= few;
     AttnSeq s;
-    int token, units = 0, run = 1, before = 0;
+    int token, units = 0, run = 1, before = 0, b = -1;
     if (tiles) {
         token = at_row - few;
-        int b = -1;
         for (int x0 = 0; x0 < a.batch && b < 0; x0 += 64) {
             const int x = x0 + lane;
             const unsigned long long here =
@@ -47,7 +46,7 @@ __device__ __forceinline__ JoinRow join_row(const A &a, int few, int each, int a
         s = attn_seq(a, b);
         token -= s.first;
     } else {
-        const int b = at_row / each;
+        b = at_row / each;
         token = at_row - b * each;
         FewRowBatch batch;
         FewRowWork work;
@@ -70,7 +69,7 @@ __device__ __forceinline__ JoinRow join_row(const A &a, int few, int each, int a
     const int r = token * heads + static_cast<int>(in_group);
     if (tiles) {
         const AttnKeys keys = attn_tile_keys(a, s, r / a.tile_rows, a.tile_rows);
-        j.parts = attn_splits(keys.first, keys.last, a.tile_chunk);
+        j.parts = attn_splits(keys.first, keys.last, attn_tile_span(a, b));
         j.step = static_cast<long long>(a.q_tokens) * a.q_heads;
         j.part0 = attn_few_parts(a) + static_cast<long long>(j.token) * a.q_heads + head;
         j.part1 = j.part0 + j.step;

@@ -138,6 +138,8 @@ struct AttnPlan
     long long few_tokens;  // of a sequence of the few-row kernel, at most
     long long tiles;
     AttnSplit tile;
+    int even_parts;   // trees: attn_even_parts
+    long long span;   // keys that a row sees at most
     long long parts;  // rows of the workspace
 };
 
@@ -174,8 +176,15 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
                                 static_cast<long long>(p->kv.head_dim),
                                 static_cast<long long>(p->q_tokens * p->q_heads));
     plan.parts = plan.few_whole ? 0 : 2ll * plan.few_workgroups * few_rows;
+    const long long rows = static_cast<long long>(p->q_tokens) * p->q_heads;
+    if (plan.run_tile && mask_bits > 0) {
+        plan.span = attn_span(mask_bits + 1, p->max_kv_len, window);
+        plan.even_parts = attn_even_parts(p->batch, plan.tiles * p->kv.kv_heads, plan.tile, plan.span, head_dim, rows);
+        plan.tile.splits = std::max(plan.tile.splits, plan.even_parts);
+    }
     if (plan.run_tile && plan.tile.splits > 1) {
-        plan.parts += plan.tile.splits * static_cast<long long>(p->q_tokens) * p->q_heads;
+        // and 4 rows for the equal spans, 64 whole numbers
+        plan.parts += plan.tile.splits * rows + (plan.even_parts > 0 ? 4 : 0);
     }
     return plan;
 }
@@ -252,7 +261,11 @@ void launch_attn(A a, const AttnPlan &plan, const tqt_attn_paged_params *p, hipS
         check_launch(where);
     }
     if (plan.run_tile) {
-        const dim3 grid(static_cast<unsigned>(plan.tiles * a.kv_heads), plan.tile.splits);
+        dim3 grid(static_cast<unsigned>(plan.tiles * a.kv_heads), plan.tile.splits);
+        if (plan.even_parts > 0) {
+            // at most two rounds, and a workgroup at least for each tile
+            grid = dim3(static_cast<unsigned>(2 * attn_tile_workgroups(a.head_dim) / a.kv_heads * a.kv_heads));
+        }
         by_head_dim<64, 96, 128, 192, 256>(a.head_dim, [&](auto dp, auto full) {
             hipLaunchKernelGGL((attn_tile_kernel<T, C, dp.value, 4, full.value, A>), grid, dim3(256), 0, stream,
                                a);
@@ -314,6 +327,15 @@ bool run_attn_tree(const tqt_attn_tree_params *p, hipStream_t stream, const char
     a.ld_mask = static_cast<int>(p->ld_mask);
     const AttnPlan plan = attn_plan(&p->attn, 32 * static_cast<long long>(p->ld_mask));
     a.few_unit = plan.few_whole ? 1 << 30 : kAttnFewRowUnit;
+    a.even_parts = plan.even_parts;
+    if (plan.even_parts > 0) {
+        const long long longest = plan.span + 63;  // a tile's keys begin at a multiple of 64
+        a.even_round = static_cast<int>(attn_tile_workgroups(a.head_dim));
+        a.even_least = static_cast<int>(std::max<long long>(
+            kAttnTileLeast, ((longest + plan.even_parts - 1) / plan.even_parts + 63) / 64 * 64));
+        a.even_most = static_cast<int>((longest + 127) / 64 * 64);
+        a.even_chunk = reinterpret_cast<int *>(static_cast<float *>(p->attn.workspace) + (plan.parts - 4) * a.head_dim);
+    }
     launch_attn<T, C>(a, plan, &p->attn, stream, where);
     return true;
 }

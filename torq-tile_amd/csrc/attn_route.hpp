@@ -109,6 +109,25 @@ inline AttnSplit attn_tile_split(long long tiles, long long kv_heads, long long 
     return {static_cast<int>(chunk), static_cast<int>(splits)};
 }
 
+// Trees: a batch's lengths differ, spans of one size leave the last of a sequence short, and workgroups are dealt to
+// the chip's engines in turn, so that a slot that falls free early waits. Where two to 64 sequences have a quarter of a
+// round of workgroups to a whole one, every one is cut into equal spans of its own, of about one size in all of them: the
+// smallest that make at most a round, or two rounds where that is shorter by more than kAttnEvenCost keys a workgroup (a
+// round's start, more parts to join). The most parts of a sequence, 0: spans of one size. (26-62 tokens, 32 / 8 heads of
+// 128, int8, ragged, us with spans of one size, equal ones in a round and in two: 16 sequences of up to 16384 keys 416, 338,
+// 301; 12 of 8192 192, 129, 146; 8 of 16384 206, 153, 169; 5 of 9000, 100 tokens, 158, 100, 118; 16 of 8192 each 243, 238,
+// 250; f16: 309, 267, 249; 141, 103, 118; 159, 126, 146; 115, 81, 88; 190, 198, 210. Half a round and more, int8: 32 of
+// up to 16384 710, 610; 24 of 8192 353, 260; 20 of 16384 each 750, 615; 32 of 8192 each 492, 496, of 4096 each 222, 239,
+// so from spans of 8192 on.)
+constexpr int kAttnEvenCost = 512;
+inline int attn_even_parts(long long batch, long long whole, const AttnSplit &split, long long span, long long head_dim,
+                           long long rows)
+{
+    const long long want = attn_tile_workgroups(head_dim) / std::max(1ll, whole);
+    const bool gains = split.splits > 1 || (want == 1 && span >= 8192);
+    return gains && batch > 1 && batch <= 64 && want <= 4 && rows <= 1 << 16 ? static_cast<int>(3 * want) : 0;
+}
+
 // The parts and their join are laid out for every row of Q, `rows` (token, query head) pairs, whether a sequence has
 // it or not: q_tokens may be a buffer's. From so many rows on keys are not split, so that the join's grid stays
 // below 2^32 work-items (256 a row). A call of so few tiles that they are split has 2^15 rows of its own at most.

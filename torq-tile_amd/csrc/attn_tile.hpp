@@ -17,10 +17,9 @@
 // over 16-bit caches).
 //
 // Trees: tiles over the context see all of it and are as any other; those that the mask reaches read its words, a
-// row's 64 bits a tile. 16 trees of 26 to 62 tokens over 4096-16384 keys (int8, 32 / 8 heads of 128) take 390-414 us and
-// 10 of join, 0.17 of the matrix cores' cycles and 0.31 of the vector issue: lengths differ, so that half of the wave
-// slots stand empty (16 sequences of 8192 each 292 us, 32 of 4096, whose keys are not split, 251), and 2796 rows fill
-// 3712.
+// row's 64 bits a tile. 16 trees of 26 to 62 tokens over 4096-16384 keys (int8, 32 / 8 heads of 128; 120 GFLOP) take 295-301
+// us, 11 of join among them, in equal spans of each sequence's own (attn_even_parts), 397-416 in spans of one size. A
+// workgroup takes 3.3 us for 64 keys with a CU to itself and 3.9 beside another one, and the 2796 rows fill 3712.
 //
 // LDS layout of a tile: [key / 16][piece / 4][key % 16][4 pieces of 16 bytes], so that each lane of the 1 KB load
 // that fills one [16][4] block has the same key in all of its loads, and looks up one page per tile. A key's
@@ -67,6 +66,68 @@ __device__ __forceinline__ bool attn_find_tile(const AttnArgs &a, int index, int
     return false;
 }
 
+// The work of a workgroup: a tile, and which of its spans of `span` keys.
+__device__ __forceinline__ bool attn_find_work(const AttnArgs &a, int index, int m, int &b, int &tile, int &split,
+                                               int &span, AttnSeq &s)
+{
+    split = blockIdx.y;
+    span = a.tile_chunk;
+    return attn_find_tile(a, index, m, b, tile, s);
+}
+
+// Trees: where even_parts says so, a sequence a lane, with spans of its own. All workgroups come to the same sizes.
+__device__ __forceinline__ bool attn_find_work(const AttnTreeArgs &a, int index, int m, int &b, int &tile, int &split,
+                                               int &span, AttnSeq &s)
+{
+    if (a.even_parts == 0) {
+        return attn_find_work(static_cast<const AttnArgs &>(a), index, m, b, tile, split, span, s);
+    }
+    const int lane = threadIdx.x & 63;
+    const AttnSeq mine = attn_seq(a, lane < a.batch ? lane : 0);
+    const int rows = mine.nq * static_cast<int>(a.group.d);
+    const int tiles = lane < a.batch && rows > a.few_rows ? (rows + m - 1) / m : 0;
+    int keys = 0;
+    if (tiles > 0) {
+        const AttnKeys k = attn_tile_keys(a, mine, 0, m);
+        keys = max(k.last - k.first, 0);
+    }
+    auto parts_of = [&](int most) { return min(max((keys + most - 1) / most, 1), a.even_parts); };
+    // the smallest span, in 64 keys, that makes at most so many workgroups
+    auto least = [&](int workgroups) {
+        int lo = a.even_least >> 6, hi = a.even_most >> 6;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const int n = wave_inclusive_sum(tiles * parts_of(mid << 6), lane, a.batch);
+            if (__builtin_amdgcn_readlane(n, 63) * a.kv_heads <= workgroups) {
+                hi = mid;
+            } else {
+                lo = mid + 1;
+            }
+        }
+        return lo << 6;
+    };
+    const int one = least(a.even_round), two = least(2 * a.even_round);
+    const int parts = parts_of(2 * two + kAttnEvenCost < one ? two : one);
+    const int each = ((keys + parts - 1) / parts + 63) & ~63;
+    const int items = tiles * attn_splits(0, keys, max(each, 64));
+    const int upto = wave_inclusive_sum(items, lane, a.batch);
+    const unsigned long long past = __ballot(upto > index);
+    if (past == 0) {
+        return false;
+    }
+    b = __builtin_ctzll(past);
+    s = attn_pick(mine, b);
+    span = max(__builtin_amdgcn_readlane(each, b), 64);
+    const int n = __builtin_amdgcn_readlane(tiles, b);
+    const int at = index - __builtin_amdgcn_readlane(upto - items, b);
+    split = at / n;
+    tile = n - 1 - (at - split * n);
+    if (threadIdx.x == 0) {
+        a.even_chunk[b] = span;  // the same from all of the sequence's workgroups
+    }
+    return true;
+}
+
 template <typename T, typename C, int DP, int NW, bool kFull, typename A>
 __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn_tile_kernel(A a)
 {
@@ -88,20 +149,20 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
 
     // the key heads of a tile side by side: with 8 (or a multiple), a head's tiles are all on one XCD, whose L2
     // its keys then pass once for them
-    const int split = blockIdx.y, index = static_cast<int>(blockIdx.x) / a.kv_heads;
+    const int index = static_cast<int>(blockIdx.x) / a.kv_heads;
     const int kvh = static_cast<int>(blockIdx.x) - index * a.kv_heads;
-    int b, tile;
+    int b, tile, split, span;
     AttnSeq s;
-    if (!attn_find_tile(a, index, kM, b, tile, s)) {
+    if (!attn_find_work(a, index, kM, b, tile, split, span, s)) {
         return;
     }
     const int group = static_cast<int>(a.group.d);
     const AttnKeys keys = attn_tile_keys(a, s, tile, kM);
-    const int splits = attn_splits(keys.first, keys.last, a.tile_chunk);
+    const int splits = attn_splits(keys.first, keys.last, span);
     if (split >= splits) {
         return;
     }
-    const int lo = keys.first + split * a.tile_chunk, hi = min(keys.last, lo + a.tile_chunk);
+    const int lo = keys.first + split * span, hi = min(keys.last, lo + span);
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
