@@ -91,7 +91,7 @@ __device__ __forceinline__ bool attn_find_work(const AttnTreeArgs &a, int index,
         const AttnKeys k = attn_tile_keys(a, mine, 0, m);
         keys = max(k.last - k.first, 0);
     }
-    auto parts_of = [&](int most) { return min(max((keys + most - 1) / most, 1), a.even_parts); };
+    auto parts_of = [&](int most) { return min((keys - 1) / most + 1, a.even_parts); };
     // the smallest span, in 64 keys, that makes at most so many workgroups
     auto least = [&](int workgroups) {
         int lo = a.even_least >> 6, hi = a.even_most >> 6;
