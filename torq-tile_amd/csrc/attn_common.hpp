@@ -100,6 +100,16 @@ constexpr int attn_few_row_per_cu(int head_dim)
     return head_dim > (std::is_same<A, AttnTreeArgs>::value ? 64 : 128) ? 1 : 2;
 }
 
+// Workgroups of the tile kernel that a CU holds. With trees two at most: at heads of 64 over 16-bit caches the third
+// spills 68 registers (63 tokens of 16 sequences of 8192 keys, 32 / 8 heads, f16, 117 us, 278 with three; 64 of 4096 204,
+// 552; of 1024 62, 126; 20 tokens of 64 of 2000 at most 77, 138).
+template <typename A>
+constexpr int attn_tile_groups(size_t cache_element, int head_dim)
+{
+    const int n = attn_tile_per_cu(cache_element, head_dim);
+    return std::is_same<A, AttnTreeArgs>::value && n > 2 ? 2 : n;
+}
+
 // A sequence of the batch, with every length brought inside what the host checked.
 struct AttnSeq
 {

@@ -129,7 +129,7 @@ __device__ __forceinline__ bool attn_find_work(const AttnTreeArgs &a, int index,
 }
 
 template <typename T, typename C, int DP, int NW, bool kFull, typename A>
-__global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn_tile_kernel(A a)
+__global__ __launch_bounds__(64 * NW, attn_tile_groups<A>(sizeof(C), DP)) void attn_tile_kernel(A a)
 {
     constexpr bool kTree = std::is_same<A, AttnTreeArgs>::value;
     constexpr bool kQuant = std::is_same<C, int8_t>::value;
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(64 * NW, attn_tile_per_cu(sizeof(C), DP)) void attn
             return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
         u32x4 x[2][4];
-        constexpr int kKeys = attn_tile_per_cu(sizeof(C), DP) > 2 ? 2 : 4;
+        constexpr int kKeys = attn_tile_groups<A>(sizeof(C), DP) > 2 ? 2 : 4;
 #pragma unroll
         for (int e = 0; e < kKeys; ++e) {
             x[0][e] = key(e >> 1, e & 1);
