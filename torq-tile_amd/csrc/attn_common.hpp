@@ -93,11 +93,12 @@ constexpr int attn_few_rows(int head_dim)
     return std::is_same<A, AttnTreeArgs>::value ? attn_tree_few_rows(head_dim) : kAttnFewRows;
 }
 
-// Workgroups of the few-row kernel that a CU holds, by their registers.
-template <typename A>
-constexpr int attn_few_row_per_cu(int head_dim)
+// Workgroups of the few-row kernel that a CU holds, by their registers: with two columns of 16 rows one at heads
+// over 64, with one at heads over 128. (Trees of 16 rows over 32 sequences of 4096 keys, int8 heads of 128: one column
+// FIG_A us, two FIG_B.)
+constexpr int attn_few_row_per_cu(int head_dim, int columns)
 {
-    return head_dim > (std::is_same<A, AttnTreeArgs>::value ? 64 : 128) ? 1 : 2;
+    return head_dim > (columns > 1 ? 64 : 128) ? 1 : 2;
 }
 
 // Workgroups of the tile kernel that a CU holds. With trees two at most: at heads of 64 over 16-bit caches the third

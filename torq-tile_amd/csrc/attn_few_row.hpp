@@ -42,11 +42,11 @@ struct FewRowTile
     static constexpr int kWaveBytes = 32 * kStride + (kQuant ? 384 : 0);
 };
 
-template <typename T, typename C, int DP, bool kFull, typename A>
-__global__ __launch_bounds__(64 * kAttnFewRowWaves, attn_few_row_per_cu<A>(DP)) void attn_few_row_kernel(A a)
+template <typename T, typename C, int DP, bool kFull, typename A, int kCols>
+__global__ __launch_bounds__(64 * kAttnFewRowWaves, attn_few_row_per_cu(DP, kCols)) void attn_few_row_kernel(A a)
 {
     constexpr bool kTree = std::is_same<A, AttnTreeArgs>::value;
-    constexpr int kRows = attn_few_rows<A>(DP), kCols = kRows / 16;  // columns of 16 rows
+    constexpr int kRows = attn_few_rows<A>(DP);  // of a part; kCols columns of 16 of them
     typedef FewRowTile<T, C, DP> Tile;
     typedef typename Half8<T>::type half8;
     constexpr bool kQuant = Tile::kQuant;

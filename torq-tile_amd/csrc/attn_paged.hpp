@@ -133,6 +133,7 @@ struct AttnPlan
 {
     bool run_few, run_tile;
     int few_workgroups;    // 0: no few-row kernel
+    int few_columns;       // of 16 rows
     bool few_whole;        // keys of a sequence and key head are not split
     bool few_many;         // parts for a row of the few-row kernel
     long long few_tokens;  // of a sequence of the few-row kernel, at most
@@ -159,12 +160,13 @@ AttnPlan attn_plan(const tqt_attn_paged_params *p, long long mask_bits = 0)
     plan.run_tile = static_cast<long long>(p->max_q_len) * group > few_rows;
     plan.few_tokens = std::min<long long>(p->max_q_len, std::max(1ll, few_rows / group));
     if (plan.run_few) {
+        plan.few_columns = static_cast<long long>(p->max_q_len) * group <= 16 ? 1 : few_rows / 16;
         const long long heads = static_cast<long long>(p->batch) * p->kv.kv_heads;
         const long long span = attn_span(mask_bits > 0 ? mask_bits + 1 : plan.few_tokens, p->max_kv_len, window);
         plan.few_whole = mask_bits > 0 && span <= attn_tree_whole(heads);
         plan.few_workgroups = attn_few_row_workgroups(
             heads * (plan.few_whole ? 1 : std::max(1ll, (span + kAttnFewRowUnit - 1) / kAttnFewRowUnit)),
-            mask_bits > 0 ? attn_few_row_per_cu<AttnTreeArgs>(head_dim) : attn_few_row_per_cu<AttnArgs>(head_dim));
+            attn_few_row_per_cu(head_dim, plan.few_columns));
         plan.few_many = plan.few_workgroups > heads * kAttnJoinManyParts;
     }
     plan.tiles = attn_tiles(p->batch, p->q_tokens, p->max_q_len, group);
@@ -255,8 +257,14 @@ void launch_attn(A a, const AttnPlan &plan, const tqt_attn_paged_params *p, hipS
     a.part_ml = a.part_o + plan.parts * a.head_dim;
     if (plan.run_few) {
         by_head_dim<64, 128, 256>(a.head_dim, [&](auto dp, auto full) {
-            hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value, A>), dim3(plan.few_workgroups),
-                               dim3(64 * kAttnFewRowWaves), 0, stream, a);
+            constexpr int kMost = attn_few_rows<A>(dp.value) / 16;
+            const dim3 grid(plan.few_workgroups), block(64 * kAttnFewRowWaves);
+            if (plan.few_columns < kMost) {
+                hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value, A, 1>), grid, block, 0, stream, a);
+            } else {
+                hipLaunchKernelGGL((attn_few_row_kernel<T, C, dp.value, full.value, A, kMost>), grid, block, 0,
+                                   stream, a);
+            }
         });
         check_launch(where);
     }
