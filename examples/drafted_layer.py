@@ -80,8 +80,8 @@ class Layer:
         mod, stream = self.mod, torch.cuda.current_stream().cuda_stream
         tokens, most = x.shape[0], max(max(new), 1)
         new_len, self.q_start = ints(new), torch.empty(self.batch + 1, dtype=torch.int32, device="cuda")
-        positions = torch.empty(tokens, dtype=torch.int32, device="cuda")
-        slots = self.slots = torch.empty(tokens, dtype=torch.int64, device="cuda")
+        positions = self.positions = torch.empty(tokens, dtype=torch.int32, device="cuda")
+        slots = torch.empty(tokens, dtype=torch.int64, device="cuda")
         mask = torch.empty((tokens, 1), dtype=torch.int32, device="cuda")
         p = mod.PagedPlanParams(
             batch=self.batch, tokens=tokens, page_size=PAGE, num_pages=self.num_pages, new_len=new_len.data_ptr(),
@@ -136,7 +136,8 @@ class Layer:
             batch=self.batch, max_keep=path.shape[1], q_start=self.q_start.data_ptr(),
             kv_len=self.with_drafted.data_ptr(), kv_len_out=self.kv_len.data_ptr(), keep=path.data_ptr(),
             ld_keep=path.stride(0), keep_len=path_len.data_ptr(), block_table=self.blocks.data_ptr(),
-            ld_table=self.per, layers=1, kv=self.kv, slots=self.slots.data_ptr(), tokens=self.slots.numel())
+            ld_table=self.per, layers=1, kv=self.kv, positions=self.positions.data_ptr(),
+            tokens=self.positions.numel())
         self.op("kv_keep_" + ("qsi8dx" if self.int8_cache else "f16"), c, torch.cuda.current_stream().cuda_stream)
 
     def exact(self, x):

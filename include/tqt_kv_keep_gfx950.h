@@ -17,9 +17,12 @@
  * fewer tokens in the cache than drafted ones keeps none, and its kv_len_out is 0. Two sequences may not share a page
  * that holds drafted tokens.
  *
- * slots, where given, are those that the step's rows were appended with, rows 0 to tokens. A sequence whose first
- * drafted row has a negative one (tqt_run_paged_plan_* had no pages for it) brought nothing: its kv_len does not count
- * its drafted tokens, so nothing moves and kv_len_out is kv_len. A step that may refuse sequences gives them.
+ * A step that may refuse sequences (tqt_run_paged_plan_* had no pages for one) gives positions, the plan's for rows 0 to
+ * tokens: a sequence whose first drafted row's position is not below its kv_len, or whose rows begin at tokens or
+ * later, was refused, its kv_len does not count its drafted tokens, and so nothing moves and kv_len_out is kv_len. slots, which
+ * the rows were appended with, may stand for them (they are not read with positions): a sequence was refused whose
+ * drafted rows have negative ones although their tokens' pages are kept. They cannot tell so where none of the last
+ * q_len tokens' pages is one of the cache, and such a sequence counts as served.
  * The function's name gives the cache's type. Conventions as in tqt_rope_gfx950.h, of the cache as in
  * tqt_kv_append_rope_gfx950.h.
  */
@@ -48,8 +51,9 @@ struct tqt_kv_keep_params
     size_t layer_stride;       /* of k and v, in elements */
     size_t scale_layer_stride; /* int8 caches: of scale_k and scale_v */
     struct tqt_paged_kv kv;
-    const int64_t *slots; /* [tokens], or NULL: every sequence was appended */
-    size_t tokens;        /* rows that q_start counts in; not read without slots */
+    const int64_t *slots; /* [tokens], or NULL */
+    size_t tokens;        /* rows that q_start counts in; not read without slots and positions */
+    const int32_t *positions; /* [tokens], or NULL; without slots too every sequence was served */
 };
 
 const char *tqt_get_error_kv_keep_f16_gfx950(const struct tqt_kv_keep_params *params);

@@ -25,6 +25,7 @@ struct KeepArgs
 {
     const int32_t *q_start, *kv_len, *keep, *keep_len, *table;
     const int64_t *slots;
+    const int32_t *positions;
     int32_t *kv_len_out;
     long long ld_keep, ld_table;
     char *k, *v;
@@ -50,6 +51,33 @@ __device__ __forceinline__ KeepPlace keep_place(const KeepArgs &a, const int32_t
     return p;
 }
 
+// Whether a sequence whose q_len > 0 drafted rows begin at `first` was refused: its kv_len does not count them. Its
+// positions say so: those of tokens that kv_len counts are below it. The slots do not always: a refused sequence has
+// none, but a token whose page is no page of the cache has none either, so the first row decides whose token, if
+// it is counted, has a page.
+__device__ __forceinline__ bool keep_refused(const KeepArgs &a, const int32_t *table, int first, int q_len, int kv_len)
+{
+    if (a.positions == nullptr && a.slots == nullptr) {
+        return false;
+    }
+    if (first < 0 || first >= a.tokens) {
+        return true;
+    }
+    if (a.positions != nullptr) {
+        return a.positions[first] >= kv_len;
+    }
+    const int base = min(max(kv_len, 0), a.most_len) - q_len;
+    for (int i = 0; i < q_len && first + i < a.tokens; ++i) {
+        if (a.slots[first + i] >= 0) {
+            return false;
+        }
+        if (base < 0 || keep_place(a, table, base + i).page >= 0) {
+            return true;
+        }
+    }
+    return false;
+}
+
 template <bool kQuant>
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a)
 {
@@ -65,13 +93,13 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a)
     const int b = static_cast<int>(ub);
     const int first = a.q_start[b];
     int q_len = max(a.q_start[b + 1] - first, 0);
+    const int32_t *keep = a.keep + b * a.ld_keep, *table = a.table + b * a.ld_table;
     // one that brought nothing keeps its length, as one without drafted tokens
-    if (a.slots != nullptr && q_len > 0 && (first < 0 || first >= a.tokens || a.slots[first] < 0)) {
+    if (q_len > 0 && keep_refused(a, table, first, q_len, a.kv_len[b])) {
         q_len = 0;
     }
     const int base = min(max(a.kv_len[b], 0), a.most_len) - q_len;
     const int most = base < 0 ? 0 : min(max(a.keep_len[b], 0), a.max_keep);
-    const int32_t *keep = a.keep + b * a.ld_keep, *table = a.table + b * a.ld_table;
     char *rows = (value ? a.v : a.k) + layer * a.layer_bytes + head * a.head_bytes + 16 * piece;
     float *scales = nullptr;
     if constexpr (kQuant) {
@@ -163,7 +191,7 @@ const char *keep_error(const tqt_kv_keep_params *p, size_t bytes, bool quant)
     if (p->kv_len_out != nullptr && p->kv_len_out < p->kv_len + p->batch && p->kv_len < p->kv_len_out + p->batch) {
         return "kv_len_out overlaps kv_len";
     }
-    if (p->slots != nullptr && p->tokens >= top) {
+    if ((p->slots != nullptr || p->positions != nullptr) && p->tokens >= top) {
         return "tokens too large";
     }
     return nullptr;
@@ -190,7 +218,8 @@ bool run_keep(const tqt_kv_keep_params *p, hipStream_t stream, const char *where
     a.table = p->block_table;
     a.kv_len_out = p->kv_len_out;
     a.slots = p->slots;
-    a.tokens = static_cast<int>(p->slots != nullptr ? p->tokens : 0);
+    a.positions = p->positions;
+    a.tokens = static_cast<int>(p->slots != nullptr || p->positions != nullptr ? p->tokens : 0);
     a.ld_keep = static_cast<long long>(p->ld_keep);
     a.ld_table = static_cast<long long>(p->ld_table);
     a.k = static_cast<char *>(c.k);

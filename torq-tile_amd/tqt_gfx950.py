@@ -367,6 +367,7 @@ class KVKeepParams(ctypes.Structure):
         ("kv", PagedKV),
         ("slots", c_vp),
         ("tokens", c_size),
+        ("positions", c_vp),
     ]
 
 
