@@ -185,6 +185,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
     const int first_kv = first_in ? a.kv_len[tid] : 0;
     auto new_len = [&](int b) { return b < kPlanThreads ? first_new : b < a.batch ? a.new_len[b] : 0; };
     auto held_pages = [&](int b) { return b < kPlanThreads ? first_held : b < a.batch ? a.held[b] : 0; };
+    auto kv_tokens = [&](int b) {
+        return min(max(b < kPlanThreads ? first_kv : b < a.batch ? a.kv_len[b] : 0, 0), kPlanMostLen);
+    };
+    // the pages of so many tokens
+    auto pages_of = [&](int n) {
+        uint32_t rest;
+        const long long pages = fast_div(static_cast<uint32_t>(n), a.page, rest);
+        return pages + (rest > 0);
+    };
     if constexpr (kRows) {
         // the way up a tree is a chain of reads
         if (a.parent != nullptr) {
@@ -205,7 +214,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
         const bool on = b0 + 64 * wave < a.batch;
         int held = 0;
         if (on && new_len(b0 + tid) < 0) {
-            held = static_cast<int>(min(max(static_cast<long long>(held_pages(b0 + tid)), 0ll), a.ld_table));
+            held = static_cast<int>(
+                min(max(static_cast<long long>(held_pages(b0 + tid)), pages_of(kv_tokens(b0 + tid))), a.ld_table));
         }
         if (!__syncthreads_or(held > 0)) {
             continue;
@@ -288,17 +298,15 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
             continue;
         }
         const int given = new_len(b), has = held_pages(b);
-        const int kv_len = min(max(b < kPlanThreads ? first_kv : in ? a.kv_len[b] : 0, 0), kPlanMostLen);
+        const int kv_len = kv_tokens(b);
         const bool ended = given < 0;
         const int n = min(max(given, 0), kPlanMostLen);
-        uint32_t rest;
-        const long long own = fast_div(static_cast<uint32_t>(kv_len), a.page, rest) + (rest > 0);
+        const long long own = pages_of(kv_len);
         const long long held = max(min(max(static_cast<long long>(has), 0ll), a.ld_table), own);
         long long need = 0;
         bool fits = in && !ended && kv_len + static_cast<long long>(n) <= kPlanMostLen;
         if (fits) {
-            const long long want = fast_div(static_cast<uint32_t>(kv_len + n), a.page, rest) + (rest > 0);
-            need = max(want - held, 0ll);
+            need = max(pages_of(kv_len + n) - held, 0ll);
             fits = held + need <= a.ld_table;
             need = fits ? need : 0;
         }
