@@ -54,3 +54,27 @@ def test_ended_tables_shorter_than_the_tokens(gpu):
     c.free = np.full(9, -9, np.int32)
     got = outcome(c)
     assert got["free"] == [5, 6, 7, 8] + [-9] * 5 and got["free_count_out"] == [4]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_tables_shorter_than_the_tokens(gpu, in_place):
+    """40 tokens of pages of 4 with a table of 2: refused, new tokens or none, and held is 2; 8 and 7 tokens fit."""
+    c = Plan([3, 0, 1, 1, 0], [40, 40, 8, 7, 8], 4, ld=2, held=[0, 900, 2, 2, 0], spare=3, tokens=7)
+    got = outcome(c, in_place)
+    assert got["refused"] == [3] and got["held_out"] == [2, 2, 2, 2, 2]
+    assert got["kv_len_out"] == [40, 40, 8, 8, 8] and got["free_count_out"] == [3]
+    assert got["q_start"] == [0, 3, 3, 4, 5, 5]
+    page = int(c.table[3, 1])
+    assert got["slots"] == [-1, -1, -1, -1, page * 4 + 3, -1, -1] and got["positions"] == [40, 41, 42, 8, 7, 0, 0]
+    assert got["table"] == c.table.tolist()
+
+
+def test_no_table(gpu):
+    """ld_table 0: nobody holds a page, and only empty sequences that stay so are served."""
+    c = Plan([0, 0, 1, -1], [0, 4, 0, 9], 4, held=[5, 1, 0, 2], spare=3)
+    c.ld = 0
+    p = c.params()
+    p.ld_table = 0
+    D.run("paged_plan", p)
+    assert c.out["held_out"].tolist()[:4] == [0] * 4 and c.out["refused"].tolist()[:1] == [2]
+    assert c.out["kv_len_out"].tolist()[:4] == [0, 4, 0, 0] and c.out["free_count_out"].tolist()[:1] == [3]

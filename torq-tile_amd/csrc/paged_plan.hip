@@ -302,9 +302,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a)
         const bool ended = given < 0;
         const int n = min(max(given, 0), kPlanMostLen);
         const long long own = pages_of(kv_len);
-        const long long held = max(min(max(static_cast<long long>(has), 0ll), a.ld_table), own);
+        const long long held = min(max(static_cast<long long>(has), own), a.ld_table);
         long long need = 0;
-        bool fits = in && !ended && kv_len + static_cast<long long>(n) <= kPlanMostLen;
+        bool fits = in && !ended && own <= a.ld_table && kv_len + static_cast<long long>(n) <= kPlanMostLen;
         if (fits) {
             need = max(pages_of(kv_len + n) - held, 0ll);
             fits = held + need <= a.ld_table;
