@@ -27,7 +27,10 @@
  * t / 32) says whether token t is this one or one that it descends from; bits from 32 * ld_mask on are left out,
  * and all others of the row's ld_mask words are 0.
  *
- * kv_len_out, held_out and free_count_out may be kv_len, held and free_count; no other two arrays may overlap.
+ * kv_len_out, held_out and free_count_out may be kv_len, held and free_count; no other two arrays may overlap. A step that
+ * tqt_run_kv_keep_* ends takes another array for kv_len_out, from which that call writes kv_len: in place every drafted
+ * token would count from the next step on. A slot of -1 does not say that its sequence was refused (its page may be none);
+ * that its first row's position is kv_len_out or more does.
  * Lengths count as 0 at least and 2^30 at most (a sequence that would grow past that is refused), held as the pages of
  * kv_len at least and as ld_table at most, free_count as 0 to free_capacity; pages that do not fit on the stack any
  * more are lost. workspace holds at least
