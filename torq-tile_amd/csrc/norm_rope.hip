@@ -46,6 +46,27 @@ __device__ __forceinline__ NormGradHead norm_grad_head(double squares, double pr
     return {static_cast<float>(r), static_cast<float>(products * r / a.head_dim)};
 }
 
+// Turns the 8 pairs of two pieces.
+__device__ __forceinline__ void turn8(bool interleaved, f32x8 c, f32x8 s, f32x8 &xa, f32x8 &xb)
+{
+    const f32x8 p = xa, q = xb;
+    if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            xa[2 * i] = p[2 * i] * c[i] - p[2 * i + 1] * s[i];
+            xa[2 * i + 1] = p[2 * i + 1] * c[i] + p[2 * i] * s[i];
+            xb[2 * i] = q[2 * i] * c[i + 4] - q[2 * i + 1] * s[i + 4];
+            xb[2 * i + 1] = q[2 * i + 1] * c[i + 4] + q[2 * i] * s[i + 4];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xa[i] = p[i] * c[i] - q[i] * s[i];
+            xb[i] = q[i] * c[i] + p[i] * s[i];
+        }
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kRopeThreads) void norm_grad_rows_kernel(NormGradArgs a)
 {

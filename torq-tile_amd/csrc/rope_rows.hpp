@@ -16,7 +16,8 @@
 // A norm, or an int8 row's maximum, is a sum over a head's threads, a power of two of them side by side: a
 // butterfly of lane moves, whose instructions hide behind the loads (the kernels alone, without and with a norm: 4099
 // tokens of 32 bf16 heads of 128, 64 turned, 15.4 and 15.6-16.7 us; 4096 tokens of 32 + 8 + 8 heads from f32 into an f16
-// cache 23.0-24.5 and 28.5-30.2, 5.1 TB/s). The squares are summed in f64, which costs 4% at most (f32: 48.1 us where a
+// cache 23.0-24.5 and 28.5-30.2, 5.1 TB/s; calls in a row, into an int8 cache from bf16: those 4096 tokens 19.9 and 22.2,
+// 4.2-4.7 TB/s, 1000 of 32 + 32 + 32 heads 11.0 and 13.1). The squares are summed in f64, which costs 4% at most (f32: 48.1 us where a
 // training step's two calls now take 50.1; the append 33.6 and 34.4).
 #pragma once
 
@@ -156,27 +157,6 @@ __device__ __forceinline__ Slot find_slot(const RopeArgs &a, int token)
     return s;
 }
 
-// Turns the 8 pairs of two pieces.
-__device__ __forceinline__ void turn8(bool interleaved, f32x8 c, f32x8 s, f32x8 &xa, f32x8 &xb)
-{
-    const f32x8 p = xa, q = xb;
-    if (interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            xa[2 * i] = p[2 * i] * c[i] - p[2 * i + 1] * s[i];
-            xa[2 * i + 1] = p[2 * i + 1] * c[i] + p[2 * i] * s[i];
-            xb[2 * i] = q[2 * i] * c[i + 4] - q[2 * i + 1] * s[i + 4];
-            xb[2 * i + 1] = q[2 * i + 1] * c[i + 4] + q[2 * i] * s[i + 4];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            xa[i] = p[i] * c[i] - q[i] * s[i];
-            xb[i] = q[i] * c[i] + p[i] * s[i];
-        }
-    }
-}
-
 // One thread: 16 elements of a head. SRC: type of X (or Q, K, V); DST: type of Y; CACHE: the cache's type, void
 // for rope alone; kNorm: heads of Q and K are normalised first.
 template <typename SRC, typename DST, typename CACHE, bool kNorm>
@@ -249,7 +229,25 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a, int
             c = __builtin_nanf("");
             s = c;
         }
-        turn8(a.interleaved, c, s * a.sign, xa, xb);
+        // (as a function, inlined, this takes the int8 instances 70 registers instead of 60 and 7 waves a SIMD instead of
+        // 8: 4096 tokens of 32 + 8 + 8 heads of 128 19.95 instead of 19.85 us, with a norm 22.6 instead of 22.2)
+        s = s * a.sign;
+        const f32x8 p = xa, q = xb;
+        if (a.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xa[2 * i] = p[2 * i] * c[i] - p[2 * i + 1] * s[i];
+                xa[2 * i + 1] = p[2 * i + 1] * c[i] + p[2 * i] * s[i];
+                xb[2 * i] = q[2 * i] * c[i + 4] - q[2 * i + 1] * s[i + 4];
+                xb[2 * i + 1] = q[2 * i + 1] * c[i + 4] + q[2 * i] * s[i + 4];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                xa[i] = p[i] * c[i] - q[i] * s[i];
+                xb[i] = q[i] * c[i] + p[i] * s[i];
+            }
+        }
     }
     QuantRow quant = {1.0f, 1.0f, true, true};
     if constexpr (kQuant) {
