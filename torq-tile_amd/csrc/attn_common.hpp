@@ -94,8 +94,12 @@ constexpr int attn_few_rows(int head_dim)
 }
 
 // Workgroups of the few-row kernel that a CU holds, by their registers: with two columns of 16 rows one at heads
-// over 64, with one at heads over 128. (Trees of 16 rows over 32 sequences of 4096 keys, int8 heads of 128: one column
-// FIG_A us, two FIG_B.)
+// over 64, with one at heads over 128. Calls whose bound is 16 rows take one column. (4 tokens of 32 / 8 heads of 128,
+// us with one column and with two, join included. Int8: one sequence of 8192 keys 18.0, 17.4; 8 of 4096 27.5, 33.5;
+// 32 of 1000 23, 28.5, of 4096 60, 99, of 8192 124, 196; 128 of 4096 235, 414. f16: one sequence of 1000 13.4, 14.3; 8 of 4096
+// 33.2, 34.7; 128 of 200 29, 44, of 4096 386, 390; but 32 of 4096 114, 106, of 8192 213, 198: one workgroup a CU takes a
+// sequence and key head whole there, two take halves that are joined. Heads of 64: 0-10 % less with one, except 32 of
+// 4096 keys and more, 1-6 % more.)
 constexpr int attn_few_row_per_cu(int head_dim, int columns)
 {
     return head_dim > (columns > 1 ? 64 : 128) ? 1 : 2;

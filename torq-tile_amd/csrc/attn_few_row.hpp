@@ -1,5 +1,6 @@
 // Attention of few rows: sequences with at most 16 rows to a key head (one decoded token of up to 16 query
-// heads, or a few tokens of fewer); with trees of new tokens 32, in two columns of the matrix instruction.
+// heads, or a few tokens of fewer); with trees of new tokens 32 (at heads up to 128), in two columns of the matrix
+// instruction, or in one where the call's bound is 16 rows.
 //
 // Bound by the cache's bytes: per key 2 d elements are read once for 4 d 16 flops on the matrix cores. The
 // batch's keys are cut into units of 128 for each key head, and the workgroups that fit the chip at once take
@@ -24,7 +25,9 @@
 // so one wave a SIMD, which still keeps the memory busy: 64 trees of 3-8 tokens over 2048-8192 keys (bf16, 32 / 8
 // heads of 128) take 256-264 us (5.1-5.3 TB/s) and 9 of join; with two waves 91 registers spill, and as tiles (those
 // of more than 16 rows, the others here) they took 242 + 108. The first tile's loads go ahead of the queries', which
-// a short context notices (64 keys 10.0 -> 9.8 us).
+// a short context notices (64 keys 10.0 -> 9.8 us). One column at heads of 128 takes 243 registers (int8 185), so two
+// waves a SIMD: 32 sequences of 4 tokens over 4096 keys, 32 / 8 heads, take 114 us from bf16 caches (4.7 TB/s), 60 from
+// int8 ones (4.6) with the join; 106 and 99 with two columns (attn_few_row_per_cu has more).
 #pragma once
 
 #include "attn_common.hpp"

@@ -46,7 +46,9 @@ inline int attn_few_row_workgroups(long long units, int per_cu)
 // With trees, spans of so many keys at most are not split where a batch has so many (sequence, key head) pairs: a
 // workgroup takes all keys of one, and no join follows. (7 tokens of 32 / 8 heads of 128, us whole and split: one
 // sequence of 200 keys 13.1, 14.4, of 400 17.4, 14.6; 8 of 1000 23.9, 24.7, of 1500 31, 28; 32 of 2000 42, 55, of 4000
-// 87, 91; 128 of 2000 187, 205, of 4000 340, 329.)
+// 87, 91; 128 of 2000 187, 205, of 4000 340, 329. 4 tokens, whose 16 rows are one column, for which the bounds were not
+// chosen, f16: one sequence of 200 9.0, 12.1, of 1000 20, 13.1; 8 of 1000 21, 17; 32 of 1000 28, 32, of 4096 101, 114;
+// 128 of 1000 103, 112, of 4096 377, 388; int8: 8 of 1000 20, 18; 32 of 1000 23, 26, of 4096 75, 61; 128 of 1000 62, 71.)
 inline long long attn_tree_whole(long long pairs)
 {
     return std::min(2048ll, std::max(256ll, 16 * pairs));
