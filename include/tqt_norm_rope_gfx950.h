@@ -16,7 +16,7 @@
  * f32 within a workgroup's share of them and in 64 bits over the workgroups, always in the same order: a call
  * repeated gives the same bits. forward.rope.Y and the Y strides are not used. dX may be dY or X, with the
  * same strides; they may not overlap otherwise. A position outside [0, max_pos) makes NaN of the rotated
- * elements of Y, of the token's dX, and of dweight.
+ * elements of Y and of dweight, and of all of the token's dX.
  *
  * weight is [head_dim] f32 on the device (with the heads' rows on the 16-byte grid, head_dim and rotary_dim
  * multiples of 16, and head_dim up to 1024 the fast calls, if it lies there too). Y may be X, as in
