@@ -25,7 +25,9 @@
  * for one that follows the context (an entry that is not below the row's own number counts as -1). Then the
  * position is kv_len[b] + depth, 0 for tokens that follow the context, and bit t of mask[row] (bit t % 32 of word
  * t / 32) says whether token t is this one or one that it descends from; bits from 32 * ld_mask on are left out,
- * and all others of the row's ld_mask words are 0.
+ * and all others of the row's ld_mask words are 0. A row's tokens are found one from the other, so a long chain takes long
+ * (8 nodes for 63 sequences and for one more a chain of 64: 8.6 us, of 512: 38, of 4096: 417): prompts are better a step
+ * without trees.
  *
  * kv_len_out, held_out and free_count_out may be kv_len, held and free_count; no other two arrays may overlap. A step that
  * tqt_run_kv_keep_* ends takes another array for kv_len_out, from which that call writes kv_len: in place every drafted

@@ -17,8 +17,8 @@
 // butterfly of lane moves, whose instructions hide behind the loads (the kernels alone, without and with a norm: 4099
 // tokens of 32 bf16 heads of 128, 64 turned, 15.4 and 15.6-16.7 us; 4096 tokens of 32 + 8 + 8 heads from f32 into an f16
 // cache 23.0-24.5 and 28.5-30.2, 5.1 TB/s; calls in a row, into an int8 cache from bf16: those 4096 tokens 19.9 and 22.2,
-// 4.2-4.7 TB/s, 1000 of 32 + 32 + 32 heads 11.0 and 13.1). The squares are summed in f64, which costs 4% at most (f32: 48.1 us where a
-// training step's two calls now take 50.1; the append 33.6 and 34.4).
+// 4.2-4.7 TB/s, 1000 of 32 + 32 + 32 heads 11.0 and 13.1). The squares are summed in f64, which costs 4% at most (f32:
+// 48.1 us where a training step's two calls now take 50.1; the append 33.6 and 34.4).
 #pragma once
 
 #include "fast_div.hpp"
